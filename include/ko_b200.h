@@ -163,7 +163,34 @@ int ko_layernorm_f16(const uint16_t *in, uint16_t *out, int64_t rows, int32_t co
                      const uint16_t *gamma, const uint16_t *beta, int ddof, void *stream);
 
 /* ------------------------------------------------------------------------------------------
- * The same operators for a caller whose rows live in HOST memory: `in` is copied to the device,
+ * LayerNorm backward, row-major [rows, cols]: with n = cols, d = n - ddof, xhat = (x - mean) * rstd and
+ * w = dy * gamma (gamma NULL: 1),
+ *     dx     = rstd * (w - sum(w) / n - xhat * sum(w * xhat) / d)  (+ residual when given)
+ *     dgamma = column sums of dy * xhat,  dbeta = column sums of dy
+ * eps and ddof as in the forward call.  mean and rstd are formed again from x, so the forward pass keeps
+ * nothing.  `residual` is the gradient that reaches x past the norm (the skip connection of a pre-norm
+ * block).  FP32 arithmetic; dx is rounded once to the element type; dgamma and dbeta are FP32 [cols],
+ * overwritten, and may each be NULL.  Column sums are added in a fixed order: the same call gives the same
+ * bits.  dx may be the same buffer as dy, x or residual; other overlaps are not allowed.
+ * `workspace`: device memory of ko_layernorm_backward_workspace(...) bytes for this shape (16-byte aligned,
+ * contents irrelevant before and after), used by this call only: calls that may overlap on the GPU, and
+ * captured graphs that may be replayed at the same time, need one each.  Nothing is allocated or kept, so
+ * the call can be captured.  No counterpart in the reference, which has the forward pass only.
+ * ---------------------------------------------------------------------------------------- */
+/* dtype: KO_DTYPE_*; depends on the shape and the current device's SM count; 0 bytes for an empty problem */
+int ko_layernorm_backward_workspace(int dtype, int64_t rows, int32_t cols, size_t *bytes);
+int ko_layernorm_backward_f32(const float *dy, const float *x, float *dx, int64_t rows, int32_t cols,
+                              float eps, const float *gamma, const float *residual, float *dgamma,
+                              float *dbeta, int ddof, void *workspace, size_t workspace_bytes, void *stream);
+int ko_layernorm_backward_f16(const uint16_t *dy, const uint16_t *x, uint16_t *dx, int64_t rows, int32_t cols,
+                              float eps, const uint16_t *gamma, const uint16_t *residual, float *dgamma,
+                              float *dbeta, int ddof, void *workspace, size_t workspace_bytes, void *stream);
+int ko_layernorm_backward_bf16(const uint16_t *dy, const uint16_t *x, uint16_t *dx, int64_t rows, int32_t cols,
+                               float eps, const uint16_t *gamma, const uint16_t *residual, float *dgamma,
+                               float *dbeta, int ddof, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------------------------
+ * The softmax and the LayerNorm forward for a caller whose rows live in HOST memory: `in` is copied to the device,
  * the operator runs and `out` is copied back, cut into `chunks` nominal row ranges (0 = 8, at most 60;
  * from 4 on, the first and last range are each cut further into a quarter, a quarter and a half, so that
  * the stretches in which only one direction of the link is busy are short) that

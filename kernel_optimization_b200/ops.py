@@ -7,6 +7,7 @@ a page-locked host buffer plus a device buffer with copies in both directions.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import numpy as np
 
@@ -147,6 +148,79 @@ def layernorm(x, eps: float, gamma=None, beta=None, ddof: int = 0, out=None, str
     fn = {torch.float32: lib.ko_layernorm_f32, torch.float16: lib.ko_layernorm_f16, torch.bfloat16: lib.ko_layernorm_bf16}[x.dtype]
     native.check(fn(_ptr(x), _ptr(out), rows, cols, eps, _ptr(gamma), _ptr(beta), ddof, s), "ko_layernorm")
     return out
+
+
+def _operand(t, name: str, device, dtypes, shape) -> int | None:
+    """Address of an operand after checking where it lives, its type and its shape (None stays None)."""
+    if t is None:
+        return None
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the operator's first input on {device}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} is {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+    return _ptr(t)
+
+
+def _on(device, stream: int | None):
+    """Context in which `device` and the stream with handle `stream` (None: the device's current one) are current, so that
+    outputs and workspaces come from the pool of the stream that uses them."""
+    import torch
+
+    if device.type != "cuda":
+        raise ValueError("operator inputs must live on a CUDA device (there is no CPU path)")
+    if stream is None:
+        return torch.cuda.device(device)
+    if stream == 0:
+        return torch.cuda.stream(torch.cuda.default_stream(device))
+    return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device))
+
+
+def _workspace(nbytes: int, device):
+    """Device memory for one call: allocated on the current stream, so the caching allocator hands it out again only to work
+    that runs after the call (inside a capture: it belongs to the graph)."""
+    import torch
+
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+@functools.lru_cache(maxsize=4096)
+def _layernorm_backward_bytes(device_index: int, dtype: int, rows: int, cols: int) -> int:
+    n = C.c_size_t()
+    native.check(native.lib().ko_layernorm_backward_workspace(dtype, rows, cols, C.byref(n)), "ko_layernorm_backward_workspace")
+    return n.value
+
+
+def layernorm_backward(dy, x, eps: float, gamma=None, ddof: int = 0, residual=None, dx=None, dgamma=None, dbeta=None,
+                       stream: int | None = None):
+    """Gradients of :func:`layernorm` (same ``eps`` and ``ddof``): ``(dx, dgamma, dbeta)``.
+
+    ``dy``, ``x`` and ``residual`` are 2-D FP32, FP16 or BF16 CUDA tensors of one shape and type, ``gamma`` a vector of that
+    type (None: 1).  The statistics are formed again from ``x``.  ``residual`` is the gradient that reaches ``x`` past the norm
+    (the skip connection of a pre-norm block) and is added to ``dx``.  ``dx`` has the inputs' type and may be ``dy``, ``x`` or
+    ``residual`` itself; ``dgamma`` and ``dbeta`` are FP32.
+    """
+    import torch
+
+    if x.dim() != 2 or x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise ValueError(f"x must be a 2-D FP32, FP16 or BF16 tensor, got {x.dtype} with {x.dim()} dimensions")
+    rows, cols = x.shape
+    same, vector = (x.dtype,), (torch.float32,)
+    lib = native.lib()
+    code, fn = {torch.float32: (DTYPE_F32, lib.ko_layernorm_backward_f32), torch.float16: (DTYPE_F16, lib.ko_layernorm_backward_f16),
+                torch.bfloat16: (DTYPE_BF16, lib.ko_layernorm_backward_bf16)}[x.dtype]
+    with _on(x.device, stream):
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format) if dx is None else dx
+        dgamma = torch.empty(cols, dtype=torch.float32, device=x.device) if dgamma is None else dgamma
+        dbeta = torch.empty(cols, dtype=torch.float32, device=x.device) if dbeta is None else dbeta
+        ws = _workspace(_layernorm_backward_bytes(x.device.index, code, rows, cols), x.device)
+        native.check(fn(_operand(dy, "dy", x.device, same, (rows, cols)), _ptr(x), _operand(dx, "dx", x.device, same, (rows, cols)), rows,
+                        cols, eps, _operand(gamma, "gamma", x.device, same, (cols,)),
+                        _operand(residual, "residual", x.device, same, (rows, cols)),
+                        _operand(dgamma, "dgamma", x.device, vector, (cols,)), _operand(dbeta, "dbeta", x.device, vector, (cols,)), ddof,
+                        _ptr(ws), 0 if ws is None else ws.numel(), _current_stream_ptr()), "ko_layernorm_backward")
+    return dx, dgamma, dbeta
 
 
 def softmax_host(t_in: Tensor, t_out: Tensor, rows: int, cols: int, chunks: int = 0, stream: int | None = None) -> None:
