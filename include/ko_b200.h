@@ -301,6 +301,40 @@ int ko_gemm_tc(int in_fmt, int out_fmt, int b_row_major, int64_t M, int64_t N, i
                const void *A, const void *B, const void *C, void *D, void *stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Linear layer on the tensor cores, forward and backward.  X[M,K] (M tokens), W[N,K], Y[M,N], all row-major,
+ * FP16 or BF16 (in_fmt 0 / 1), products accumulated in FP32:
+ *   ko_linear                  Z = X W^T + bias;  Y = act(Z) + residual
+ *   ko_linear_backward_input   dX = (dY W) * act'(Z)      (Z: what the layer BEFORE put through act, i.e. X = act(Z))
+ *   ko_linear_backward_weight  dW = dY^T X + C;  dbias = column sums of dY
+ * act: KO_ACT_*; act' is taken at the stored, 16-bit Z.  bias[N], residual[M,N], Z[M,N] (forward: an output),
+ * C[N,K] and dbias may be NULL.  bias and Z have the inputs' type; dbias is FP32; residual and Y, dX, C and dW
+ * are FP32 (out_fmt 0) or the inputs' type (out_fmt 1 for FP16, 2 for BF16): the FP32 result is rounded to nearest
+ * even once.  FP32 results use the CUDA library's erfcf / expf; for 16-bit results the activations are accurate to
+ * about 1e-6 absolutely before that rounding.
+ * Row pitches must be multiples of 16 bytes: K % 8 == 0, and N % 8 == 0 in the backward calls (the forward call takes
+ * any N); X, W and dY 16-byte aligned.  Any M: up to 32 tokens the forward call runs a kernel that streams W, beyond
+ * that tiles on tcgen05.  Y may be the residual, dX (16-bit) may be Z, dW may be C; other overlaps are not allowed.
+ * An activation in ko_linear_backward_input needs Z; without one (KO_ACT_NONE) Z is ignored.
+ * `workspace`: as for ko_layernorm_backward_*; ko_linear_*_workspace gives the bytes for a shape (often 0, then it may
+ * be NULL).  Nothing is allocated or kept, every call can be captured.  All sums have a fixed order: the same call
+ * gives the same bits.  No counterpart in the reference, whose GEMM's epilogue adds C at most.
+ * ---------------------------------------------------------------------------------------- */
+enum { KO_ACT_NONE = 0, KO_ACT_RELU = 1, KO_ACT_GELU = 2 /* erf */, KO_ACT_GELU_TANH = 3, KO_ACT_SILU = 4 };
+
+int ko_linear_workspace(int64_t M, int64_t N, int64_t K, size_t *bytes);
+int ko_linear(int in_fmt, int out_fmt, int activation, int64_t M, int64_t N, int64_t K, const void *X,
+              const void *W, const void *bias, const void *residual, void *Y, void *Z, void *workspace,
+              size_t workspace_bytes, void *stream);
+int ko_linear_backward_input_workspace(int64_t M, int64_t N, int64_t K, size_t *bytes);
+int ko_linear_backward_input(int in_fmt, int out_fmt, int activation, int64_t M, int64_t N, int64_t K,
+                             const void *dY, const void *W, const void *Z, void *dX, void *workspace,
+                             size_t workspace_bytes, void *stream);
+int ko_linear_backward_weight_workspace(int64_t M, int64_t N, int64_t K, size_t *bytes);
+int ko_linear_backward_weight(int in_fmt, int out_fmt, int64_t M, int64_t N, int64_t K, const void *dY,
+                              const void *X, const void *C, void *dW, float *dbias, void *workspace,
+                              size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------------------------
  * Probes of the source-level helper templates (kernel_optimization_b200/common/{common,functors}.h
  * and the Welford combiners of nn_operators/layernorm/layernorm.h).  The reference exposes these
  * helpers only as device templates; each probe instantiates them in a small kernel and runs them

@@ -1,4 +1,4 @@
-"""B200 (sm_100a) row softmax / Welford LayerNorm (forward, backward) / SGEMM / tcgen05 GEMM operator set.
+"""B200 (sm_100a) row softmax / Welford LayerNorm (forward, backward) / SGEMM / tcgen05 GEMM / linear layer operator set.
 
 The product is the native library ``lib/libko_b200.so`` (hand-written CUDA behind the C ABI of
 ``include/ko_b200.h``).  This package is the thin Python plumbing around it: a ctypes loader, a
@@ -16,6 +16,9 @@ from .ops import (  # noqa: F401
     layernorm,
     layernorm_backward,
     layernorm_host,
+    linear,
+    linear_backward_input,
+    linear_backward_weight,
     sgemm,
     softmax,
     softmax_host,

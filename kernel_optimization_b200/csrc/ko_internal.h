@@ -29,7 +29,8 @@ int current_device_info(DeviceInfo *out);
 constexpr int kStatusWordCount = 4;
 int device_status_word(int which, unsigned int **out);
 
-inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool aligned_to(const void *p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1u)) == 0; }
+inline bool aligned16(const void *p) { return aligned_to(p, 16); }
 
 }  // namespace ko
 

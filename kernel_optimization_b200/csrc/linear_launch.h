@@ -1,0 +1,156 @@
+// Host side shared by the linear layer's entry points: how a product is cut up, and its launch on the tensor-core kernels.
+#pragma once
+
+#include "ko_internal.h"
+#include "row_launch.h"
+#include "tensor_maps.h"
+
+#include <algorithm>
+#include <map>
+#include <mutex>
+#include <utility>
+
+#include "../nn_operators/gemm/tensor_core_gemm_pair.h"
+#include "../nn_operators/linear/linear_epilogue.h"
+
+namespace ko {
+
+// D[M, N] = A B over K, in 128 x bn tiles of one CTA (K cut into `split` slices), or 256 x 256 tiles of a pair of CTAs
+struct ProductPlan {
+    bool pair;
+    int bn, split;
+    size_t bytes() const { return split > 1 ? (size_t)tiles * split * 128 * bn * sizeof(float) : 0; }
+    long long tiles;
+};
+
+// tma: D can be stored by TMA; without it only the 128 x 128 tile is built.  Modelled microseconds per candidate: start,
+// then rounds of work units x K-blocks of 64 x time per K-block; slices add a second kernel and the partial tiles' way
+// through the L2 (written once, read once).
+inline ProductPlan plan_product(int64_t M, int64_t N, int64_t K, bool tma, int sms) {
+    const long long k_blocks = (K + tc::kBK - 1) / tc::kBK;
+    ProductPlan best{false, 128, 1, 0};
+    double best_cost = 1e300;
+    if (tma && M > 128 && N > 128) {
+        const long long tiles = ((M + 255) / 256) * ((N + 255) / 256);
+        const long long rounds = (tiles + sms / 2 - 1) / (sms / 2);
+        best_cost = 4.0 + (double)rounds * (double)k_blocks * 0.35;
+        best = {true, 256, 1, tiles};
+    }
+    for (int bn : {128, 256}) {
+        if (bn == 256 && (!tma || N <= 128)) continue;
+        const long long tiles = ((M + 127) / 128) * ((N + bn - 1) / bn);
+        const long long most = std::min<long long>(std::max<long long>(sms / tiles, 1), std::max<long long>(k_blocks / 4, 1));
+        for (int split = 1; split <= most && split <= 64; ++split) {
+            const long long rounds = (tiles * split + sms - 1) / sms;
+            double cost = 3.3 + (double)rounds * (double)((k_blocks + split - 1) / split) * (bn == 256 ? 0.31 : 0.26);
+            if (split > 1) cost += 3.0 + (2.0 * split + 1.0) * (double)M * (double)N * 4.0 / 5e6;
+            if (cost < best_cost) {
+                best_cost = cost;
+                best = {false, bn, split, tiles};
+            }
+        }
+    }
+    return best;
+}
+
+// room for either way a call may store D
+inline size_t product_workspace(int64_t M, int64_t N, int64_t K, int sms) {
+    if (M == 0 || N == 0 || K == 0) return 0;
+    return std::max(plan_product(M, N, K, true, sms).bytes(), plan_product(M, N, K, false, sms).bytes());
+}
+
+// clusters of two CTAs of a pair kernel that the current device holds at once (cached per kernel and device)
+inline int resident_pairs_of(const void *kernel, unsigned threads, size_t smem, int *out) {
+    static std::mutex mu;
+    static std::map<std::pair<const void *, int>, int> cached;
+    int dev = 0;
+    KO_CUDA(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> lock(mu);
+    int &n = cached[{kernel, dev}];
+    if (n == 0) {
+        int fresh = 0;
+        if (int st = max_resident_clusters(kernel, threads, 2, smem, &fresh)) return st;
+        n = fresh;
+    }
+    *out = n;
+    return KO_OK;
+}
+
+template <class Epi, int BN, bool kTmaStore>
+int launch_product_tile(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &md, const LinearParams &p, int sms, cudaStream_t s) {
+    using Cfg = tc::TileConfig<BN>;
+    auto kernel = tc::gemm_tcgen05_kernel<BN, kTmaStore, 1, 2, Epi>;
+    if (int st = ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), Cfg::kSmemBytes)) return st;
+    const long long units = (long long)((p.M + 127) / 128) * ((p.N + BN - 1) / BN) * p.split_k;
+    return launch_overlapped(kernel, (unsigned)std::min<long long>(units, sms), 64u + 32u * Epi::kWarps, (size_t)Cfg::kSmemBytes, s, ma, mb, mb, md, p);
+}
+
+template <class Epi>
+int launch_product_pair(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &md, const LinearParams &p, cudaStream_t s) {
+    using Cfg = tc::PairConfig;
+    auto kernel = tc::gemm_tcgen05_pair_kernel<true, Epi>;
+    const void *id = reinterpret_cast<const void *>(kernel);
+    constexpr unsigned threads = 64u + 32u * Epi::kWarps;
+    if (int st = ensure_dynamic_smem(id, Cfg::kSmemBytes)) return st;
+    int resident = 0;
+    if (int st = resident_pairs_of(id, threads, Cfg::kSmemBytes, &resident)) return st;
+    const long long tiles = (long long)((p.M + 255) / 256) * ((p.N + 255) / 256);
+    return launch_clustered_overlapped(kernel, 2u * (unsigned)std::min<long long>(tiles, resident), threads, 2u, (size_t)Cfg::kSmemBytes, s, ma,
+                                       mb, mb, md, p);
+}
+
+// Runs the product that `p` describes (M, N, K, D, fmt, out_fmt, b_row_major, bias, extra, pre, activation set by the
+// caller; the rest filled in here).  A: [M, K], or [K, M] for the weight gradient; B: [N, K], or [K, N] with b_row_major.
+// Everything has been checked but the workspace.
+template <LinearMode kMode, bool kOut16>
+int run_product(LinearParams p, const void *A, const void *B, void *workspace, size_t workspace_bytes, cudaStream_t s, const DeviceInfo &info,
+                const char *name) {
+    using Epi = LinearEpilogue<kMode, kOut16>;
+    EncodeTiledFn encode = nullptr;
+    if (int st = get_encode_fn(&encode)) return st;
+    const bool tma = p.N % (kOut16 ? 8 : 4) == 0 && aligned16(p.D) && (p.pre == nullptr || (p.N % 8 == 0 && aligned16(p.pre)));
+    const ProductPlan plan = plan_product(p.M, p.N, p.K, tma, info.sm_count);
+    const size_t need = product_workspace(p.M, p.N, p.K, info.sm_count);
+    KO_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), KO_ERR_INVALID_ARG, "%s: the workspace needs %zu bytes, got %zu",
+               name, need, workspace ? workspace_bytes : (size_t)0);
+    KO_REQUIRE(aligned16(workspace), KO_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", name);
+    p.extra_vec = p.extra && aligned16(p.extra) && p.N % (Epi::kExtra16 ? 8 : 4) == 0;
+    p.bias_vec = p.bias && aligned16(p.bias) && p.N % 8 == 0;
+    p.C = nullptr;
+    p.tiles_n = p.wide_tiles_n = p.bn_wide = p.bn_narrow = 0;
+    p.split_k = plan.split;
+    p.partials = static_cast<float *>(workspace);
+    if (int st = device_status_word(0, &p.status)) return st;
+
+    alignas(64) CUtensorMap map_a, map_b, map_d;
+    if (Epi::kTransA) {
+        if (int st = make_map_b_row_major(encode, &map_a, p.fmt, A, p.K, p.M)) return st;
+    } else {
+        if (int st = make_map(encode, &map_a, p.fmt, A, p.M, p.K, tc::kBM)) return st;
+    }
+    if (p.b_row_major) {
+        if (int st = make_map_b_row_major(encode, &map_b, p.fmt, B, p.K, p.N)) return st;
+    } else {
+        if (int st = make_map(encode, &map_b, p.fmt, B, p.N, p.K, plan.pair ? 128 : plan.bn)) return st;
+    }
+    map_d = map_a;  // unused by the direct-store epilogue
+    p.map_pre = map_a;
+    if (tma) {
+        if (int st = make_store_map(encode, &map_d, p.out_fmt, p.D, p.M, p.N)) return st;
+        if (p.pre)
+            if (int st = make_store_map(encode, &p.map_pre, p.fmt + 1, p.pre, p.M, p.N)) return st;
+    }
+    int st;
+    if (plan.pair) st = launch_product_pair<Epi>(map_a, map_b, map_d, p, s);
+    else if (!tma) st = launch_product_tile<Epi, 128, false>(map_a, map_b, map_d, p, info.sm_count, s);
+    else if (plan.bn == 128) st = launch_product_tile<Epi, 128, true>(map_a, map_b, map_d, p, info.sm_count, s);
+    else st = launch_product_tile<Epi, 256, true>(map_a, map_b, map_d, p, info.sm_count, s);
+    if (st != KO_OK || plan.split <= 1) return st;
+    const long long chunks = plan.tiles * 4 * (plan.bn / 32);
+    return launch_overlapped(linear_slice_sum_kernel<kMode, kOut16>, (unsigned)chunks, 256u, (size_t)0, s, p, plan.bn);
+}
+
+// the checks that the three entry points share; M tokens, N output features, K input features
+int check_linear(const char *name, int in_fmt, int out_fmt, int activation, int64_t M, int64_t N, int64_t K);
+
+}  // namespace ko

@@ -67,6 +67,12 @@ PROTOTYPES = {
     "ko_gemm_f16_f16": (_int, [_i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
     "ko_gemm_bf16_bf16": (_int, [_i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
     "ko_gemm_tc": (_int, [_int, _int, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "ko_linear_workspace": (_int, [_i64, _i64, _i64, C.POINTER(_sz)]),
+    "ko_linear": (_int, [_int, _int, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ko_linear_backward_input_workspace": (_int, [_i64, _i64, _i64, C.POINTER(_sz)]),
+    "ko_linear_backward_input": (_int, [_int, _int, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ko_linear_backward_weight_workspace": (_int, [_i64, _i64, _i64, C.POINTER(_sz)]),
+    "ko_linear_backward_weight": (_int, [_int, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "ko_context_create": (_int, [_int, C.POINTER(_vp)]),
     "ko_context_destroy": (_int, [_vp]),
     "ko_context_stats": (_int, [_vp, C.POINTER(_sz), C.POINTER(_sz), C.POINTER(_sz), C.POINTER(_sz)]),

@@ -242,6 +242,24 @@ struct GemmParams {
     float *partials;
 };
 
+// What the kernels below do with a finished accumulator.  This one: D = acc (+ C).  A fused epilogue (kFused) brings its
+// own parameters, operands and chunk writer (see ../linear/linear_epilogue.h); kTransA: A is stored [K, M] (M contiguous).
+struct PlainEpilogue {
+    using Params = GemmParams;
+    static constexpr int kWarps = 4;  // epilogue warps, a multiple of 4: each quadrant of TMEM lanes is shared by kWarps / 4
+    static constexpr bool kTransA = false;
+    static constexpr bool kFused = false;
+};
+
+template <class Epi, bool kFused = Epi::kFused>
+struct FusedOperands {
+    struct type {};
+};
+template <class Epi>
+struct FusedOperands<Epi, true> {
+    using type = typename Epi::Operands;
+};
+
 // where column tile tn starts and how wide it is
 template <int BN>
 __device__ __forceinline__ void column_tile(const GemmParams &p, int tn, int &col0, int &bn) {
@@ -338,50 +356,57 @@ __device__ __forceinline__ void store_row_segment(const float (&v)[32], const Ge
     }
 }
 
-// One 32 x 32 chunk of D from registers: lane = row row_base + lane, r = its 32 consecutive columns starting at column
-// `col` (FP32 bits).  kTmaStore: registers -> swizzled shared box -> TMA store (box store_seq % kBoxes of this warp's
-// kBoxes staging boxes of box_bytes each, store_seq counts the warp's stores across tiles); otherwise direct 16-byte
-// stores (and + C).  Warp-collective.
+// One 32 x 32 chunk from registers through a swizzled shared-memory box to a TMA store: lane = row row_base + lane, r =
+// its 32 consecutive columns starting at column `col` (FP32 bits, rounded here to the type out_fmt); box store_seq %
+// kBoxes of this warp's staging boxes of box_bytes each, store_seq counts the warp's stores.  Warp-collective.
+template <int kBoxes>
+__device__ __forceinline__ void stage_chunk(const CUtensorMap *map, int M, int N, int out_fmt, const uint32_t (&r)[32], int row_base,
+                                            int col, int lane, uint32_t warp_boxes, uint32_t box_bytes, uint32_t &store_seq) {
+    // row = lane, 8 chunks of 16 B, chunk j stored at j ^ (row & 7): conflict-free, and exactly the 128-byte
+    // swizzle the store's tensor map undoes
+    const uint32_t box = warp_boxes + (store_seq % kBoxes) * box_bytes;
+    if (lane == 0) bulk_wait_group_read<kBoxes - 1>();  // the store issued from this box kBoxes chunks ago has read it
+    __syncwarp();
+    if (out_fmt == 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t dst = box + (uint32_t)lane * 128u + (uint32_t)((j ^ (lane & 7)) << 4);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(r[4 * j]), "r"(r[4 * j + 1]),
+                         "r"(r[4 * j + 2]), "r"(r[4 * j + 3])
+                         : "memory");
+        }
+    } else {
+        // 16-bit D: rows of 64 bytes, 4 chunks of 16 B, chunk j stored at j ^ ((row >> 1) & 3): the
+        // 64-byte swizzle of the store's tensor map, conflict-free for 8 consecutive rows
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t dst = box + (uint32_t)lane * 64u + (uint32_t)((j ^ ((lane >> 1) & 3)) << 4);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst),
+                         "r"(pack16(__uint_as_float(r[8 * j]), __uint_as_float(r[8 * j + 1]), out_fmt)),
+                         "r"(pack16(__uint_as_float(r[8 * j + 2]), __uint_as_float(r[8 * j + 3]), out_fmt)),
+                         "r"(pack16(__uint_as_float(r[8 * j + 4]), __uint_as_float(r[8 * j + 5]), out_fmt)),
+                         "r"(pack16(__uint_as_float(r[8 * j + 6]), __uint_as_float(r[8 * j + 7]), out_fmt))
+                         : "memory");
+        }
+    }
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) {
+        // rows / columns beyond M / N are clipped by the map; a box that lies entirely outside is
+        // skipped, but still closes a (then empty) group so that the box rotation holds
+        if (row_base < M && col < N) tma_store_2d(map, col, row_base, box);
+        bulk_commit_group();
+    }
+    ++store_seq;
+}
+
+// One 32 x 32 chunk of D from registers.  kTmaStore: stage_chunk; otherwise direct 16-byte stores (and + C).
+// Warp-collective.
 template <bool kTmaStore, int kBoxes>
 __device__ __forceinline__ void store_chunk(const CUtensorMap *map_d, const GemmParams &p, const uint32_t (&r)[32], int row_base,
                                             int col, int lane, uint32_t warp_boxes, uint32_t box_bytes, uint32_t &store_seq) {
     if constexpr (kTmaStore) {
-        // row = lane, 8 chunks of 16 B, chunk j stored at j ^ (row & 7): conflict-free, and exactly the 128-byte
-        // swizzle the store's tensor map undoes
-        const uint32_t box = warp_boxes + (store_seq % kBoxes) * box_bytes;
-        if (lane == 0) bulk_wait_group_read<kBoxes - 1>();  // the store issued from this box kBoxes chunks ago has read it
-        __syncwarp();
-        if (p.out_fmt == 0) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t dst = box + (uint32_t)lane * 128u + (uint32_t)((j ^ (lane & 7)) << 4);
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(r[4 * j]), "r"(r[4 * j + 1]),
-                             "r"(r[4 * j + 2]), "r"(r[4 * j + 3])
-                             : "memory");
-            }
-        } else {
-            // 16-bit D: rows of 64 bytes, 4 chunks of 16 B, chunk j stored at j ^ ((row >> 1) & 3): the
-            // 64-byte swizzle of the store's tensor map, conflict-free for 8 consecutive rows
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t dst = box + (uint32_t)lane * 64u + (uint32_t)((j ^ ((lane >> 1) & 3)) << 4);
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst),
-                             "r"(pack16(__uint_as_float(r[8 * j]), __uint_as_float(r[8 * j + 1]), p.out_fmt)),
-                             "r"(pack16(__uint_as_float(r[8 * j + 2]), __uint_as_float(r[8 * j + 3]), p.out_fmt)),
-                             "r"(pack16(__uint_as_float(r[8 * j + 4]), __uint_as_float(r[8 * j + 5]), p.out_fmt)),
-                             "r"(pack16(__uint_as_float(r[8 * j + 6]), __uint_as_float(r[8 * j + 7]), p.out_fmt))
-                             : "memory");
-            }
-        }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) {
-            // rows / columns beyond M / N are clipped by the map; a box that lies entirely outside is
-            // skipped, but still closes a (then empty) group so that the box rotation holds
-            if (row_base < p.M && col < p.N) tma_store_2d(map_d, col, row_base, box);
-            bulk_commit_group();
-        }
-        ++store_seq;
+        stage_chunk<kBoxes>(map_d, p.M, p.N, p.out_fmt, r, row_base, col, lane, warp_boxes, box_bytes, store_seq);
     } else {
         const int row = row_base + lane;
         if (row < p.M && col < p.N) {
@@ -430,9 +455,10 @@ __device__ __forceinline__ void epilogue_block(const CUtensorMap *map_d, const G
 
 // One epilogue warp writes its 32 rows x bn columns of a K slice's accumulator into the slice's slot: 32 x 32 chunks
 // of 4 KB, row-major inside a chunk (a lane's 32 columns are 128 contiguous bytes).
-__device__ __forceinline__ void publish_block(float *slot_chunks, uint32_t t_row, int bn, int lane) {
+// (c_begin, c_step: the columns of this warp where several warps share the rows)
+__device__ __forceinline__ void publish_block(float *slot_chunks, uint32_t t_row, int bn, int lane, int c_begin = 0, int c_step = 32) {
 #pragma unroll 1
-    for (int c0 = 0; c0 < bn; c0 += 32) {
+    for (int c0 = c_begin; c0 < bn; c0 += c_step) {
         float v[32];
         tmem_ld_32x32(t_row + c0, v);
         float4 *dst = reinterpret_cast<float4 *>(slot_chunks + ((size_t)(c0 >> 5) << 10) + lane * 32);
@@ -443,11 +469,11 @@ __device__ __forceinline__ void publish_block(float *slot_chunks, uint32_t t_row
 
 // kTmaStore: D is written by TMA stores staged through shared memory (needs a 16-byte row pitch and base for D
 // and no C operand); otherwise every thread stores its row segment directly (and adds C when given)
-template <int BN, bool kTmaStore, int MT = 1, int kBoxes = 2>
-__global__ void __launch_bounds__(kThreads, 1)
+template <int BN, bool kTmaStore, int MT = 1, int kBoxes = 2, class Epi = PlainEpilogue>
+__global__ void __launch_bounds__(64 + 32 * Epi::kWarps, 1)
 gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                     const __grid_constant__ CUtensorMap map_b_narrow, const __grid_constant__ CUtensorMap map_d,
-                    const GemmParams p) {
+                    const __grid_constant__ typename Epi::Params p) {
     using Cfg = TileConfig<BN, MT, kBoxes>;
     constexpr int kTileM = MT * kBM;
     extern __shared__ uint8_t ko_tc_smem_raw[];
@@ -490,7 +516,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(acc_ready_bar(a), 1);
-            mbar_init(acc_free_bar(a), 4);  // one arrival per epilogue warp
+            mbar_init(acc_free_bar(a), Epi::kWarps);  // one arrival per epilogue warp
         }
         mbar_init(drain_bar, 1);
         *abort_flag = 0;
@@ -536,7 +562,13 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     }
                     mbar_expect_tx(full_bar(s), stage_bytes);
                     const uint32_t dst = ring + s * Cfg::kStageBytes;
-                    tma_load_2d(dst, &map_a, kb * kBK, tm * kTileM, full_bar(s));  // one box of kTileM rows
+                    if constexpr (Epi::kTransA) {
+#pragma unroll
+                        for (int mb = 0; mb < kTileM / 64; ++mb)
+                            tma_load_2d(dst + mb * 8192, &map_a, tm * kTileM + mb * 64, kb * kBK, full_bar(s));
+                    } else {
+                        tma_load_2d(dst, &map_a, kb * kBK, tm * kTileM, full_bar(s));  // one box of kTileM rows
+                    }
                     if (!p.b_row_major) {
                         tma_load_2d(dst + Cfg::kBytesA, b_map, kb * kBK, col0, full_bar(s));
                     } else {
@@ -567,7 +599,8 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             // the low word is the address in 16-byte units plus the leading offset (1 for K-major, 8192 bytes for a
             // row-major B).  Building them per MMA cost the issuing thread about 75 cycles per instruction.
             const uint32_t desc_hi = (uint32_t)(1024 >> 4) | (1u << 14) | (2u << 29);
-            const uint32_t a_lo0 = ((ring & 0x3ffffu) >> 4) | (1u << 16);
+            const uint32_t a_lo0 = ((ring & 0x3ffffu) >> 4) | (Epi::kTransA ? (uint32_t)(8192 >> 4) << 16 : 1u << 16);
+            constexpr uint32_t a_kstep = Epi::kTransA ? 2048u >> 4 : 2u;
             const uint32_t b_lo0 = (((ring + Cfg::kBytesA) & 0x3ffffu) >> 4) | (p.b_row_major ? (uint32_t)(8192 >> 4) << 16 : 1u << 16);
             const uint32_t b_kstep = p.b_row_major ? 2048u >> 4 : (uint32_t)(kUmmaK * 2) >> 4;
             bool ok = true;
@@ -577,7 +610,8 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 unit_of(u, t, slice, kb0, kb1);
                 tile_of(p, t, tiles_m, tiles_n, tm, tn);
                 column_tile<BN>(p, tn, col0, bn);
-                const uint32_t idesc = make_idesc(p.fmt, kBM, bn) | (p.b_row_major ? 1u << 16 : 0u);  // bit 16: B is MN-major
+                // bit 15: A is MN-major, bit 16: B is MN-major
+                const uint32_t idesc = make_idesc(p.fmt, kBM, bn) | (p.b_row_major ? 1u << 16 : 0u) | (Epi::kTransA ? 1u << 15 : 0u);
                 // MT = 1: two accumulators used in turn; MT = 2: one accumulator per half, both busy with every tile
                 const uint32_t acc = MT == 1 ? (local_tile & 1u) : 0u, acc_phase = (MT == 1 ? (local_tile >> 1) : local_tile) & 1u;
                 if (!mbar_wait(acc_free_bar(acc), acc_phase ^ 1u, abort_flag)) { ok = false; break; }
@@ -593,9 +627,9 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     for (int k = 0; k < kBK / kUmmaK; ++k) {
                         // advancing K inside the swizzled row: +32 bytes per 16 elements (K-major); row-major B: 16 K-rows
                         // further = two 8-row atoms = 2048 bytes
-                        umma_f16_words(d_tmem, a_lo + k * 2, desc_hi, b_lo + k * b_kstep, desc_hi, idesc, accumulate);
+                        umma_f16_words(d_tmem, a_lo + k * a_kstep, desc_hi, b_lo + k * b_kstep, desc_hi, idesc, accumulate);
                         if (MT == 2)  // rows 128..255 of the tile: 16 KB further in the stage, accumulator columns BN..2BN-1
-                            umma_f16_words(d_tmem + BN, a_lo + (kBM * kBK * 2 >> 4) + k * 2, desc_hi, b_lo + k * b_kstep, desc_hi, idesc, accumulate);
+                            umma_f16_words(d_tmem + BN, a_lo + (kBM * kBK * 2 >> 4) + k * a_kstep, desc_hi, b_lo + k * b_kstep, desc_hi, idesc, accumulate);
                         accumulate = 1u;
                     }
                     umma_commit(empty_bar(stage));  // the stage is reusable once these MMAs have read it
@@ -615,10 +649,13 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         }
         __syncwarp();
     } else {
-        // ------------------------------------------------------------------ epilogue (warps 2..5)
+        // ------------------------------------------------------------------ epilogue (warps 2..)
         const int quad = warp & 3;  // TMEM lanes [32*quad, 32*quad+32) are the ones this warp may read
+        const int c_begin = ((warp - 2) >> 2) * 32;          // warps that share a quadrant take its 32-column chunks in turn
+        constexpr int c_step = 8 * Epi::kWarps;
         uint32_t local_tile = 0;
         uint32_t store_seq = 0;  // TMA stores issued by this warp so far: store n uses staging box n % kBoxes
+        [[maybe_unused]] typename FusedOperands<Epi>::type operands;
         bool ok = true;
         for (long long u = blockIdx.x; u < num_units && ok; u += gridDim.x, ++local_tile) {
             long long t;
@@ -627,6 +664,8 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             tile_of(p, t, tiles_m, tiles_n, tm, tn);
             column_tile<BN>(p, tn, col0, bn);
             const uint32_t acc = MT == 1 ? (local_tile & 1u) : 0u, acc_phase = (MT == 1 ? (local_tile >> 1) : local_tile) & 1u;
+            if constexpr (Epi::kFused)  // the first chunk's operands arrive while the tile is still being computed
+                if (split == 1) Epi::load(operands, p, tm * kTileM + quad * 32 + lane, col0 + c_begin);
             if (!mbar_wait(acc_ready_bar(acc), acc_phase, abort_flag)) {
                 if (lane == 0 && !*abort_flag) atomicCAS(p.status, kStatusOk, kTimeoutEpilogue);
                 *abort_flag = 1;
@@ -641,8 +680,13 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
 #pragma unroll 1
                 for (int half = 0; half < MT; ++half) {
                     const uint32_t t_row = tmem_base + ((uint32_t)(quad * 32) << 16) + (MT == 1 ? acc * BN : half * BN);
-                    publish_block(slot + ((size_t)((half * 4 + quad) * (BN / 32)) << 10), t_row, bn, lane);
+                    publish_block(slot + ((size_t)((half * 4 + quad) * (BN / 32)) << 10), t_row, bn, lane, c_begin, c_step);
                 }
+            } else if constexpr (Epi::kFused) {
+                static_assert(!Epi::kFused || MT == 1, "fused epilogues: 128-row tiles");
+                const uint32_t t_row = tmem_base + ((uint32_t)(quad * 32) << 16) + acc * BN;
+                Epi::template block<kTmaStore>(&map_d, p, operands, t_row, tm * kTileM + quad * 32, col0, bn, c_begin, lane,
+                                               store_base + (uint32_t)(warp - 2) * (uint32_t)(Cfg::kStoreBytes / Epi::kWarps), store_seq);
             } else {
 #pragma unroll 1
                 for (int half = 0; half < MT; ++half) {
@@ -652,7 +696,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                                                       (uint32_t)Cfg::kStoreBoxBytes, store_seq);
                 }  // halves
             }
-            // the accumulator buffer may be overwritten once all four warps have read it
+            // the accumulator buffer may be overwritten once all epilogue warps have read it
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(acc_free_bar(acc));

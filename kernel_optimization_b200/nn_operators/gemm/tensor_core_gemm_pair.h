@@ -105,11 +105,11 @@ __device__ __forceinline__ bool mbar_wait_remote(uint32_t bar, uint32_t parity, 
 }
 
 // map_b / map_b_narrow: boxes of bn_wide / 2 and bn_narrow / 2 rows (128 rows when the tiles are uniform)
-template <bool kTmaStore>
-__global__ void __launch_bounds__(kThreads, 1)
+template <bool kTmaStore, class Epi = PlainEpilogue>
+__global__ void __launch_bounds__(64 + 32 * Epi::kWarps, 1)
 gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                          const __grid_constant__ CUtensorMap map_b_narrow, const __grid_constant__ CUtensorMap map_d,
-                         const GemmParams p) {
+                         const __grid_constant__ typename Epi::Params p) {
     using Cfg = PairConfig;
     constexpr int BN = Cfg::kBN, kTileM = 2 * kBM;
     extern __shared__ uint8_t ko_tc_pair_smem_raw[];
@@ -142,7 +142,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(acc_ready_bar(a), 1);
-            mbar_init(acc_free_bar(a), 8);  // four epilogue warps of each CTA
+            mbar_init(acc_free_bar(a), 2 * Epi::kWarps);  // the epilogue warps of each CTA
         }
         mbar_init(drain_bar, 1);
         *abort_flag = 0;
@@ -191,7 +191,14 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                     }
                     const uint32_t leader_full = map_to_cluster_rank(full_bar(s), 0);
                     const uint32_t dst = ring + s * Cfg::kStageBytes;
-                    tma_load_2d_pair(dst, &map_a, kb * kBK, tm * kTileM + (int)rank * kBM, leader_full);
+                    if constexpr (Epi::kTransA) {
+                        // A stored [K, M]: this CTA's 128 rows of the tile as two boxes of 64 K-rows x 64 M (MN-major operand)
+#pragma unroll
+                        for (int mb = 0; mb < kBM / 64; ++mb)
+                            tma_load_2d_pair(dst + mb * 8192, &map_a, tm * kTileM + (int)rank * kBM + mb * 64, kb * kBK, leader_full);
+                    } else {
+                        tma_load_2d_pair(dst, &map_a, kb * kBK, tm * kTileM + (int)rank * kBM, leader_full);
+                    }
                     if (!p.b_row_major) {
                         tma_load_2d_pair(dst + Cfg::kBytesA, b_map, kb * kBK, col0 + (int)rank * half, leader_full);
                     } else {
@@ -212,7 +219,8 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
             uint32_t stage = 0, phase = 0;  // ring position of K-block `it` and the parity of its fill
             // descriptor words of the ring's first stage, stepped by 32-bit adds (see the single-CTA kernel)
             const uint32_t desc_hi = (uint32_t)(1024 >> 4) | (1u << 14) | (2u << 29);
-            const uint32_t a_lo0 = ((ring & 0x3ffffu) >> 4) | (1u << 16);
+            const uint32_t a_lo0 = ((ring & 0x3ffffu) >> 4) | (Epi::kTransA ? (uint32_t)(8192 >> 4) << 16 : 1u << 16);
+            constexpr uint32_t a_kstep = Epi::kTransA ? 2048u >> 4 : 2u;
             const uint32_t b_lo0 = (((ring + Cfg::kBytesA) & 0x3ffffu) >> 4) | (p.b_row_major ? (uint32_t)(8192 >> 4) << 16 : 1u << 16);
             const uint32_t b_kstep = p.b_row_major ? 2048u >> 4 : (uint32_t)(kUmmaK * 2) >> 4;
             bool ok = true;
@@ -222,7 +230,8 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                 int tm, tn, col0, bn;
                 tile_of(p, t, tiles_m, tiles_n, tm, tn);
                 column_tile<BN>(p, tn, col0, bn);
-                const uint32_t idesc = make_idesc(p.fmt, kTileM, bn) | (p.b_row_major ? 1u << 16 : 0u);  // bit 16: B is MN-major
+                // bit 15: A is MN-major, bit 16: B is MN-major
+                const uint32_t idesc = make_idesc(p.fmt, kTileM, bn) | (p.b_row_major ? 1u << 16 : 0u) | (Epi::kTransA ? 1u << 15 : 0u);
                 const uint32_t acc = local_tile & 1u, acc_phase = (local_tile >> 1) & 1u;
                 if (!mbar_wait_remote(acc_free_bar(acc), acc_phase ^ 1u, abort_flag)) { ok = false; break; }
                 tc_fence_after();
@@ -234,7 +243,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                     uint32_t accumulate = kb != 0 ? 1u : 0u;
 #pragma unroll
                     for (int k = 0; k < kBK / kUmmaK; ++k) {
-                        umma_f16_pair_words(d_tmem, a_lo + k * 2, desc_hi, b_lo + k * b_kstep, desc_hi, idesc, accumulate);
+                        umma_f16_pair_words(d_tmem, a_lo + k * a_kstep, desc_hi, b_lo + k * b_kstep, desc_hi, idesc, accumulate);
                         accumulate = 1u;
                     }
                     // the stage is reusable once these MMAs have read it (in both CTAs: the commit tracks both SMs); the
@@ -259,8 +268,10 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         }
         __syncwarp();
     } else {
-        // ------------------------------------------------------------------ epilogue (warps 2..5, both CTAs)
+        // ------------------------------------------------------------------ epilogue (warps 2.., both CTAs)
         const int quad = warp & 3;
+        [[maybe_unused]] const int c_begin = ((warp - 2) >> 2) * 32;
+        [[maybe_unused]] typename FusedOperands<Epi>::type operands;
         uint32_t local_tile = 0, store_seq = 0;
         bool ok = true;
         for (long long t = pair; t < num_tiles && ok; t += pairs, ++local_tile) {
@@ -268,6 +279,8 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
             tile_of(p, t, tiles_m, tiles_n, tm, tn);
             column_tile<BN>(p, tn, col0, bn);
             const uint32_t acc = local_tile & 1u, acc_phase = (local_tile >> 1) & 1u;
+            const int row_base = tm * kTileM + (int)rank * kBM + quad * 32;
+            if constexpr (Epi::kFused) Epi::load(operands, p, row_base + lane, col0 + c_begin);  // while the tile is being computed
             if (!mbar_wait(acc_ready_bar(acc), acc_phase, abort_flag)) {
                 if (lane == 0 && !*abort_flag) atomicCAS(p.status, kStatusOk, kTimeoutEpilogue);
                 *abort_flag = 1;
@@ -276,10 +289,14 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
             }
             tc_fence_after();
             const uint32_t t_row = tmem_base + ((uint32_t)(quad * 32) << 16) + acc * BN;
-            epilogue_block<kTmaStore, Cfg::kStoreBoxes>(&map_d, p, t_row, tm * kTileM + (int)rank * kBM + quad * 32, col0, bn, lane,
-                                                        store_base + (uint32_t)((warp - 2) * Cfg::kStoreBoxes) * Cfg::kStoreBoxBytes,
-                                                        (uint32_t)Cfg::kStoreBoxBytes, store_seq);
-            // the accumulator may be overwritten once all eight epilogue warps of the pair have read theirs
+            if constexpr (Epi::kFused)
+                Epi::template block<kTmaStore>(&map_d, p, operands, t_row, row_base, col0, bn, c_begin, lane,
+                                               store_base + (uint32_t)(warp - 2) * (uint32_t)(Cfg::kStoreBytes / Epi::kWarps), store_seq);
+            else
+                epilogue_block<kTmaStore, Cfg::kStoreBoxes>(&map_d, p, t_row, row_base, col0, bn, lane,
+                                                            store_base + (uint32_t)((warp - 2) * Cfg::kStoreBoxes) * Cfg::kStoreBoxBytes,
+                                                            (uint32_t)Cfg::kStoreBoxBytes, store_seq);
+            // the accumulator may be overwritten once all epilogue warps of the pair have read theirs
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(map_to_cluster_rank(acc_free_bar(acc), 0));

@@ -278,3 +278,115 @@ def gemm_tc(a, b, c=None, out=None, stream: int | None = None, out_dtype=None, b
     native.check(native.lib().ko_gemm_tc(in_fmt, out_fmt, 1 if b_row_major else 0, M, N, K, _ptr(a), _ptr(b), _ptr(c), _ptr(out), s),
                  "ko_gemm_tc")
     return out
+
+
+# ------------------------------------------------------------------ linear layer, forward and backward
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
+
+def _activation_code(name: str) -> int:
+    if name not in ACTIVATIONS:
+        raise ValueError(f"unknown activation {name!r}, expected one of {', '.join(ACTIVATIONS)}")
+    return ACTIVATIONS[name]
+
+
+def _linear_types(a, out, out_dtype, default):
+    """(in_fmt, out_fmt, out_dtype) of a product whose inputs have `a`'s type."""
+    import torch
+
+    if a.dim() != 2 or a.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"the inputs must be 2-D FP16 or BF16 tensors, got {a.dtype} with {a.dim()} dimensions")
+    if out_dtype is None:
+        out_dtype = default if out is None else out.dtype
+    if out_dtype not in (torch.float32, a.dtype):
+        raise ValueError(f"the output is FP32 or the inputs' {a.dtype}, not {out_dtype}")
+    in_fmt = 0 if a.dtype == torch.float16 else 1
+    return in_fmt, 0 if out_dtype == torch.float32 else in_fmt + 1, out_dtype
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_bytes(device_index: int, entry: str, m: int, n: int, k: int) -> int:
+    nbytes = C.c_size_t()
+    native.check(getattr(native.lib(), entry)(m, n, k, C.byref(nbytes)), entry)
+    return nbytes.value
+
+
+def linear(x, w, bias=None, activation: str = "none", residual=None, out=None, out_dtype=None, return_pre: bool = False, pre=None,
+           stream: int | None = None):
+    """``y = act(x @ w.T + bias) + residual`` on the tensor cores.
+
+    ``x`` [tokens, k] and ``w`` [n, k] are FP16 or BF16 with k a multiple of 8, ``bias`` [n] has their type; ``y`` and ``residual``
+    [tokens, n] have ``out_dtype``: the inputs' type (default) or FP32.  ``activation``: none, relu, gelu (erf), gelu_tanh or silu.
+    With ``return_pre`` (or a tensor ``pre`` to write) the result is ``(y, pre)``, ``pre = x @ w.T + bias`` in the inputs' type:
+    what :func:`linear_backward_input` of the next layer takes.  ``out`` may be ``residual`` itself.
+    """
+    import torch
+
+    in_fmt, out_fmt, out_dtype = _linear_types(x, out, out_dtype, x.dtype)
+    act = _activation_code(activation)
+    device, same, to = x.device, (x.dtype,), (out_dtype,)
+    if w.dim() != 2:
+        raise ValueError(f"w must have 2 dimensions, got {w.dim()}")
+    (m, k), n = x.shape, w.shape[0]
+    with _on(device, stream):
+        out = torch.empty((m, n), dtype=out_dtype, device=device) if out is None else out
+        if return_pre and pre is None:
+            pre = torch.empty((m, n), dtype=x.dtype, device=device)
+        ws = _workspace(_linear_bytes(device.index, "ko_linear_workspace", m, n, k), device)
+        native.check(native.lib().ko_linear(in_fmt, out_fmt, act, m, n, k, _ptr(x), _operand(w, "w", device, same, (n, k)),
+                                            _operand(bias, "bias", device, same, (n,)), _operand(residual, "residual", device, to, (m, n)),
+                                            _operand(out, "out", device, to, (m, n)), _operand(pre, "pre", device, same, (m, n)),
+                                            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
+                                            _current_stream_ptr()), "ko_linear")
+    return out if pre is None else (out, pre)
+
+
+def linear_backward_input(dy, w, pre=None, activation: str = "none", out=None, out_dtype=None, stream: int | None = None):
+    """``dx = (dy @ w) * act'(pre)``: the gradient of :func:`linear`'s input, taken on through the activation that made it.
+
+    ``dy`` [tokens, n] and ``w`` [n, k] are FP16 or BF16, n and k multiples of 8; ``pre`` [tokens, k] (the inputs' type) is the
+    pre-activation of the layer before, needed unless ``activation`` is none.  ``dx`` [tokens, k] has ``out_dtype``: the inputs'
+    type (default; ``out`` may then be ``pre`` itself) or FP32.
+    """
+    import torch
+
+    in_fmt, out_fmt, out_dtype = _linear_types(dy, out, out_dtype, dy.dtype)
+    act = _activation_code(activation)
+    device, same = dy.device, (dy.dtype,)
+    if w.dim() != 2:
+        raise ValueError(f"w must have 2 dimensions, got {w.dim()}")
+    (m, n), k = dy.shape, w.shape[1]
+    with _on(device, stream):
+        out = torch.empty((m, k), dtype=out_dtype, device=device) if out is None else out
+        ws = _workspace(_linear_bytes(device.index, "ko_linear_backward_input_workspace", m, n, k), device)
+        native.check(native.lib().ko_linear_backward_input(
+            in_fmt, out_fmt, act, m, n, k, _ptr(dy), _operand(w, "w", device, same, (n, k)), _operand(pre, "pre", device, same, (m, k)),
+            _operand(out, "out", device, (out_dtype,), (m, k)), None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
+            _current_stream_ptr()), "ko_linear_backward_input")
+    return out
+
+
+def linear_backward_weight(dy, x, c=None, out=None, out_dtype=None, return_bias: bool = True, dbias=None, stream: int | None = None):
+    """``dw = dy.T @ x (+ c)`` and, with ``return_bias`` (or a tensor ``dbias`` to write), ``dbias`` = the column sums of ``dy``.
+
+    ``dy`` [tokens, n] and ``x`` [tokens, k] are FP16 or BF16, n and k multiples of 8, any number of tokens.  ``dw`` and ``c`` [n, k]
+    have ``out_dtype``: FP32 (default) or the inputs' type; ``out`` may be ``c`` itself (gradients gathered over micro-batches).
+    ``dbias`` [n] is FP32.  Returns ``(dw, dbias)``, or ``dw`` alone.
+    """
+    import torch
+
+    in_fmt, out_fmt, out_dtype = _linear_types(dy, out, out_dtype, torch.float32)
+    device, to = dy.device, (out_dtype,)
+    if x.dim() != 2:
+        raise ValueError(f"x must have 2 dimensions, got {x.dim()}")
+    (m, n), k = dy.shape, x.shape[1]
+    with _on(device, stream):
+        out = torch.empty((n, k), dtype=out_dtype, device=device) if out is None else out
+        if return_bias and dbias is None:
+            dbias = torch.empty(n, dtype=torch.float32, device=device)
+        ws = _workspace(_linear_bytes(device.index, "ko_linear_backward_weight_workspace", m, n, k), device)
+        native.check(native.lib().ko_linear_backward_weight(
+            in_fmt, out_fmt, m, n, k, _ptr(dy), _operand(x, "x", device, (dy.dtype,), (m, k)), _operand(c, "c", device, to, (n, k)),
+            _operand(out, "out", device, to, (n, k)), _operand(dbias, "dbias", device, (torch.float32,), (n,)),
+            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _current_stream_ptr()), "ko_linear_backward_weight")
+    return out if dbias is None else (out, dbias)
