@@ -75,6 +75,290 @@ __device__ __forceinline__ void block_allreduce_sums(float (&v)[N], float *scrat
     __syncthreads();
 }
 
+// Rows that fit the registers of up to 16 warps: one pass over memory.  kLanes threads (part of a warp, or whole warps) hold a
+// row, each of them kVecs chunks of E columns of x and dy; a block takes kRows consecutive rows at a time and persists over
+// the rows, so a thread meets the same columns in every row: gamma stays in registers and so do its dgamma and dbeta, which
+// leave once per block.  Per row two reductions of two values each: sum x and sum w, then, with the mean, sum dev^2 and
+// sum w dev.
+//
+// Consecutive rows are consecutive bytes: one thread brings a step's rows of x, dy and the residual into a shared-memory
+// ring by one bulk copy each (cp.async.bulk, counted in bytes on an mbarrier), several steps ahead, so the bytes in flight
+// depend neither on registers nor on how many warps the row's reductions keep waiting.  Bulk copies want 16-byte
+// boundaries: rows of single elements (E == 1: odd widths, unaligned operands) come by plain loads instead.
+//
+// 16-bit rows leave about 34 instruction slots per element at full bandwidth (6 bytes an element, 22 bytes per clock and
+// SM), so arithmetic runs on packed FP32 pairs, elements are unpacked once, and a thread holds 16 columns to spread the
+// reductions' shuffles over many elements.
+constexpr int kBackwardWarpsPerSm = 16;  // at 128 registers a thread
+constexpr int kBackwardMaxStages = 8;
+
+// warps of a block for rows of `lanes` threads: whole rows, about eight warps
+__host__ __device__ constexpr int backward_warps(int lanes) {
+    const int group = lanes <= 32 ? 1 : lanes / 32;
+    if (group == 3 || group == 5) return 15;
+    return group >= 8 ? group : group * (8 / group);
+}
+__host__ __device__ constexpr int backward_blocks_per_sm(int lanes) { return kBackwardWarpsPerSm / backward_warps(lanes); }
+
+// sums of two values over the kLanes threads of a row, in every thread of it
+template <int kLanes>
+struct RowReduce {
+    float *scratch;  // [2][warps of a row][2], 16-byte aligned; only for rows of several warps
+    int barrier;     // named barrier of the row's warps
+    int turn = 0;
+    __device__ __forceinline__ void operator()(float &a, float &b) {
+        constexpr int kWidth = kLanes < 32 ? kLanes : 32;
+        // the lower half of the lanes goes on with a, the upper half with b: five exchanges for both sums
+        const int lane = threadIdx.x & 31;
+        const bool upper = lane & (kWidth / 2);
+        float v = upper ? b : a;
+        v += __shfl_xor_sync(kFullMask, upper ? a : b, kWidth / 2);
+#pragma unroll
+        for (int m = kWidth / 4; m > 0; m >>= 1) v += __shfl_xor_sync(kFullMask, v, m);
+        if constexpr (kLanes <= 32) {
+            a = __shfl_sync(kFullMask, v, 0, kWidth);
+            b = __shfl_sync(kFullMask, v, kWidth / 2, kWidth);
+        } else {
+            // Two scratch halves in turn: whoever writes a half again has passed the barrier of the reduction in between, so
+            // everyone has read it.
+            constexpr int kGroup = kLanes / 32;
+            float *half = scratch + turn * 2 * kGroup;
+            turn ^= 1;
+            if ((lane & 15) == 0) half[2 * ((threadIdx.x >> 5) % kGroup) + (lane >> 4)] = v;
+            asm volatile("bar.sync %0, %1;" ::"r"(barrier), "n"(kLanes) : "memory");
+            f32x2 sum = *reinterpret_cast<const f32x2 *>(half);
+#pragma unroll
+            for (int w = 1; w < kGroup; ++w) sum = pair_add(sum, *reinterpret_cast<const f32x2 *>(half + 2 * w));
+            pair_split(sum, a, b);
+        }
+    }
+};
+
+// stages: steps of kRows rows in the ring (dynamic shared memory: [stages][x, dy(, residual)][kRows][cols], at least
+// 2 * kCapacity floats for the column sums at the end); status: the staged row operators' device status word
+template <typename T, int E, int kVecs, int kLanes>
+__global__ void __launch_bounds__(32 * backward_warps(kLanes), backward_blocks_per_sm(kLanes))
+layernorm_backward_resident_kernel(const LayerNormBackwardArgs<T> a, int stages, unsigned *status) {
+    using Chunk = RowChunk<T, E>;
+    using Raw = typename Chunk::Raw;
+    constexpr int kWarps = backward_warps(kLanes), kRows = 32 * kWarps / kLanes;
+    constexpr int kCapacity = kLanes * kVecs * E, kPairs = kVecs * E / 2;
+    constexpr bool kSingles = E == 1;  // a pair then spans two chunks, and rows come by plain loads
+    extern __shared__ __align__(16) uint8_t ring[];
+    __shared__ __align__(16) float scratch[kLanes > 32 ? kRows : 1][kLanes > 32 ? 4 * (kLanes / 32) : 1];
+    __shared__ uint64_t full[kBackwardMaxStages], empty[kBackwardMaxStages];
+    __shared__ int abort_flag;
+    const int slot = threadIdx.x / kLanes, t = threadIdx.x % kLanes;
+    RowReduce<kLanes> reduce{kLanes > 32 ? scratch[slot] : nullptr, 1 + slot};
+    const float inv_n = 1.0f / (float)a.cols, inv_d = a.cols > a.ddof ? 1.0f / (float)(a.cols - a.ddof) : 0.f;
+    f32x2 gamma[kPairs], dgamma[kPairs], dbeta[kPairs];
+    bool active[kVecs];
+
+    auto unpack = [](const Raw (&raw)[kVecs], f32x2 (&p)[kPairs]) {
+        if constexpr (kSingles) {
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) p[i] = pair_of(RowIo<T>::to_float(raw[2 * i]), RowIo<T>::to_float(raw[2 * i + 1]));
+        } else {
+#pragma unroll
+            for (int v = 0; v < kVecs; ++v) RowIo<T>::unpack_pairs(raw[v], p + v * (E / 2));
+        }
+    };
+    // the thread's chunks of a row; zeros past the row's end, or everywhere in a row that is not there
+    auto load = [&](const T *row, bool there, f32x2 (&p)[kPairs]) {
+        Raw raw[kVecs];
+#pragma unroll
+        for (int v = 0; v < kVecs; ++v) raw[v] = active[v] && there ? Chunk::load(row + (t + v * kLanes) * E) : Chunk::zero();
+        unpack(raw, p);
+    };
+
+    // ring: step i of this block (rows step_row(i) .. + kRows - 1) lives in stage i % stages
+    const uint32_t tensor_bytes = (uint32_t)(kRows * a.cols * (int)sizeof(T)), stage_bytes = tensor_bytes * (a.residual ? 3u : 2u);
+    const long long steps = (a.rows - 1 - (long long)blockIdx.x * kRows) / ((long long)gridDim.x * kRows) + 1;  // the grid has no idle block
+    auto step_row = [&](long long i) { return ((long long)blockIdx.x + i * gridDim.x) * kRows; };
+    auto bring = [&](long long i) {
+        const int s = (int)(i % stages);
+        const long long first = step_row(i);
+        const uint32_t bytes = (uint32_t)(a.rows - first < kRows ? a.rows - first : kRows) * (uint32_t)a.cols * (uint32_t)sizeof(T);
+        const uint32_t bar = smem_u32(full + s), dst = smem_u32(ring) + (uint32_t)s * stage_bytes;
+        mbar_expect_tx(bar, a.residual ? 3u * bytes : 2u * bytes);
+        bulk_load_1d(dst, a.x + (size_t)first * a.cols, bytes, bar);
+        bulk_load_1d(dst + tensor_bytes, a.dy + (size_t)first * a.cols, bytes, bar);
+        if (a.residual) bulk_load_1d(dst + 2 * tensor_bytes, a.residual + (size_t)first * a.cols, bytes, bar);
+    };
+    auto give_up = [&](unsigned code) {  // a wait ran out: the rest runs through without waiting, the host is told
+        atomicCAS(status, 0u, code);
+        *(volatile int *)&abort_flag = 1;
+    };
+
+    if (!kSingles && threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) {
+            mbar_init(smem_u32(full + s), 1);
+            mbar_init(smem_u32(empty + s), kWarps);
+        }
+        abort_flag = 0;
+        fence_barrier_init();
+        fence_proxy_async();
+    }
+    grid_launch_dependents();
+    if (!kSingles) __syncthreads();
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) active[v] = (t + v * kLanes) * E < a.cols;
+    grid_dependency_wait();
+    if (!kSingles && threadIdx.x == 0)
+        for (long long i = 0; i < stages && i < steps; ++i) bring(i);
+    // a row's columns past the last one: x = dy = gamma = 0
+    if (a.gamma) {
+        load(a.gamma, true, gamma);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+            const float lo = active[2 * i / E] ? 1.f : 0.f, hi = active[(2 * i + 1) / E] ? 1.f : 0.f;
+            gamma[i] = pair_of(lo, hi);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) dgamma[i] = dbeta[i] = pair_of(0.f, 0.f);
+
+    int stage = 0;
+    uint32_t phase = 0;
+    for (long long i = 0; i < steps; ++i) {
+        // all threads of a block make the same number of steps: a row past the end is zeros and nothing is stored
+        const long long r = step_row(i) + slot;
+        const bool there = r < a.rows;
+        f32x2 x[kPairs], dy[kPairs];
+        const T *staged = reinterpret_cast<const T *>(ring + (size_t)stage * stage_bytes) + slot * a.cols;
+        if constexpr (kSingles) {
+            load(a.x + (size_t)r * a.cols, there, x);
+            load(a.dy + (size_t)r * a.cols, there, dy);
+        } else {
+            if (!mbar_wait(smem_u32(full + stage), phase, &abort_flag)) give_up(2u);
+            load(staged, there, x);
+            load(staged + kRows * a.cols, there, dy);
+        }
+        f32x2 sum_x2 = x[0], sum_w2 = pair_mul(dy[0], gamma[0]);
+#pragma unroll
+        for (int i = 1; i < kPairs; ++i) {
+            sum_x2 = pair_add(sum_x2, x[i]);
+            sum_w2 = pair_fma(dy[i], gamma[i], sum_w2);
+        }
+        float lo, hi, sum_x, sum_w;
+        pair_split(sum_x2, lo, hi);
+        sum_x = lo + hi;
+        pair_split(sum_w2, lo, hi);
+        sum_w = lo + hi;
+        reduce(sum_x, sum_w);
+        // the stage of the step before: by now every warp of this row is done with it
+        if (!kSingles && threadIdx.x == 0 && i > 0 && i - 1 + stages < steps) {
+            const int before = stage ? stage - 1 : stages - 1;
+            if (!mbar_wait(smem_u32(empty + before), stage ? phase : phase ^ 1u, &abort_flag)) give_up(3u);
+            else bring(i - 1 + stages);
+        }
+        const float mean = sum_x * inv_n;
+        f32x2 minus_mean[kSingles ? kPairs : kVecs];  // 0 past the row's end: the deviation is 0 there
+#pragma unroll
+        for (int i = 0; i < (kSingles ? kPairs : kVecs); ++i)
+            minus_mean[i] = kSingles ? pair_of(active[(2 * i) % kVecs] ? -mean : 0.f, active[(2 * i + 1) % kVecs] ? -mean : 0.f)
+                                     : (active[i] ? pair_of(-mean, -mean) : pair_of(0.f, 0.f));
+        f32x2 m2_2 = pair_of(0.f, 0.f), sum_wd2 = m2_2;
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+            x[i] = pair_add(x[i], minus_mean[kSingles ? i : 2 * i / E]);  // x holds the deviations from here on
+            m2_2 = pair_fma(x[i], x[i], m2_2);
+            sum_wd2 = pair_fma(pair_mul(dy[i], gamma[i]), x[i], sum_wd2);
+        }
+        float m2, sum_wd;
+        pair_split(m2_2, lo, hi);
+        m2 = lo + hi;
+        pair_split(sum_wd2, lo, hi);
+        sum_wd = lo + hi;
+        reduce(m2, sum_wd);
+        const float rstd = rsqrtf(fmaf(m2, inv_d, a.eps));
+        // dx = rstd w - rstd c1 - xhat rstd c2, c1 = sum(w) / n, c2 = sum(w xhat) / d
+        const float offset = -rstd * sum_w * inv_n, slope = -rstd * (sum_wd * rstd * inv_d);
+        const f32x2 rstd2 = pair_of(rstd, rstd), offset2 = pair_of(offset, offset), slope2 = pair_of(slope, slope);
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+            const f32x2 xhat = pair_mul(x[i], rstd2);
+            dgamma[i] = pair_fma(dy[i], xhat, dgamma[i]);
+            dbeta[i] = pair_add(dbeta[i], dy[i]);
+            x[i] = pair_fma(xhat, slope2, pair_fma(pair_mul(dy[i], gamma[i]), rstd2, offset2));
+        }
+        if (a.residual) {
+            f32x2 add[kPairs];
+            load(kSingles ? a.residual + (size_t)r * a.cols : staged + 2 * kRows * a.cols, there, add);
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) x[i] = pair_add(x[i], add[i]);
+        }
+        if constexpr (!kSingles) {
+            __syncwarp();
+            if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(empty + stage));
+            if (++stage == stages) {
+                stage = 0;
+                phase ^= 1u;
+            }
+        }
+        if (there) {
+            T *out = a.dx + (size_t)r * a.cols + t * E;
+#pragma unroll
+            for (int v = 0; v < kVecs; ++v)
+                if (active[v]) {
+                    if constexpr (kSingles) {
+                        pair_split(x[v / 2], lo, hi);
+                        out[v * kLanes] = RowIo<T>::from_float(v & 1 ? hi : lo);
+                    } else {
+                        Chunk::store(out + v * kLanes * E, RowIo<T>::pack_pairs(x + v * (E / 2)));
+                    }
+                }
+        }
+    }
+    if (!kSingles && threadIdx.x == 0 && *(volatile int *)&abort_flag) {
+        // copies on their way still land in this block's shared memory: wait (bounded) for each stage's last one
+        for (int s = 0; s < stages; ++s)
+            for (uint32_t parity = 0; parity < 2; ++parity)
+                for (uint32_t spin = 0; spin < kSpinLimit / 64 && !mbar_try_wait(smem_u32(full + s), parity); ++spin) {}
+    }
+    if (a.partials == nullptr) return;
+    auto column = [&](int i) { return kSingles ? t + i * kLanes : (t + (i / E) * kLanes) * E + i % E; };  // of the thread's i-th value
+    float *out = a.partials + (size_t)blockIdx.x * 2 * a.cols;
+    if constexpr (kRows > 1) {
+        float *fold = reinterpret_cast<float *>(ring);  // every stage has been read: the ring is free
+        __syncthreads();
+        // the block's rows add their column sums one after the other, then the block writes one partial row
+        for (int turn = 0; turn < kRows; ++turn) {
+            if (slot == turn) {
+#pragma unroll
+                for (int i = 0; i < kPairs; ++i)
+#pragma unroll
+                    for (int which = 0; which < 2; ++which) {
+                        float v[2];
+                        pair_split(which ? dbeta[i] : dgamma[i], v[0], v[1]);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float *at = fold + which * kCapacity + column(2 * i + h);
+                            *at = turn ? *at + v[h] : v[h];
+                        }
+                    }
+            }
+            __syncthreads();
+        }
+        for (int i = threadIdx.x; i < a.cols; i += 32 * kWarps) {
+            out[i] = fold[i];
+            out[a.cols + i] = fold[kCapacity + i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i)
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                float v[2];
+                pair_split(which ? dbeta[i] : dgamma[i], v[0], v[1]);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (column(2 * i + h) < a.cols) out[which * a.cols + column(2 * i + h)] = v[h];
+            }
+    }
+}
+
 // Rows of any length: one block per row forms the row's terms in two passes over x (the second one and dy come from
 // the L1 / L2).
 template <typename T, int E>
@@ -176,9 +460,10 @@ __global__ void __launch_bounds__(256) layernorm_backward_apply_kernel(const Lay
     }
 }
 
-// dgamma / dbeta = the partial rows added in order: a block takes 32 columns, warp w the partial rows w, w + 8, ...
+// dgamma / dbeta = the partial rows added in a fixed order: a block takes 32 columns, warp w of 32 the partial rows w, w + 32,
+// ... (few loads per thread, all in flight: the kernel is latency)
 // (a template only so that the header may be included by several translation units)
-template <int kWarps = 8>
+template <int kWarps = 32>
 __global__ void __launch_bounds__(32 * kWarps) layernorm_backward_fold_kernel(const float *partials, int partial_rows, int cols,
                                                                               float *dgamma, float *dbeta) {
     __shared__ float fold[2][kWarps][32];

@@ -6,6 +6,7 @@ a page-locked host buffer plus a device buffer with copies in both directions.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import functools
 
@@ -21,7 +22,8 @@ _SIZE_OF = {DTYPE_F32: 4, DTYPE_F16: 2, DTYPE_BF16: 2}
 def _current_stream_ptr() -> int:
     import torch
 
-    return int(torch.cuda.current_stream().cuda_stream)
+    # the handle alone: building the Stream object around it (torch.cuda.current_stream()) costs the host 3 us a call
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _ptr(t) -> int | None:
@@ -151,16 +153,21 @@ def layernorm(x, eps: float, gamma=None, beta=None, ddof: int = 0, out=None, str
 
 
 def _operand(t, name: str, device, dtypes, shape) -> int | None:
-    """Address of an operand after checking where it lives, its type and its shape (None stays None)."""
+    """Address of an operand after checking where it lives, its type, shape and layout (None stays None)."""
     if t is None:
         return None
+    if t.device == device and t.dtype in dtypes and t.shape == shape and t.is_contiguous():
+        return t.data_ptr()
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, the operator's first input on {device}")
     if t.dtype not in dtypes:
         raise ValueError(f"{name} is {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
-    return _ptr(t)
+    raise ValueError(f"{name} must be contiguous")
+
+
+_HERE = contextlib.nullcontext()
 
 
 def _on(device, stream: int | None):
@@ -171,18 +178,21 @@ def _on(device, stream: int | None):
     if device.type != "cuda":
         raise ValueError("operator inputs must live on a CUDA device (there is no CPU path)")
     if stream is None:
-        return torch.cuda.device(device)
+        return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
     if stream == 0:
         return torch.cuda.stream(torch.cuda.default_stream(device))
     return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device))
 
 
 def _workspace(nbytes: int, device):
-    """Device memory for one call: allocated on the current stream, so the caching allocator hands it out again only to work
-    that runs after the call (inside a capture: it belongs to the graph)."""
+    """(tensor, address, bytes) of device memory for one call: allocated on the current stream, so the caching allocator hands
+    it out again only to work that runs after the call (inside a capture: it belongs to the graph)."""
     import torch
 
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    if nbytes == 0:
+        return None, None, 0
+    t = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return t, t.data_ptr(), nbytes
 
 
 @functools.lru_cache(maxsize=4096)
@@ -211,15 +221,15 @@ def layernorm_backward(dy, x, eps: float, gamma=None, ddof: int = 0, residual=No
     code, fn = {torch.float32: (DTYPE_F32, lib.ko_layernorm_backward_f32), torch.float16: (DTYPE_F16, lib.ko_layernorm_backward_f16),
                 torch.bfloat16: (DTYPE_BF16, lib.ko_layernorm_backward_bf16)}[x.dtype]
     with _on(x.device, stream):
-        dx = torch.empty_like(x, memory_format=torch.contiguous_format) if dx is None else dx
+        dx = torch.empty(rows, cols, dtype=x.dtype, device=x.device) if dx is None else dx
         dgamma = torch.empty(cols, dtype=torch.float32, device=x.device) if dgamma is None else dgamma
         dbeta = torch.empty(cols, dtype=torch.float32, device=x.device) if dbeta is None else dbeta
-        ws = _workspace(_layernorm_backward_bytes(x.device.index, code, rows, cols), x.device)
+        ws, ws_at, ws_bytes = _workspace(_layernorm_backward_bytes(x.device.index, code, rows, cols), x.device)
         native.check(fn(_operand(dy, "dy", x.device, same, (rows, cols)), _ptr(x), _operand(dx, "dx", x.device, same, (rows, cols)), rows,
                         cols, eps, _operand(gamma, "gamma", x.device, same, (cols,)),
                         _operand(residual, "residual", x.device, same, (rows, cols)),
                         _operand(dgamma, "dgamma", x.device, vector, (cols,)), _operand(dbeta, "dbeta", x.device, vector, (cols,)), ddof,
-                        _ptr(ws), 0 if ws is None else ws.numel(), _current_stream_ptr()), "ko_layernorm_backward")
+                        ws_at, ws_bytes, _current_stream_ptr()), "ko_layernorm_backward")
     return dx, dgamma, dbeta
 
 
@@ -329,15 +339,14 @@ def linear(x, w, bias=None, activation: str = "none", residual=None, out=None, o
         raise ValueError(f"w must have 2 dimensions, got {w.dim()}")
     (m, k), n = x.shape, w.shape[0]
     with _on(device, stream):
-        out = torch.empty((m, n), dtype=out_dtype, device=device) if out is None else out
+        out = torch.empty(m, n, dtype=out_dtype, device=device) if out is None else out
         if return_pre and pre is None:
-            pre = torch.empty((m, n), dtype=x.dtype, device=device)
-        ws = _workspace(_linear_bytes(device.index, "ko_linear_workspace", m, n, k), device)
+            pre = torch.empty(m, n, dtype=x.dtype, device=device)
+        ws, ws_at, ws_bytes = _workspace(_linear_bytes(device.index, "ko_linear_workspace", m, n, k), device)
         native.check(native.lib().ko_linear(in_fmt, out_fmt, act, m, n, k, _ptr(x), _operand(w, "w", device, same, (n, k)),
                                             _operand(bias, "bias", device, same, (n,)), _operand(residual, "residual", device, to, (m, n)),
                                             _operand(out, "out", device, to, (m, n)), _operand(pre, "pre", device, same, (m, n)),
-                                            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
-                                            _current_stream_ptr()), "ko_linear")
+                                            ws_at, ws_bytes, _current_stream_ptr()), "ko_linear")
     return out if pre is None else (out, pre)
 
 
@@ -357,12 +366,11 @@ def linear_backward_input(dy, w, pre=None, activation: str = "none", out=None, o
         raise ValueError(f"w must have 2 dimensions, got {w.dim()}")
     (m, n), k = dy.shape, w.shape[1]
     with _on(device, stream):
-        out = torch.empty((m, k), dtype=out_dtype, device=device) if out is None else out
-        ws = _workspace(_linear_bytes(device.index, "ko_linear_backward_input_workspace", m, n, k), device)
+        out = torch.empty(m, k, dtype=out_dtype, device=device) if out is None else out
+        ws, ws_at, ws_bytes = _workspace(_linear_bytes(device.index, "ko_linear_backward_input_workspace", m, n, k), device)
         native.check(native.lib().ko_linear_backward_input(
             in_fmt, out_fmt, act, m, n, k, _ptr(dy), _operand(w, "w", device, same, (n, k)), _operand(pre, "pre", device, same, (m, k)),
-            _operand(out, "out", device, (out_dtype,), (m, k)), None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
-            _current_stream_ptr()), "ko_linear_backward_input")
+            _operand(out, "out", device, (out_dtype,), (m, k)), ws_at, ws_bytes, _current_stream_ptr()), "ko_linear_backward_input")
     return out
 
 
@@ -381,12 +389,12 @@ def linear_backward_weight(dy, x, c=None, out=None, out_dtype=None, return_bias:
         raise ValueError(f"x must have 2 dimensions, got {x.dim()}")
     (m, n), k = dy.shape, x.shape[1]
     with _on(device, stream):
-        out = torch.empty((n, k), dtype=out_dtype, device=device) if out is None else out
+        out = torch.empty(n, k, dtype=out_dtype, device=device) if out is None else out
         if return_bias and dbias is None:
             dbias = torch.empty(n, dtype=torch.float32, device=device)
-        ws = _workspace(_linear_bytes(device.index, "ko_linear_backward_weight_workspace", m, n, k), device)
+        ws, ws_at, ws_bytes = _workspace(_linear_bytes(device.index, "ko_linear_backward_weight_workspace", m, n, k), device)
         native.check(native.lib().ko_linear_backward_weight(
             in_fmt, out_fmt, m, n, k, _ptr(dy), _operand(x, "x", device, (dy.dtype,), (m, k)), _operand(c, "c", device, to, (n, k)),
             _operand(out, "out", device, to, (n, k)), _operand(dbias, "dbias", device, (torch.float32,), (n,)),
-            None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _current_stream_ptr()), "ko_linear_backward_weight")
+            ws_at, ws_bytes, _current_stream_ptr()), "ko_linear_backward_weight")
     return out if dbias is None else (out, dbias)
