@@ -72,6 +72,20 @@ int ko_sgemm_f32_tuned(int64_t M, int64_t N, int64_t K, const float *A, const fl
 int ko_gemm_tc_tuned(int fmt, int out_fmt, int b_row_major, int64_t M, int64_t N, int64_t K, const void *A, const void *B,
                      const void *C, void *D, int bn, int store_mode, void *stream);
 
+/* the linear layer's calls with a pinned plan: tile 0 = choose, 128 / 256 = columns of D per 128-row tile of one CTA, 2048 = a
+ * pair of CTAs per 256 x 256 tile (both only where D can be stored by TMA); slices: with a pinned tile, K slices (0 / 1 = none,
+ * at most 64; not for 2048), for which the workspace must hold slices * tiles * 128 * tile floats; a pinned tile also takes the
+ * forward call past the few-token kernel */
+int ko_linear_tuned(int in_fmt, int out_fmt, int activation, int64_t M, int64_t N, int64_t K, const void *X, const void *W,
+                    const void *bias, const void *residual, void *Y, void *Z, void *workspace, size_t workspace_bytes, int tile,
+                    int slices, void *stream);
+int ko_linear_backward_input_tuned(int in_fmt, int out_fmt, int activation, int64_t M, int64_t N, int64_t K, const void *dY,
+                                   const void *W, const void *Z, void *dX, void *workspace, size_t workspace_bytes, int tile,
+                                   int slices, void *stream);
+int ko_linear_backward_weight_tuned(int in_fmt, int out_fmt, int64_t M, int64_t N, int64_t K, const void *dY, const void *X,
+                                    const void *C, void *dW, float *dbias, void *workspace, size_t workspace_bytes, int tile,
+                                    int slices, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

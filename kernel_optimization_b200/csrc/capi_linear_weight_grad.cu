@@ -1,5 +1,6 @@
 // C-ABI launchers of the linear layer's gradients with respect to its weight and bias.
 #include "linear_launch.h"
+#include "../../include/ko_b200_tuning.h"
 
 namespace {
 
@@ -32,23 +33,8 @@ int column_sum(const void *in, int64_t rows, int cols, float *partials, float *o
     return ko::launch_overlapped(ko::column_fold_kernel<>, (unsigned)((cols + 31) / 32), 256u, (size_t)0, s, (const float *)partials, chunks, cols, out);
 }
 
-}  // namespace
-
-extern "C" {
-
-int ko_linear_backward_weight_workspace(int64_t M, int64_t N, int64_t K, size_t *bytes) {
-    KO_REQUIRE(bytes != nullptr, KO_ERR_INVALID_ARG, "linear backward weight: NULL bytes");
-    *bytes = 0;
-    if (int st = ko::check_linear("linear backward weight", 0, 0, 0, M, N, K)) return st;
-    if (M == 0 || N == 0) return KO_OK;
-    ko::DeviceInfo info;
-    if (int st = ko::current_device_info(&info)) return st;
-    *bytes = round16(ko::product_workspace(N, K, M, info.sm_count)) + column_bytes(M, N, info.sm_count);
-    return KO_OK;
-}
-
-int ko_linear_backward_weight(int in_fmt, int out_fmt, int64_t M, int64_t N, int64_t K, const void *dY, const void *X, const void *C,
-                              void *dW, float *dbias, void *workspace, size_t workspace_bytes, void *stream) {
+int dispatch(int in_fmt, int out_fmt, int64_t M, int64_t N, int64_t K, const void *dY, const void *X, const void *C,
+                              void *dW, float *dbias, void *workspace, size_t workspace_bytes, void *stream, const ko::PinnedPlan &pin) {
     const char *name = "linear backward weight";
     if (int st = ko::check_linear(name, in_fmt, out_fmt, 0, M, N, K)) return st;
     if (N == 0) return KO_OK;
@@ -70,7 +56,10 @@ int ko_linear_backward_weight(int in_fmt, int out_fmt, int64_t M, int64_t N, int
     KO_REQUIRE(dW != dY && dW != X && (dbias == nullptr || (const void *)dbias != dW), KO_ERR_INVALID_ARG, "%s: outputs must not alias the inputs or each other", name);
     ko::DeviceInfo info;
     if (int st = ko::current_device_info(&info)) return st;
-    const size_t product_bytes = round16(ko::product_workspace(N, K, M, info.sm_count)), sum_bytes = column_bytes(M, N, info.sm_count);
+    size_t product_bytes = round16(ko::product_workspace(N, K, M, info.sm_count));
+    if (pin.slices > 1)  // the bias gradient's part lies behind the product's
+        product_bytes = std::max(product_bytes, (size_t)((N + 127) / 128) * ((K + pin.tile - 1) / pin.tile) * pin.slices * 128 * pin.tile * sizeof(float));
+    const size_t sum_bytes = column_bytes(M, N, info.sm_count);
     const size_t need = product_bytes + sum_bytes;
     KO_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), KO_ERR_INVALID_ARG, "%s: the workspace needs %zu bytes, got %zu", name,
                need, workspace ? workspace_bytes : (size_t)0);
@@ -85,8 +74,35 @@ int ko_linear_backward_weight(int in_fmt, int out_fmt, int64_t M, int64_t N, int
     p.M = (int)N; p.N = (int)K; p.K = (int)M;  // the product's shape
     p.D = dW; p.fmt = in_fmt; p.out_fmt = out_fmt; p.b_row_major = 1;
     p.extra = C;
-    return out_fmt ? ko::run_product<ko::LinearMode::kWeightGrad, true>(p, dY, X, workspace, product_bytes, s, info, name)
-                   : ko::run_product<ko::LinearMode::kWeightGrad, false>(p, dY, X, workspace, product_bytes, s, info, name);
+    return out_fmt ? ko::run_product<ko::LinearMode::kWeightGrad, true>(p, dY, X, workspace, product_bytes, s, info, name, pin)
+                   : ko::run_product<ko::LinearMode::kWeightGrad, false>(p, dY, X, workspace, product_bytes, s, info, name, pin);
+}
+
+}  // namespace
+
+extern "C" {
+
+int ko_linear_backward_weight_workspace(int64_t M, int64_t N, int64_t K, size_t *bytes) {
+    KO_REQUIRE(bytes != nullptr, KO_ERR_INVALID_ARG, "linear backward weight: NULL bytes");
+    *bytes = 0;
+    if (int st = ko::check_linear("linear backward weight", 0, 0, 0, M, N, K)) return st;
+    if (M == 0 || N == 0) return KO_OK;
+    ko::DeviceInfo info;
+    if (int st = ko::current_device_info(&info)) return st;
+    *bytes = round16(ko::product_workspace(N, K, M, info.sm_count)) + column_bytes(M, N, info.sm_count);
+    return KO_OK;
+}
+
+int ko_linear_backward_weight(int in_fmt, int out_fmt, int64_t M, int64_t N, int64_t K, const void *dY, const void *X, const void *C,
+                              void *dW, float *dbias, void *workspace, size_t workspace_bytes, void *stream) {
+    return dispatch(in_fmt, out_fmt, M, N, K, dY, X, C, dW, dbias, workspace, workspace_bytes, stream, {});
+}
+
+int ko_linear_backward_weight_tuned(int in_fmt, int out_fmt, int64_t M, int64_t N, int64_t K, const void *dY, const void *X, const void *C,
+                                    void *dW, float *dbias, void *workspace, size_t workspace_bytes, int tile, int slices, void *stream) {
+    KO_REQUIRE(tile == 0 || tile == 128 || tile == 256 || tile == 2048, KO_ERR_INVALID_ARG, "linear backward weight: tile code %d not in {128,256,2048}", tile);
+    KO_REQUIRE(slices == 0 || tile != 0, KO_ERR_INVALID_ARG, "linear backward weight: slices need a tile code");
+    return dispatch(in_fmt, out_fmt, M, N, K, dY, X, C, dW, dbias, workspace, workspace_bytes, stream, {tile, slices});
 }
 
 }  // extern "C"

@@ -24,8 +24,11 @@ struct ProductPlan {
 };
 
 // tma: D can be stored by TMA; without it only the 128 x 128 tile is built.  Modelled microseconds per candidate: start,
-// then rounds of work units x K-blocks of 64 x time per K-block; slices add a second kernel and the partial tiles' way
-// through the L2 (written once, read once).
+// then rounds of work units x (K-blocks of 64 x time per K-block + time between tiles); slices add a second kernel and the
+// partial tiles' way through the L2 (written once, read once) at 5 TB/s.  Fitted to
+// forced plans, BF16, measured (modelled): 16384 x 4096 x 1024 pair 103 (102), 128 x 256 110 (111), 128 x 128 164 (173);
+// 4096^3 93 (96), 102 (103), 142 (144); 8192 x 768 x 768 16.6 (14.9), 17.4 (15.7), 18.2 (18.0); 2048 x 1024 x 1024 13.6 (12.3),
+// 14.0 (11.0), 11.1 (9.1); 768 x 768 x 8192 in four slices of 128-wide tiles 20.2 (20.2), in eight of 256-wide ones 21.3 (21.1).
 inline ProductPlan plan_product(int64_t M, int64_t N, int64_t K, bool tma, int sms) {
     const long long k_blocks = (K + tc::kBK - 1) / tc::kBK;
     ProductPlan best{false, 128, 1, 0};
@@ -33,17 +36,21 @@ inline ProductPlan plan_product(int64_t M, int64_t N, int64_t K, bool tma, int s
     if (tma && M > 128 && N > 128) {
         const long long tiles = ((M + 255) / 256) * ((N + 255) / 256);
         const long long rounds = (tiles + sms / 2 - 1) / (sms / 2);
-        best_cost = 4.0 + (double)rounds * (double)k_blocks * 0.35;
+        best_cost = 4.5 + (double)rounds * ((double)k_blocks * 0.335 + 1.7);
         best = {true, 256, 1, tiles};
     }
     for (int bn : {128, 256}) {
         if (bn == 256 && (!tma || N <= 128)) continue;
+        const double per_block = bn == 256 ? 0.36 : 0.29, per_tile = bn == 256 ? 1.9 : 1.5, start = bn == 256 ? 4.3 : 3.0;
         const long long tiles = ((M + 127) / 128) * ((N + bn - 1) / bn);
         const long long most = std::min<long long>(std::max<long long>(sms / tiles, 1), std::max<long long>(k_blocks / 4, 1));
         for (int split = 1; split <= most && split <= 64; ++split) {
             const long long rounds = (tiles * split + sms - 1) / sms;
-            double cost = 3.3 + (double)rounds * (double)((k_blocks + split - 1) / split) * (bn == 256 ? 0.31 : 0.26);
-            if (split > 1) cost += 3.0 + (2.0 * split + 1.0) * (double)M * (double)N * 4.0 / 5e6;
+            double cost = start + (double)rounds * ((double)((k_blocks + split - 1) / split) * per_block + per_tile);
+            if (split > 1) {
+                const double written = (double)((M + 31) / 32 * 32) * N * split, read = (double)M * N * split;
+                cost += 2.2 + (written + read + (double)M * N) * 4.0 / 5e6;
+            }
             if (cost < best_cost) {
                 best_cost = cost;
                 best = {false, bn, split, tiles};
@@ -51,6 +58,26 @@ inline ProductPlan plan_product(int64_t M, int64_t N, int64_t K, bool tma, int s
         }
     }
     return best;
+}
+
+// a plan pinned by a tuning call: tile 0 = choose, 128 / 256 = columns of a CTA's tile, 2048 = the pair of CTAs; slices 0 =
+// choose (1 with a pinned tile)
+struct PinnedPlan {
+    int tile = 0, slices = 0;
+};
+inline int pin_product(const PinnedPlan &pin, int64_t M, int64_t N, int64_t K, bool tma, const char *name, ProductPlan *plan) {
+    if (pin.tile == 0 && pin.slices == 0) return KO_OK;
+    KO_REQUIRE(pin.tile == 128 || pin.tile == 256 || pin.tile == 2048, KO_ERR_INVALID_ARG, "%s: tile code %d not in {128,256,2048}", name, pin.tile);
+    KO_REQUIRE(tma || pin.tile == 128, KO_ERR_SHAPE, "%s: without TMA stores there is only the 128-column tile", name);
+    const long long k_blocks = (K + tc::kBK - 1) / tc::kBK;
+    KO_REQUIRE(pin.slices >= 0 && pin.slices <= 64 && pin.slices <= k_blocks && (pin.tile != 2048 || pin.slices <= 1), KO_ERR_INVALID_ARG,
+               "%s: %d K slices out of range", name, pin.slices);
+    plan->pair = pin.tile == 2048;
+    plan->bn = plan->pair ? 256 : pin.tile;
+    plan->split = pin.slices > 1 ? pin.slices : 1;
+    const int rows = plan->pair ? 256 : 128;
+    plan->tiles = ((M + rows - 1) / rows) * ((N + plan->bn - 1) / plan->bn);
+    return KO_OK;
 }
 
 // room for either way a call may store D
@@ -78,7 +105,7 @@ inline int resident_pairs_of(const void *kernel, unsigned threads, size_t smem, 
 
 template <class Epi, int BN, bool kTmaStore>
 int launch_product_tile(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &md, const LinearParams &p, int sms, cudaStream_t s) {
-    using Cfg = tc::TileConfig<BN>;
+    using Cfg = typename tc::TileConfigFor<BN, 1, 2, Epi>::type;
     auto kernel = tc::gemm_tcgen05_kernel<BN, kTmaStore, 1, 2, Epi>;
     if (int st = ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), Cfg::kSmemBytes)) return st;
     const long long units = (long long)((p.M + 127) / 128) * ((p.N + BN - 1) / BN) * p.split_k;
@@ -87,7 +114,7 @@ int launch_product_tile(const CUtensorMap &ma, const CUtensorMap &mb, const CUte
 
 template <class Epi>
 int launch_product_pair(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &md, const LinearParams &p, cudaStream_t s) {
-    using Cfg = tc::PairConfig;
+    using Cfg = typename tc::PairConfigFor<Epi>::type;
     auto kernel = tc::gemm_tcgen05_pair_kernel<true, Epi>;
     const void *id = reinterpret_cast<const void *>(kernel);
     constexpr unsigned threads = 64u + 32u * Epi::kWarps;
@@ -104,18 +131,19 @@ int launch_product_pair(const CUtensorMap &ma, const CUtensorMap &mb, const CUte
 // Everything has been checked but the workspace.
 template <LinearMode kMode, bool kOut16>
 int run_product(LinearParams p, const void *A, const void *B, void *workspace, size_t workspace_bytes, cudaStream_t s, const DeviceInfo &info,
-                const char *name) {
+                const char *name, const PinnedPlan &pin = {}) {
     using Epi = LinearEpilogue<kMode, kOut16>;
     EncodeTiledFn encode = nullptr;
     if (int st = get_encode_fn(&encode)) return st;
-    const bool tma = p.N % (kOut16 ? 8 : 4) == 0 && aligned16(p.D) && (p.pre == nullptr || (p.N % 8 == 0 && aligned16(p.pre)));
-    const ProductPlan plan = plan_product(p.M, p.N, p.K, tma, info.sm_count);
-    const size_t need = product_workspace(p.M, p.N, p.K, info.sm_count);
+    // 16-byte row pitches and bases of everything the epilogue touches: TMA and vector loads; else its row-wise form
+    const bool sixteen = kOut16 || p.pre || p.bias || (p.extra && Epi::kExtra16);
+    const bool tma = p.N % (sixteen ? 8 : 4) == 0 && aligned16(p.D) && aligned16(p.pre) && aligned16(p.bias) && aligned16(p.extra);
+    ProductPlan plan = plan_product(p.M, p.N, p.K, tma, info.sm_count);
+    if (int st = pin_product(pin, p.M, p.N, p.K, tma, name, &plan)) return st;
+    const size_t need = std::max(plan.bytes(), product_workspace(p.M, p.N, p.K, info.sm_count));
     KO_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), KO_ERR_INVALID_ARG, "%s: the workspace needs %zu bytes, got %zu",
                name, need, workspace ? workspace_bytes : (size_t)0);
     KO_REQUIRE(aligned16(workspace), KO_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", name);
-    p.extra_vec = p.extra && aligned16(p.extra) && p.N % (Epi::kExtra16 ? 8 : 4) == 0;
-    p.bias_vec = p.bias && aligned16(p.bias) && p.N % 8 == 0;
     p.C = nullptr;
     p.tiles_n = p.wide_tiles_n = p.bn_wide = p.bn_narrow = 0;
     p.split_k = plan.split;
@@ -134,11 +162,13 @@ int run_product(LinearParams p, const void *A, const void *B, void *workspace, s
         if (int st = make_map(encode, &map_b, p.fmt, B, p.N, p.K, plan.pair ? 128 : plan.bn)) return st;
     }
     map_d = map_a;  // unused by the direct-store epilogue
-    p.map_pre = map_a;
+    p.map_pre = p.map_extra = map_a;
     if (tma) {
-        if (int st = make_store_map(encode, &map_d, p.out_fmt, p.D, p.M, p.N)) return st;
+        if (int st = make_store_map(encode, &map_d, p.out_fmt, p.D, p.M, p.N, Epi::kChunk)) return st;
         if (p.pre)
-            if (int st = make_store_map(encode, &p.map_pre, p.fmt + 1, p.pre, p.M, p.N)) return st;
+            if (int st = make_store_map(encode, &p.map_pre, p.fmt + 1, p.pre, p.M, p.N, Epi::kChunk)) return st;
+        if (p.extra)
+            if (int st = make_store_map(encode, &p.map_extra, Epi::kExtra16 ? p.fmt + 1 : 0, const_cast<void *>(p.extra), p.M, p.N, Epi::kChunk)) return st;
     }
     int st;
     if (plan.pair) st = launch_product_pair<Epi>(map_a, map_b, map_d, p, s);

@@ -60,18 +60,19 @@ inline int make_map_b_row_major(EncodeTiledFn encode, CUtensorMap *map, int fmt,
     return KO_OK;
 }
 
-// [M, N] row-major output, boxes of 32 rows x 32 columns: FP32 rows of 128 bytes with the 128-byte swizzle,
-// 16-bit rows of 64 bytes with the 64-byte swizzle
-inline int make_store_map(EncodeTiledFn encode, CUtensorMap *map, int out_fmt, void *D, int64_t M, int64_t N) {
+// [M, N] row-major output (or an operand read in the same shape), boxes of 32 rows x 32 columns: FP32 rows of 128 bytes with
+// the 128-byte swizzle, 16-bit rows of 64 bytes with the 64-byte swizzle; 64 columns of 16 bits: 128 bytes again
+inline int make_store_map(EncodeTiledFn encode, CUtensorMap *map, int out_fmt, void *D, int64_t M, int64_t N, int columns = 32) {
     const cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)M};
     const cuuint64_t strides[1] = {(cuuint64_t)N * (out_fmt == 0 ? 4 : 2)};
-    const cuuint32_t box[2] = {32, 32};
+    const cuuint32_t box[2] = {(cuuint32_t)columns, 32};
     const cuuint32_t elem_strides[2] = {1, 1};
     const CUtensorMapDataType dt = out_fmt == 0   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : out_fmt == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                   : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     const CUresult r = encode(map, dt, 2, D, dims, strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              out_fmt == 0 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                              columns * (out_fmt == 0 ? 4 : 2) == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                              CU_TENSOR_MAP_L2_PROMOTION_NONE,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     KO_REQUIRE(r == CUDA_SUCCESS, KO_ERR_CUDA, "cuTensorMapEncodeTiled (D) failed with CUresult %d", (int)r);
     return KO_OK;

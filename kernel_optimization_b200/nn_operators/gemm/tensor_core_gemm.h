@@ -60,7 +60,8 @@ enum : unsigned { kStatusOk = 0, kTimeoutProducer = 1, kTimeoutMma = 2, kTimeout
 // kBoxes: staging boxes per epilogue warp for the TMA stores of D (a store keeps its box until it has been read out
 // of shared memory).  Two are in use; four, paid for with one stage of the operand ring, measured slower at every
 // shape (FFN 16384 x 3072 x 768: 80.4 against 78.8 us), so the stores in flight are not what limits the epilogue.
-template <int BN, int MT = 1, int kBoxes = 2>
+// kStagingBytes: shared memory of the epilogue's boxes
+template <int BN, int MT = 1, int kBoxes = 2, int kStagingBytes = 4 * kBoxes * 32 * 32 * 4>
 struct TileConfig {
     static constexpr int kBN = BN;
     static constexpr int kBytesA = MT * kBM * kBK * 2;
@@ -71,7 +72,7 @@ struct TileConfig {
     // epilogue staging for TMA stores: per epilogue warp kBoxes 32-row x 32-column FP32 boxes (4 KB each)
     static constexpr int kStoreBoxes = kBoxes;
     static constexpr int kStoreBoxBytes = 32 * 32 * 4;
-    static constexpr int kStoreBytes = 4 * kBoxes * kStoreBoxBytes;
+    static constexpr int kStoreBytes = kStagingBytes;
     static constexpr int kSmemLimit = 232448;  // 227 KB: the most one CTA may use
     // + 1024 so the stage ring can be aligned to the 1024-byte swizzle period; as many stages as fit, at most 6
     static constexpr int kFit = (kSmemLimit - 1024 - kBarrierBytes - kStoreBytes) / kStageBytes;
@@ -252,12 +253,21 @@ struct PlainEpilogue {
 };
 
 template <class Epi, bool kFused = Epi::kFused>
-struct FusedOperands {
+struct FusedState {
     struct type {};
 };
 template <class Epi>
-struct FusedOperands<Epi, true> {
-    using type = typename Epi::Operands;
+struct FusedState<Epi, true> {
+    using type = typename Epi::State;
+};
+// the tile configuration that goes with an epilogue
+template <int BN, int MT, int kBoxes, class Epi, bool kFused = Epi::kFused>
+struct TileConfigFor {
+    using type = TileConfig<BN, MT, kBoxes>;
+};
+template <int BN, int MT, int kBoxes, class Epi>
+struct TileConfigFor<BN, MT, kBoxes, Epi, true> {
+    using type = TileConfig<BN, MT, kBoxes, Epi::kWarps * Epi::kBoxesPerWarp * (int)Epi::kBoxBytes>;
 };
 
 // where column tile tn starts and how wide it is
@@ -474,7 +484,7 @@ __global__ void __launch_bounds__(64 + 32 * Epi::kWarps, 1)
 gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                     const __grid_constant__ CUtensorMap map_b_narrow, const __grid_constant__ CUtensorMap map_d,
                     const __grid_constant__ typename Epi::Params p) {
-    using Cfg = TileConfig<BN, MT, kBoxes>;
+    using Cfg = typename TileConfigFor<BN, MT, kBoxes, Epi>::type;
     constexpr int kTileM = MT * kBM;
     extern __shared__ uint8_t ko_tc_smem_raw[];
     // stage ring on a 1024-byte boundary (swizzle period), barriers behind it
@@ -491,6 +501,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     const uint32_t drain_bar = bar_base + 8u * (2 * Cfg::kStages + 4);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * Cfg::kStages + 5);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    [[maybe_unused]] auto fused_bar = [&](int w) { return bar_base + 8u * (2 * Cfg::kStages + 7 + w); };  // behind the two words above
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int tiles_m = (p.M + kTileM - 1) / kTileM, tiles_n = p.tiles_n ? p.tiles_n : (p.N + BN - 1) / BN;
@@ -519,6 +530,8 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             mbar_init(acc_free_bar(a), Epi::kWarps);  // one arrival per epilogue warp
         }
         mbar_init(drain_bar, 1);
+        if constexpr (Epi::kFused)
+            for (int w = 0; w < Epi::kWarps; ++w) mbar_init(fused_bar(w), 1);
         *abort_flag = 0;
         fence_barrier_init();
         fence_proxy_async();
@@ -651,11 +664,15 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     } else {
         // ------------------------------------------------------------------ epilogue (warps 2..)
         const int quad = warp & 3;  // TMEM lanes [32*quad, 32*quad+32) are the ones this warp may read
-        const int c_begin = ((warp - 2) >> 2) * 32;          // warps that share a quadrant take its 32-column chunks in turn
-        constexpr int c_step = 8 * Epi::kWarps;
+        // warps that share a quadrant take its column chunks in turn
+        [[maybe_unused]] const int share = (warp - 2) >> 2;
         uint32_t local_tile = 0;
         uint32_t store_seq = 0;  // TMA stores issued by this warp so far: store n uses staging box n % kBoxes
-        [[maybe_unused]] typename FusedOperands<Epi>::type operands;
+        [[maybe_unused]] typename FusedState<Epi>::type fused;
+        if constexpr (Epi::kFused) {
+            fused.boxes = store_base + (uint32_t)((warp - 2) * Epi::kBoxesPerWarp) * Epi::kBoxBytes;
+            fused.bar = fused_bar(warp - 2);
+        }
         bool ok = true;
         for (long long u = blockIdx.x; u < num_units && ok; u += gridDim.x, ++local_tile) {
             long long t;
@@ -664,8 +681,8 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             tile_of(p, t, tiles_m, tiles_n, tm, tn);
             column_tile<BN>(p, tn, col0, bn);
             const uint32_t acc = MT == 1 ? (local_tile & 1u) : 0u, acc_phase = (MT == 1 ? (local_tile >> 1) : local_tile) & 1u;
-            if constexpr (Epi::kFused)  // the first chunk's operands arrive while the tile is still being computed
-                if (split == 1) Epi::load(operands, p, tm * kTileM + quad * 32 + lane, col0 + c_begin);
+            if constexpr (Epi::kFused)  // the first chunk's operand arrives while the tile is still being computed
+                if (kTmaStore && split == 1) Epi::bring(fused, p, tm * kTileM + quad * 32, col0 + share * Epi::kChunk, lane);
             if (!mbar_wait(acc_ready_bar(acc), acc_phase, abort_flag)) {
                 if (lane == 0 && !*abort_flag) atomicCAS(p.status, kStatusOk, kTimeoutEpilogue);
                 *abort_flag = 1;
@@ -680,13 +697,19 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
 #pragma unroll 1
                 for (int half = 0; half < MT; ++half) {
                     const uint32_t t_row = tmem_base + ((uint32_t)(quad * 32) << 16) + (MT == 1 ? acc * BN : half * BN);
-                    publish_block(slot + ((size_t)((half * 4 + quad) * (BN / 32)) << 10), t_row, bn, lane, c_begin, c_step);
+                    if (Epi::kFused && tm * kTileM + half * kBM + quad * 32 >= p.M) continue;  // rows that nobody adds
+                    publish_block(slot + ((size_t)((half * 4 + quad) * (BN / 32)) << 10), t_row, bn, lane, share * 32, 8 * Epi::kWarps);
                 }
             } else if constexpr (Epi::kFused) {
                 static_assert(!Epi::kFused || MT == 1, "fused epilogues: 128-row tiles");
                 const uint32_t t_row = tmem_base + ((uint32_t)(quad * 32) << 16) + acc * BN;
-                Epi::template block<kTmaStore>(&map_d, p, operands, t_row, tm * kTileM + quad * 32, col0, bn, c_begin, lane,
-                                               store_base + (uint32_t)(warp - 2) * (uint32_t)(Cfg::kStoreBytes / Epi::kWarps), store_seq);
+                if (!Epi::template block<kTmaStore>(&map_d, p, fused, t_row, tm * kTileM + quad * 32, col0, bn, share * Epi::kChunk, lane,
+                                                    abort_flag)) {
+                    if (lane == 0 && !*abort_flag) atomicCAS(p.status, kStatusOk, kTimeoutEpilogue);
+                    *abort_flag = 1;
+                    ok = false;
+                    break;
+                }
             } else {
 #pragma unroll 1
                 for (int half = 0; half < MT; ++half) {
@@ -702,7 +725,8 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             if (lane == 0) mbar_arrive(acc_free_bar(acc));
         }
         // shared memory must outlive the reads of the stores still in flight
-        if (kTmaStore && lane == 0) bulk_wait_group_read<0>();
+        if constexpr (Epi::kFused) Epi::finish(fused, lane);
+        else if (kTmaStore && lane == 0) bulk_wait_group_read<0>();
         __syncwarp();
     }
 

@@ -30,19 +30,31 @@
 namespace ko {
 namespace tc {
 
-struct PairConfig {
+// kStagingBytes: shared memory of the epilogue's boxes; as many stages of operands as fit beside it, at most 6
+template <int kStagingBytes>
+struct PairConfigOf {
     static constexpr int kBN = 256;                          // widest tile; TMEM holds two accumulators of it
     static constexpr int kBytesA = kBM * kBK * 2;            // this CTA's 128 rows
     static constexpr int kBytesB = (kBN / 2) * kBK * 2;      // this CTA's half of the B tile, at most
     static constexpr int kStageBytes = kBytesA + kBytesB;    // 32 KB
-    static constexpr int kStages = 6;
     static constexpr int kTmemCols = 2 * kBN;
     static constexpr int kStoreBoxes = 2;
     static constexpr int kStoreBoxBytes = 32 * 32 * 4;
-    static constexpr int kStoreBytes = 4 * kStoreBoxes * kStoreBoxBytes;
+    static constexpr int kStoreBytes = kStagingBytes;
     static constexpr int kBarrierBytes = 256;
+    static constexpr int kFit = (232448 - 1024 - kBarrierBytes - kStoreBytes) / kStageBytes;
+    static constexpr int kStages = kFit > 6 ? 6 : kFit;
     static constexpr int kSmemBytes = kStages * kStageBytes + kStoreBytes + kBarrierBytes + 1024;
-    static_assert(kSmemBytes <= 232448, "stage ring exceeds the shared memory of an SM");
+    static_assert(kStages >= 2 && kSmemBytes <= 232448, "stage ring exceeds the shared memory of an SM");
+};
+using PairConfig = PairConfigOf<4 * 2 * 32 * 32 * 4>;
+template <class Epi, bool kFused = Epi::kFused>
+struct PairConfigFor {
+    using type = PairConfig;
+};
+template <class Epi>
+struct PairConfigFor<Epi, true> {
+    using type = PairConfigOf<Epi::kWarps * Epi::kBoxesPerWarp * (int)Epi::kBoxBytes>;
 };
 
 // ---- cta_group::2 forms of the PTX wrappers ----
@@ -110,7 +122,7 @@ __global__ void __launch_bounds__(64 + 32 * Epi::kWarps, 1)
 gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                          const __grid_constant__ CUtensorMap map_b_narrow, const __grid_constant__ CUtensorMap map_d,
                          const __grid_constant__ typename Epi::Params p) {
-    using Cfg = PairConfig;
+    using Cfg = typename PairConfigFor<Epi>::type;
     constexpr int BN = Cfg::kBN, kTileM = 2 * kBM;
     extern __shared__ uint8_t ko_tc_pair_smem_raw[];
     const uint32_t raw = smem_u32(ko_tc_pair_smem_raw);
@@ -126,6 +138,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     const uint32_t drain_bar = bar_base + 8u * (2 * Cfg::kStages + 4);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * Cfg::kStages + 5);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    [[maybe_unused]] auto fused_bar = [&](int w) { return bar_base + 8u * (2 * Cfg::kStages + 7 + w); };  // behind the two words above
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_cta_rank();  // 0 = leader
@@ -145,6 +158,8 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
             mbar_init(acc_free_bar(a), 2 * Epi::kWarps);  // the epilogue warps of each CTA
         }
         mbar_init(drain_bar, 1);
+        if constexpr (Epi::kFused)
+            for (int w = 0; w < Epi::kWarps; ++w) mbar_init(fused_bar(w), 1);
         *abort_flag = 0;
         fence_barrier_init();
         fence_proxy_async();
@@ -270,8 +285,12 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     } else {
         // ------------------------------------------------------------------ epilogue (warps 2.., both CTAs)
         const int quad = warp & 3;
-        [[maybe_unused]] const int c_begin = ((warp - 2) >> 2) * 32;
-        [[maybe_unused]] typename FusedOperands<Epi>::type operands;
+        [[maybe_unused]] const int share = (warp - 2) >> 2;
+        [[maybe_unused]] typename FusedState<Epi>::type fused;
+        if constexpr (Epi::kFused) {
+            fused.boxes = store_base + (uint32_t)((warp - 2) * Epi::kBoxesPerWarp) * Epi::kBoxBytes;
+            fused.bar = fused_bar(warp - 2);
+        }
         uint32_t local_tile = 0, store_seq = 0;
         bool ok = true;
         for (long long t = pair; t < num_tiles && ok; t += pairs, ++local_tile) {
@@ -280,7 +299,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
             column_tile<BN>(p, tn, col0, bn);
             const uint32_t acc = local_tile & 1u, acc_phase = (local_tile >> 1) & 1u;
             const int row_base = tm * kTileM + (int)rank * kBM + quad * 32;
-            if constexpr (Epi::kFused) Epi::load(operands, p, row_base + lane, col0 + c_begin);  // while the tile is being computed
+            if constexpr (Epi::kFused) Epi::bring(fused, p, row_base, col0 + share * Epi::kChunk, lane);  // while the tile is being computed
             if (!mbar_wait(acc_ready_bar(acc), acc_phase, abort_flag)) {
                 if (lane == 0 && !*abort_flag) atomicCAS(p.status, kStatusOk, kTimeoutEpilogue);
                 *abort_flag = 1;
@@ -289,9 +308,14 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
             }
             tc_fence_after();
             const uint32_t t_row = tmem_base + ((uint32_t)(quad * 32) << 16) + acc * BN;
-            if constexpr (Epi::kFused)
-                Epi::template block<kTmaStore>(&map_d, p, operands, t_row, row_base, col0, bn, c_begin, lane,
-                                               store_base + (uint32_t)(warp - 2) * (uint32_t)(Cfg::kStoreBytes / Epi::kWarps), store_seq);
+            if constexpr (Epi::kFused) {
+                if (!Epi::template block<kTmaStore>(&map_d, p, fused, t_row, row_base, col0, bn, share * Epi::kChunk, lane, abort_flag)) {
+                    if (lane == 0 && !*abort_flag) atomicCAS(p.status, kStatusOk, kTimeoutEpilogue);
+                    *abort_flag = 1;
+                    ok = false;
+                    break;
+                }
+            }
             else
                 epilogue_block<kTmaStore, Cfg::kStoreBoxes>(&map_d, p, t_row, row_base, col0, bn, lane,
                                                             store_base + (uint32_t)((warp - 2) * Cfg::kStoreBoxes) * Cfg::kStoreBoxBytes,
@@ -301,7 +325,8 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(map_to_cluster_rank(acc_free_bar(acc), 0));
         }
-        if (kTmaStore && lane == 0) bulk_wait_group_read<0>();
+        if constexpr (Epi::kFused) Epi::finish(fused, lane);
+        else if (kTmaStore && lane == 0) bulk_wait_group_read<0>();
         __syncwarp();
     }
 

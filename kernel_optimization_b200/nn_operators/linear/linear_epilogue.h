@@ -2,14 +2,13 @@
 //   forward        Y = act(X W^T + bias) + residual, and Z = X W^T + bias (16 bits) when the backward pass wants it
 //   input grad     dX = (dY W) * act'(Z)
 //   weight grad    dW = dY^T X + C   (A = dY stored [tokens, features]: MN-major operand)
-// An accumulator chunk of 32 rows x 32 columns stays in registers from tensor memory to the store; what it is combined
-// with (residual, Z or C: one row segment of 64 or 128 bytes per lane; the bias: the same 64 bytes for all lanes) is
-// loaded one chunk ahead, the first chunk's while the tile is still being multiplied.  Everything is FP32 until one
-// rounding to the stored type.  Eight epilogue warps, two per quadrant of TMEM lanes: an activation is 10 to 20
-// instructions an element, and four warps alone could not hide them behind the MMAs of the next tile.
+// An accumulator chunk of 32 rows x 128 bytes of output (64 columns of 16 bits, 32 of FP32) goes from tensor memory through
+// registers to a swizzled box in shared memory and out by one TMA store of full 128-byte lines.  What it is combined with
+// (residual, Z or C) comes the other way: one TMA load per chunk into a box of the warp's own, issued a chunk ahead -- the
+// first chunk's while the tile is still being multiplied -- so neither direction takes issue slots or L1 from the warps.
+// Everything is FP32 until one rounding to the stored type.  Eight epilogue warps, two per quadrant of TMEM lanes: an
+// activation costs about ten issue slots an element, which four warps alone could not hide behind the next tile's MMAs.
 #pragma once
-
-#include <type_traits>
 
 #include "../gemm/tensor_core_gemm.h"
 #include "activation.h"
@@ -23,8 +22,7 @@ struct LinearParams : tc::GemmParams {
     const void *extra;  // forward: residual, weight grad: C (both of D's type); input grad: Z (the inputs' type); may be null
     void *pre;          // forward: Z out (the inputs' type); may be null
     int activation;
-    int bias_vec, extra_vec;  // 16-byte accesses allowed: base aligned, row pitch a multiple of 16 bytes
-    alignas(64) CUtensorMap map_pre;
+    alignas(64) CUtensorMap map_pre, map_extra;
 };
 
 // two 16-bit values of type kBf16 ? BF16 : FP16 as FP32
@@ -48,7 +46,8 @@ __device__ __forceinline__ float widen16_at(const void *base, size_t i) {
 }
 
 // The same epilogue for one element, where speed does not depend on it: acc -> the value to be stored (before rounding);
-// Z is written here.
+// Z is written here.  (__fadd_rn: no contraction with an activation's last product, so that every form of the epilogue
+// gives the same bits.)
 template <LinearMode kMode, bool kBf16, bool kOut16>
 __device__ __forceinline__ float linear_finish_one(const LinearParams &p, float acc, int row, int col) {
     const size_t at = (size_t)row * p.N + col;
@@ -63,9 +62,9 @@ __device__ __forceinline__ float linear_finish_one(const LinearParams &p, float 
             const float z = widen16_at<kBf16>(p.extra, at);
             with_activation(p.activation, [&](auto act) { v *= activation_slope<act.value, !kOut16>(z); });
         } else if constexpr (kOut16) {
-            v += widen16_at<kBf16>(p.extra, at);
+            v = __fadd_rn(v, widen16_at<kBf16>(p.extra, at));
         } else {
-            v += static_cast<const float *>(p.extra)[at];
+            v = __fadd_rn(v, static_cast<const float *>(p.extra)[at]);
         }
     }
     return v;
@@ -84,158 +83,279 @@ struct LinearEpilogue {
     static constexpr bool kTransA = kMode == LinearMode::kWeightGrad;
     static constexpr bool kFused = true;
     static constexpr bool kExtra16 = kMode == LinearMode::kInputGrad || kOut16;
-    static constexpr int kExtraVecs = kExtra16 ? 4 : 8;  // 16-byte vectors per lane and chunk
-    // 4 KB of staging per warp: two boxes of 32 x 32 16-bit values, or one of FP32 (then Z, if any, takes its turn in it)
-    static constexpr int kBoxes = kOut16 ? 2 : 1;
-    static constexpr uint32_t kBoxBytes = kOut16 ? 2048 : 4096;
+    static constexpr int kChunk = kOut16 ? 64 : 32;           // columns
+    static constexpr int kStep = kChunk * (kWarps / 4);        // from one chunk of a warp to its next
+    static constexpr uint32_t kBoxBytes = 4096;
+    static constexpr int kBoxesPerWarp = 2;
 
-    struct Operands {
-        uint4 extra[kExtraVecs];
-        uint4 bias[4];
+    // a warp's boxes and mbarrier, and where it stands with them
+    struct State {
+        uint32_t boxes, bar;
+        uint32_t stores = 0;  // TMA stores issued
+        uint32_t phase = 0;   // of the extra operand's box
+        bool coming = false;  // an extra load has been issued and not waited for
     };
 
-    // 32 columns of row `row` from column `col` on; what lies outside the matrix is left at zero
-    __device__ __forceinline__ static void load(Operands &o, const Params &p, int row, int col) {
-#pragma unroll
-        for (int j = 0; j < kExtraVecs; ++j) o.extra[j] = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o.bias[j] = make_uint4(0u, 0u, 0u, 0u);
-        if (p.extra != nullptr && row < p.M) {
-            constexpr int kPer = kExtra16 ? 8 : 4;
-            const char *at = static_cast<const char *>(p.extra) + ((size_t)row * p.N + col) * (kExtra16 ? 2 : 4);
-            if (p.extra_vec) {
-#pragma unroll
-                for (int j = 0; j < kExtraVecs; ++j)
-                    if (col + j * kPer < p.N) o.extra[j] = *reinterpret_cast<const uint4 *>(at + j * 16);
-            } else {
-                load_singly<kExtraVecs, kExtra16>(o.extra, at, p.N - col);
-            }
+    // the extra operand's chunk at (row_base, col) on its way into box 1
+    __device__ __forceinline__ static void bring(State &st, const Params &p, int row_base, int col, int lane) {
+        if (p.extra == nullptr || row_base >= p.M || col >= p.N) return;
+        if (lane == 0) {
+            // a box is filled whole: what lies outside the matrix arrives as zeros and counts
+            mbar_expect_tx(st.bar, kExtra16 && !kOut16 ? kBoxBytes / 2 : kBoxBytes);
+            tc::tma_load_2d(st.boxes + kBoxBytes, &p.map_extra, col, row_base, st.bar);
         }
-        if constexpr (kMode == LinearMode::kForward) {
-            if (p.bias != nullptr) {
-                const char *at = static_cast<const char *>(p.bias) + (size_t)col * 2;
-                if (p.bias_vec) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (col + j * 8 < p.N) o.bias[j] = *reinterpret_cast<const uint4 *>(at + j * 16);
-                } else {
-                    load_singly<4, true>(o.bias, at, p.N - col);
+        st.coming = true;
+    }
+
+    // rows row_base .. + 31 of a tile (accumulator at TMEM address t_row), this warp's chunks c_begin, c_begin + kStep, ...
+    // to D and Z; false when a wait ran out
+    template <bool kTmaStore>
+    __device__ __forceinline__ static bool block(const CUtensorMap *map_d, const Params &p, State &st, uint32_t t_row, int row_base, int col0,
+                                                 int bn, int c_begin, int lane, volatile int *abort_flag) {
+#pragma unroll 1
+        for (int c0 = c_begin; c0 < bn; c0 += kStep) {
+            if (row_base >= p.M || col0 + c0 >= p.N) break;
+            if constexpr (kTmaStore) {
+                if (st.coming) {
+                    if (!mbar_wait(st.bar, st.phase, abort_flag)) return false;
+                    st.phase ^= 1u;
+                    st.coming = false;
+                }
+                if (p.fmt) chunk<true>(map_d, p, st, t_row + c0, row_base, col0 + c0, c0 + kStep < bn, lane);
+                else chunk<false>(map_d, p, st, t_row + c0, row_base, col0 + c0, c0 + kStep < bn, lane);
+            } else {
+#pragma unroll 1
+                for (int h = 0; h < kChunk; h += 32) {
+                    uint32_t r[32];
+                    tc::tmem_ld_32x32_issue(t_row + c0 + h, r);
+                    tc::tmem_ld_wait();
+                    if (p.fmt) chunk_by_rows<true>(p, r, row_base, col0 + c0 + h, lane, st.boxes);
+                    else chunk_by_rows<false>(p, r, row_base, col0 + c0 + h, lane, st.boxes);
                 }
             }
         }
+        return true;
     }
 
-    // the chunks c_begin, c_begin + 8 * kWarps, ... of this warp's 32 rows (accumulator at TMEM address t_row) to D and Z
-    template <bool kTmaStore>
-    __device__ __forceinline__ static void block(const CUtensorMap *map_d, const Params &p, Operands &next, uint32_t t_row, int row_base,
-                                                 int col0, int bn, int c_begin, int lane, uint32_t boxes, uint32_t &store_seq) {
-#pragma unroll 1
-        for (int c0 = c_begin; c0 < bn; c0 += 8 * kWarps) {
-            uint32_t r[32];
-            tc::tmem_ld_32x32_issue(t_row + c0, r);
-            const Operands o = next;
-            if (c0 + 8 * kWarps < bn) load(next, p, row_base + lane, col0 + c0 + 8 * kWarps);
-            tc::tmem_ld_wait();
-            if (p.fmt) chunk<kTmaStore, true>(map_d, p, o, r, row_base, col0 + c0, lane, boxes, store_seq);
-            else chunk<kTmaStore, false>(map_d, p, o, r, row_base, col0 + c0, lane, boxes, store_seq);
-        }
+    // before the block leaves: nothing may still arrive in its shared memory or be read from it
+    __device__ __forceinline__ static void finish(State &st, int lane) {
+        if (st.coming)
+            for (uint32_t spin = 0; spin < kSpinLimit && !mbar_try_wait(st.bar, st.phase); ++spin) {}
+        if (lane == 0) tc::bulk_wait_group_read<0>();
     }
 
 private:
-    template <int kVecs, bool k16>
-    __device__ __forceinline__ static void load_singly(uint4 (&v)[kVecs], const char *at, int left) {
+    // Rows that start anywhere (odd N, unaligned operands): the chunk is turned in shared memory (4 KB, column c of row r at
+    // c ^ r: no bank conflict either way) so that a lane has one column, and every access is 32 neighbouring elements of
+    // a row.  Written straight from a lane's own row, each store touched 32 sectors: 1021 x 2053 x 1096 FP32 22 us.
+    template <bool kBf16>
+    __device__ __forceinline__ static void chunk_by_rows(const Params &p, const uint32_t (&r)[32], int row_base, int col, int lane, uint32_t box) {
+        __syncwarp();
 #pragma unroll
-        for (int j = 0; j < kVecs; ++j) {
-            uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int i = j * 4 + e;  // 32-bit word of the segment
-                if constexpr (k16) {
-                    const uint16_t *h = reinterpret_cast<const uint16_t *>(at);
-                    if (2 * i < left) w[e] = h[2 * i];
-                    if (2 * i + 1 < left) w[e] |= (uint32_t)h[2 * i + 1] << 16;
-                } else {
-                    if (i < left) w[e] = reinterpret_cast<const uint32_t *>(at)[i];
-                }
-            }
-            v[j] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-    }
-    template <bool kBf16, int kVecs>
-    __device__ __forceinline__ static void unpack16(const uint4 (&v)[kVecs], float (&f)[32]) {
-        static_assert(kVecs == 4, "32 values of 16 bits");
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            widen16<kBf16>(v[j].x, f[8 * j], f[8 * j + 1]);
-            widen16<kBf16>(v[j].y, f[8 * j + 2], f[8 * j + 3]);
-            widen16<kBf16>(v[j].z, f[8 * j + 4], f[8 * j + 5]);
-            widen16<kBf16>(v[j].w, f[8 * j + 6], f[8 * j + 7]);
+        for (int c = 0; c < 32; ++c) asm volatile("st.shared.b32 [%0], %1;" ::"r"(box + (uint32_t)(lane * 32 + (c ^ lane)) * 4u), "r"(r[c]) : "memory");
+        __syncwarp();
+        if (col + lane >= p.N) return;
+        const int rows = min(32, p.M - row_base);
+#pragma unroll 4
+        for (int i = 0; i < rows; ++i) {
+            float v;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(box + (uint32_t)(i * 32 + (lane ^ i)) * 4u) : "memory");
+            linear_store_one<kBf16, kOut16>(p, linear_finish_one<kMode, kBf16, kOut16>(p, v, row_base + i, col + lane), row_base + i, col + lane);
         }
     }
 
-    template <bool kTmaStore, bool kBf16>
-    __device__ __forceinline__ static void put(const CUtensorMap *map, void *base, int out_fmt, const Params &p, const float (&v)[32],
-                                               int row_base, int col, int lane, uint32_t boxes, uint32_t &store_seq) {
-        if constexpr (kTmaStore) {
-            uint32_t bits[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) bits[i] = __float_as_uint(v[i]);
-            tc::stage_chunk<kBoxes>(map, p.M, p.N, out_fmt, bits, row_base, col, lane, boxes, kBoxBytes, store_seq);
-        } else {
-            const int row = row_base + lane;
-            if (row >= p.M || col >= p.N) return;
-            tc::GemmParams q = p;
-            q.C = nullptr;
-            q.D = base;
-            if (out_fmt == 0) tc::store_row_segment<float>(v, q, row, col);
-            else if (kBf16) tc::store_row_segment<__nv_bfloat16>(v, q, row, col);
-            else tc::store_row_segment<__half>(v, q, row, col);
-        }
+    // address of 16-byte piece j of row `lane` of a box: rows of 128 bytes with the 128-byte swizzle, or of 64 bytes with the
+    // 64-byte one
+    template <int kRowBytes>
+    __device__ __forceinline__ static uint32_t piece(uint32_t box, int lane, int j) {
+        return kRowBytes == 128 ? box + (uint32_t)lane * 128u + (uint32_t)((j ^ (lane & 7)) << 4)
+                                : box + (uint32_t)lane * 64u + (uint32_t)((j ^ ((lane >> 1) & 3)) << 4);
     }
-
-    template <bool kTmaStore, bool kBf16>
-    __device__ __forceinline__ static void chunk(const CUtensorMap *map_d, const Params &p, const Operands &o, const uint32_t (&r)[32],
-                                                 int row_base, int col, int lane, uint32_t boxes, uint32_t &store_seq) {
-        float v[32];
+    __device__ __forceinline__ static void put_piece(uint32_t at, const uint4 &v) {
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+    }
+    __device__ __forceinline__ static uint4 get_piece(uint32_t at) {
+        uint4 v;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+        return v;
+    }
+    template <bool kBf16>
+    __device__ __forceinline__ static f32x2 widen(uint32_t w) {
+        float lo, hi;
+        widen16<kBf16>(w, lo, hi);
+        return pair_of(lo, hi);
+    }
+    template <bool kBf16>
+    __device__ __forceinline__ static uint32_t narrow(f32x2 v) {
+        float lo, hi;
+        pair_split(v, lo, hi);
+        if constexpr (kBf16) return pack_bf16(lo, hi);
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    // 32 values as 16-bit pieces j0 .. j0 + 3 of the lane's row
+    template <bool kBf16, int kRowBytes>
+    __device__ __forceinline__ static void put16(const f32x2 (&v)[16], uint32_t box, int lane, int j0) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+        for (int j = 0; j < 4; ++j)
+            put_piece(piece<kRowBytes>(box, lane, j0 + j),
+                      make_uint4(narrow<kBf16>(v[4 * j]), narrow<kBf16>(v[4 * j + 1]), narrow<kBf16>(v[4 * j + 2]), narrow<kBf16>(v[4 * j + 3])));
+    }
+    // the box D leaves from, free to be written: box 0 where box 1 belongs to the extra operand or to Z, else both in turn
+    __device__ __forceinline__ static uint32_t free_box(State &st, const Params &p, int lane) {
+        const bool turns = p.extra == nullptr && p.pre == nullptr;
+        if (lane == 0) {
+            if (turns) tc::bulk_wait_group_read<1>();
+            else tc::bulk_wait_group_read<0>();
+        }
+        __syncwarp();
+        return st.boxes + (turns ? (st.stores & 1u) * kBoxBytes : 0u);
+    }
+    __device__ __forceinline__ static void send(State &st, const CUtensorMap *map, uint32_t box, int row_base, int col, int lane) {
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) {
+            tc::tma_store_2d(map, col, row_base, box);  // rows and columns beyond the matrix are clipped by the map
+            tc::bulk_commit_group();
+        }
+        ++st.stores;
+    }
+    // 32 accumulator columns plus the bias
+    template <bool kBf16>
+    __device__ __forceinline__ static void accumulators(const Params &p, uint32_t taddr, int col, f32x2 (&v)[16]) {
+        uint32_t r[32];
+        tc::tmem_ld_32x32_issue(taddr, r);
+        uint4 bias[4];
         if constexpr (kMode == LinearMode::kForward) {
             if (p.bias) {
-                float b[32];
-                unpack16<kBf16>(o.bias, b);
+                const uint4 *at = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.bias) + col);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] += b[i];
+                for (int j = 0; j < 4; ++j) bias[j] = col + j * 8 < p.N ? at[j] : make_uint4(0u, 0u, 0u, 0u);
             }
-            if (p.pre) put<kTmaStore, kBf16>(&p.map_pre, p.pre, kBf16 ? 2 : 1, p, v, row_base, col, lane, boxes, store_seq);
-            with_activation(p.activation, [&](auto act) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = activate<act.value, !kOut16>(v[i]);
-            });
         }
-        if (p.extra) {
-            float x[32];
-            if constexpr (kExtra16) {
-                unpack16<kBf16>(o.extra, x);
-            } else {
+        tc::tmem_ld_wait();
 #pragma unroll
-                for (int j = 0; j < kExtraVecs; ++j) {
-                    x[4 * j] = __uint_as_float(o.extra[j].x);
-                    x[4 * j + 1] = __uint_as_float(o.extra[j].y);
-                    x[4 * j + 2] = __uint_as_float(o.extra[j].z);
-                    x[4 * j + 3] = __uint_as_float(o.extra[j].w);
+        for (int i = 0; i < 16; ++i) v[i] = pair_of(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+        if constexpr (kMode == LinearMode::kForward) {
+            if (p.bias) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[4 * j] = pair_add(v[4 * j], widen<kBf16>(bias[j].x));
+                    v[4 * j + 1] = pair_add(v[4 * j + 1], widen<kBf16>(bias[j].y));
+                    v[4 * j + 2] = pair_add(v[4 * j + 2], widen<kBf16>(bias[j].z));
+                    v[4 * j + 3] = pair_add(v[4 * j + 3], widen<kBf16>(bias[j].w));
                 }
             }
-            if constexpr (kMode == LinearMode::kInputGrad) {
-                with_activation(p.activation, [&](auto act) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] *= activation_slope<act.value, !kOut16>(x[i]);
-                });
-            } else {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] += x[i];
-            }
         }
-        put<kTmaStore, kBf16>(map_d, p.D, kOut16 ? (kBf16 ? 2 : 1) : 0, p, v, row_base, col, lane, boxes, store_seq);
+    }
+
+    template <bool kBf16>
+    __device__ __forceinline__ static void chunk(const CUtensorMap *map_d, const Params &p, State &st, uint32_t taddr, int row_base, int col,
+                                                 bool more, int lane) {
+        constexpr int kHalves = kChunk / 32;
+        constexpr int kRow16 = kOut16 ? 128 : 64;  // bytes of a 16-bit tensor's box row
+        const bool keep_z = kMode == LinearMode::kForward && p.pre != nullptr;
+        if (keep_z && p.extra) {  // box 1 is taken: Z goes ahead through box 0, from a reading of the accumulators of its own
+            const uint32_t box = free_box(st, p, lane);
+#pragma unroll 1
+            for (int h = 0; h < kHalves; ++h) {
+                f32x2 v[16];
+                accumulators<kBf16>(p, taddr + h * 32, col + h * 32, v);
+                put16<kBf16, kRow16>(v, box, lane, h * 4);
+            }
+            send(st, &p.map_pre, box, row_base, col, lane);
+        }
+        const uint32_t d_box = free_box(st, p, lane), z_box = st.boxes + kBoxBytes;
+        if constexpr (kOut16) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint4 extra[4];
+                if (p.extra)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) extra[j] = get_piece(piece<128>(z_box, lane, h * 4 + j));
+                if (h == 1) next_extra(st, p, row_base, col, more, lane);
+                f32x2 v[16];
+                accumulators<kBf16>(p, taddr + h * 32, col + h * 32, v);
+                if constexpr (kMode == LinearMode::kForward) {
+                    if (keep_z && !p.extra) put16<kBf16, 128>(v, z_box, lane, h * 4);
+                    with_activation(p.activation, [&](auto act) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[i] = activate_pair<act.value>(v[i]);
+                    });
+                }
+                if (p.extra) {
+                    f32x2 x[16];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        x[4 * j] = widen<kBf16>(extra[j].x);
+                        x[4 * j + 1] = widen<kBf16>(extra[j].y);
+                        x[4 * j + 2] = widen<kBf16>(extra[j].z);
+                        x[4 * j + 3] = widen<kBf16>(extra[j].w);
+                    }
+                    if constexpr (kMode == LinearMode::kInputGrad) {
+                        with_activation(p.activation, [&](auto act) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) v[i] = pair_mul(v[i], slope_pair<act.value>(x[i]));
+                        });
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[i] = pair_add(v[i], x[i]);
+                    }
+                }
+                put16<kBf16, 128>(v, d_box, lane, h * 4);
+            }
+        } else {
+            // FP32 results: the accumulators go to the box as they are; activation, slope or addition (library functions of
+            // some 40 instructions) then work on the lane's row of it, four values at a time
+            f32x2 v[16];
+            accumulators<kBf16>(p, taddr, col, v);
+            if (keep_z && !p.extra) put16<kBf16, 64>(v, z_box, lane, 0);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float4 f;
+                pair_split(v[2 * j], f.x, f.y);
+                pair_split(v[2 * j + 1], f.z, f.w);
+                put_piece(piece<128>(d_box, lane, j), make_uint4(__float_as_uint(f.x), __float_as_uint(f.y), __float_as_uint(f.z), __float_as_uint(f.w)));
+            }
+            if (p.extra || (kMode == LinearMode::kForward && p.activation != kActNone)) {
+                with_activation(kMode == LinearMode::kWeightGrad ? (int)kActNone : p.activation, [&](auto act) {
+#pragma unroll 1
+                    for (int j = 0; j < 8; ++j) {
+                        const uint4 w = get_piece(piece<128>(d_box, lane, j));
+                        float f[4] = {__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w)}, x[4] = {0.f, 0.f, 0.f, 0.f};
+                        if (p.extra) {
+                            if constexpr (kExtra16) {
+                                const uint4 e = get_piece(piece<64>(z_box, lane, j >> 1));
+                                widen16<kBf16>(j & 1 ? e.z : e.x, x[0], x[1]);
+                                widen16<kBf16>(j & 1 ? e.w : e.y, x[2], x[3]);
+                            } else {
+                                const uint4 e = get_piece(piece<128>(z_box, lane, j));
+                                x[0] = __uint_as_float(e.x), x[1] = __uint_as_float(e.y), x[2] = __uint_as_float(e.z), x[3] = __uint_as_float(e.w);
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if constexpr (kMode == LinearMode::kInputGrad) f[i] *= slope_exact<act.value>(x[i]);
+                            else f[i] = __fadd_rn(activate_exact<act.value>(f[i]), x[i]);
+                        }
+                        put_piece(piece<128>(d_box, lane, j), make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])));
+                    }
+                });
+            }
+            next_extra(st, p, row_base, col, more, lane);
+        }
+        if (keep_z && !p.extra) {  // both boxes in one group of stores
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) tc::tma_store_2d(&p.map_pre, col, row_base, z_box);
+        }
+        send(st, map_d, d_box, row_base, col, lane);
+    }
+    // the extra operand's box has been read: the next chunk's may come
+    __device__ __forceinline__ static void next_extra(State &st, const Params &p, int row_base, int col, bool more, int lane) {
+        if (p.extra == nullptr) return;
+        __syncwarp();
+        if (more) bring(st, p, row_base, col + kStep, lane);
     }
 };
 

@@ -19,11 +19,12 @@ _NP_OF = {DTYPE_F32: np.float32, DTYPE_F16: np.uint16, DTYPE_BF16: np.uint16}
 _SIZE_OF = {DTYPE_F32: 4, DTYPE_F16: 2, DTYPE_BF16: 2}
 
 
-def _current_stream_ptr() -> int:
+def _current_stream_ptr(device_index: int | None = None) -> int:
+    """Handle of the current stream of a device (None: the current one).  The handle alone: building the Stream object
+    around it (torch.cuda.current_stream()) costs the host 3 us a call."""
     import torch
 
-    # the handle alone: building the Stream object around it (torch.cuda.current_stream()) costs the host 3 us a call
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device_index is None else device_index)
 
 
 def _ptr(t) -> int | None:
@@ -216,20 +217,20 @@ def layernorm_backward(dy, x, eps: float, gamma=None, ddof: int = 0, residual=No
     if x.dim() != 2 or x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise ValueError(f"x must be a 2-D FP32, FP16 or BF16 tensor, got {x.dtype} with {x.dim()} dimensions")
     rows, cols = x.shape
-    same, vector = (x.dtype,), (torch.float32,)
+    device, same, vector = x.device, (x.dtype,), (torch.float32,)
     lib = native.lib()
     code, fn = {torch.float32: (DTYPE_F32, lib.ko_layernorm_backward_f32), torch.float16: (DTYPE_F16, lib.ko_layernorm_backward_f16),
                 torch.bfloat16: (DTYPE_BF16, lib.ko_layernorm_backward_bf16)}[x.dtype]
-    with _on(x.device, stream):
-        dx = torch.empty(rows, cols, dtype=x.dtype, device=x.device) if dx is None else dx
-        dgamma = torch.empty(cols, dtype=torch.float32, device=x.device) if dgamma is None else dgamma
-        dbeta = torch.empty(cols, dtype=torch.float32, device=x.device) if dbeta is None else dbeta
-        ws, ws_at, ws_bytes = _workspace(_layernorm_backward_bytes(x.device.index, code, rows, cols), x.device)
-        native.check(fn(_operand(dy, "dy", x.device, same, (rows, cols)), _ptr(x), _operand(dx, "dx", x.device, same, (rows, cols)), rows,
-                        cols, eps, _operand(gamma, "gamma", x.device, same, (cols,)),
-                        _operand(residual, "residual", x.device, same, (rows, cols)),
-                        _operand(dgamma, "dgamma", x.device, vector, (cols,)), _operand(dbeta, "dbeta", x.device, vector, (cols,)), ddof,
-                        ws_at, ws_bytes, _current_stream_ptr()), "ko_layernorm_backward")
+    with _on(device, stream):
+        dx = torch.empty(rows, cols, dtype=x.dtype, device=device) if dx is None else dx
+        dgamma = torch.empty(cols, dtype=torch.float32, device=device) if dgamma is None else dgamma
+        dbeta = torch.empty(cols, dtype=torch.float32, device=device) if dbeta is None else dbeta
+        ws, ws_at, ws_bytes = _workspace(_layernorm_backward_bytes(device.index, code, rows, cols), device)
+        native.check(fn(_operand(dy, "dy", device, same, (rows, cols)), _ptr(x), _operand(dx, "dx", device, same, (rows, cols)), rows,
+                        cols, eps, _operand(gamma, "gamma", device, same, (cols,)),
+                        _operand(residual, "residual", device, same, (rows, cols)),
+                        _operand(dgamma, "dgamma", device, vector, (cols,)), _operand(dbeta, "dbeta", device, vector, (cols,)), ddof,
+                        ws_at, ws_bytes, _current_stream_ptr(device.index)), "ko_layernorm_backward")
     return dx, dgamma, dbeta
 
 
@@ -346,7 +347,7 @@ def linear(x, w, bias=None, activation: str = "none", residual=None, out=None, o
         native.check(native.lib().ko_linear(in_fmt, out_fmt, act, m, n, k, _ptr(x), _operand(w, "w", device, same, (n, k)),
                                             _operand(bias, "bias", device, same, (n,)), _operand(residual, "residual", device, to, (m, n)),
                                             _operand(out, "out", device, to, (m, n)), _operand(pre, "pre", device, same, (m, n)),
-                                            ws_at, ws_bytes, _current_stream_ptr()), "ko_linear")
+                                            ws_at, ws_bytes, _current_stream_ptr(device.index)), "ko_linear")
     return out if pre is None else (out, pre)
 
 
@@ -370,7 +371,7 @@ def linear_backward_input(dy, w, pre=None, activation: str = "none", out=None, o
         ws, ws_at, ws_bytes = _workspace(_linear_bytes(device.index, "ko_linear_backward_input_workspace", m, n, k), device)
         native.check(native.lib().ko_linear_backward_input(
             in_fmt, out_fmt, act, m, n, k, _ptr(dy), _operand(w, "w", device, same, (n, k)), _operand(pre, "pre", device, same, (m, k)),
-            _operand(out, "out", device, (out_dtype,), (m, k)), ws_at, ws_bytes, _current_stream_ptr()), "ko_linear_backward_input")
+            _operand(out, "out", device, (out_dtype,), (m, k)), ws_at, ws_bytes, _current_stream_ptr(device.index)), "ko_linear_backward_input")
     return out
 
 
@@ -396,5 +397,5 @@ def linear_backward_weight(dy, x, c=None, out=None, out_dtype=None, return_bias:
         native.check(native.lib().ko_linear_backward_weight(
             in_fmt, out_fmt, m, n, k, _ptr(dy), _operand(x, "x", device, (dy.dtype,), (m, k)), _operand(c, "c", device, to, (n, k)),
             _operand(out, "out", device, to, (n, k)), _operand(dbias, "dbias", device, (torch.float32,), (n,)),
-            ws_at, ws_bytes, _current_stream_ptr()), "ko_linear_backward_weight")
+            ws_at, ws_bytes, _current_stream_ptr(device.index)), "ko_linear_backward_weight")
     return out if dbias is None else (out, dbias)
