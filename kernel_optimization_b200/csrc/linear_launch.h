@@ -23,33 +23,35 @@ struct ProductPlan {
     long long tiles;
 };
 
-// tma: D can be stored by TMA; without it only the 128 x 128 tile is built.  Modelled microseconds per candidate: start,
-// then rounds of work units x (K-blocks of 64 x time per K-block + time between tiles); slices add a second kernel and the
-// partial tiles' way through the L2 (written once, read once) at 5 TB/s.  Fitted to
-// forced plans, BF16, measured (modelled): 16384 x 4096 x 1024 pair 103 (102), 128 x 256 110 (111), 128 x 128 164 (173);
-// 4096^3 93 (96), 102 (103), 142 (144); 8192 x 768 x 768 16.6 (14.9), 17.4 (15.7), 18.2 (18.0); 2048 x 1024 x 1024 13.6 (12.3),
-// 14.0 (11.0), 11.1 (9.1); 768 x 768 x 8192 in four slices of 128-wide tiles 20.2 (20.2), in eight of 256-wide ones 21.3 (21.1).
-inline ProductPlan plan_product(int64_t M, int64_t N, int64_t K, bool tma, int sms) {
+// tma: D can be stored by TMA; without it only the 128 x 128 tile is built.  element_bytes: what the epilogue moves per element
+// of D (D itself, Z, the extra operand).  Modelled microseconds per candidate: start, then rounds of work units x (K-blocks
+// of 64 x time per K-block + epilogue time that the next tile does not hide); slices add a second kernel and the partial
+// tiles' way through the L2 (written once, read once) at 5 TB/s.  Fitted to forced plans, BF16, measured (modelled):
+// 16384 x 4096 x 1024 pair 103 (103), 128 x 256 110 (112), 128 x 128 164 (165); 4096^3 93 (97), 102 (103), 142 (139);
+// 8192 x 768 x 768 16.6 (15.9), 17.4 (16.3), 18.2 (17.1); 2048 x 1024 x 1024 13.6 (11.6), 14.0 (11.8), 11.1 (8.8); 4096 x 4096 x 64
+// to FP32 19.0 (17.7), 15.5 (17.3), 14.0 (17.3); 768 x 768 x 8192 in four slices of 128-wide tiles 20.2 (19.9).
+inline ProductPlan plan_product(int64_t M, int64_t N, int64_t K, bool tma, int element_bytes, int sms) {
     const long long k_blocks = (K + tc::kBK - 1) / tc::kBK;
     ProductPlan best{false, 128, 1, 0};
     double best_cost = 1e300;
     if (tma && M > 128 && N > 128) {
         const long long tiles = ((M + 255) / 256) * ((N + 255) / 256);
         const long long rounds = (tiles + sms / 2 - 1) / (sms / 2);
-        best_cost = 4.5 + (double)rounds * ((double)k_blocks * 0.335 + 1.7);
+        best_cost = 4.5 + (double)rounds * ((double)k_blocks * 0.335 + 0.3 + 0.7 * element_bytes);
         best = {true, 256, 1, tiles};
     }
     for (int bn : {128, 256}) {
         if (bn == 256 && (!tma || N <= 128)) continue;
-        const double per_block = bn == 256 ? 0.36 : 0.29, per_tile = bn == 256 ? 1.9 : 1.5, start = bn == 256 ? 4.3 : 3.0;
+        const double per_block = bn == 256 ? 0.36 : 0.29, start = bn == 256 ? 4.3 : 3.0;
+        const auto per_tile = [&](int bytes) { return bn == 256 ? 0.5 + 0.6 * bytes : 0.5 + 0.35 * bytes; };
         const long long tiles = ((M + 127) / 128) * ((N + bn - 1) / bn);
         const long long most = std::min<long long>(std::max<long long>(sms / tiles, 1), std::max<long long>(k_blocks / 4, 1));
         for (int split = 1; split <= most && split <= 64; ++split) {
             const long long rounds = (tiles * split + sms - 1) / sms;
-            double cost = start + (double)rounds * ((double)((k_blocks + split - 1) / split) * per_block + per_tile);
+            double cost = start + (double)rounds * ((double)((k_blocks + split - 1) / split) * per_block + per_tile(split > 1 ? 4 : element_bytes));
             if (split > 1) {
-                const double written = (double)((M + 31) / 32 * 32) * N * split, read = (double)M * N * split;
-                cost += 2.2 + (written + read + (double)M * N) * 4.0 / 5e6;
+                const double written = (double)((M + 31) / 32 * 32) * (double)N * split, read = (double)M * (double)N * split;
+                cost += 2.2 + ((written + read) * 4.0 + (double)M * (double)N * element_bytes) / 5e6;
             }
             if (cost < best_cost) {
                 best_cost = cost;
@@ -80,10 +82,13 @@ inline int pin_product(const PinnedPlan &pin, int64_t M, int64_t N, int64_t K, b
     return KO_OK;
 }
 
-// room for either way a call may store D
+// room for whatever plan a call of this shape may take: with or without TMA, any operands
 inline size_t product_workspace(int64_t M, int64_t N, int64_t K, int sms) {
     if (M == 0 || N == 0 || K == 0) return 0;
-    return std::max(plan_product(M, N, K, true, sms).bytes(), plan_product(M, N, K, false, sms).bytes());
+    size_t most = 0;
+    for (int element_bytes = 2; element_bytes <= 10; element_bytes += 2)
+        most = std::max({most, plan_product(M, N, K, true, element_bytes, sms).bytes(), plan_product(M, N, K, false, element_bytes, sms).bytes()});
+    return most;
 }
 
 // clusters of two CTAs of a pair kernel that the current device holds at once (cached per kernel and device)
@@ -128,21 +133,25 @@ int launch_product_pair(const CUtensorMap &ma, const CUtensorMap &mb, const CUte
 
 // Runs the product that `p` describes (M, N, K, D, fmt, out_fmt, b_row_major, bias, extra, pre, activation set by the
 // caller; the rest filled in here).  A: [M, K], or [K, M] for the weight gradient; B: [N, K], or [K, N] with b_row_major.
-// Everything has been checked but the workspace.
-template <LinearMode kMode, bool kOut16>
+// Everything has been checked but the workspace.  `first` launches what goes ahead of the product once nothing is left to
+// refuse, `beside` what may run beside it, between it and the sum of its slices.
+struct Nothing {
+    int operator()() const { return KO_OK; }
+};
+template <LinearMode kMode, bool kOut16, class First = Nothing, class Beside = Nothing>
 int run_product(LinearParams p, const void *A, const void *B, void *workspace, size_t workspace_bytes, cudaStream_t s, const DeviceInfo &info,
-                const char *name, const PinnedPlan &pin = {}) {
+                const char *name, const PinnedPlan &pin = {}, const First &first = {}, const Beside &beside = {}) {
     using Epi = LinearEpilogue<kMode, kOut16>;
     EncodeTiledFn encode = nullptr;
     if (int st = get_encode_fn(&encode)) return st;
     // 16-byte row pitches and bases of everything the epilogue touches: TMA and vector loads; else its row-wise form
     const bool sixteen = kOut16 || p.pre || p.bias || (p.extra && Epi::kExtra16);
     const bool tma = p.N % (sixteen ? 8 : 4) == 0 && aligned16(p.D) && aligned16(p.pre) && aligned16(p.bias) && aligned16(p.extra);
-    ProductPlan plan = plan_product(p.M, p.N, p.K, tma, info.sm_count);
+    const int element_bytes = (kOut16 ? 2 : 4) + (p.pre ? 2 : 0) + (p.extra ? (Epi::kExtra16 ? 2 : 4) : 0);
+    ProductPlan plan = plan_product(p.M, p.N, p.K, tma, element_bytes, info.sm_count);
     if (int st = pin_product(pin, p.M, p.N, p.K, tma, name, &plan)) return st;
-    const size_t need = std::max(plan.bytes(), product_workspace(p.M, p.N, p.K, info.sm_count));
-    KO_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), KO_ERR_INVALID_ARG, "%s: the workspace needs %zu bytes, got %zu",
-               name, need, workspace ? workspace_bytes : (size_t)0);
+    KO_REQUIRE(plan.bytes() == 0 || (workspace != nullptr && workspace_bytes >= plan.bytes()), KO_ERR_INVALID_ARG,
+               "%s: the workspace needs %zu bytes, got %zu", name, plan.bytes(), workspace ? workspace_bytes : (size_t)0);
     KO_REQUIRE(aligned16(workspace), KO_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", name);
     p.C = nullptr;
     p.tiles_n = p.wide_tiles_n = p.bn_wide = p.bn_narrow = 0;
@@ -170,11 +179,13 @@ int run_product(LinearParams p, const void *A, const void *B, void *workspace, s
         if (p.extra)
             if (int st = make_store_map(encode, &p.map_extra, Epi::kExtra16 ? p.fmt + 1 : 0, const_cast<void *>(p.extra), p.M, p.N, Epi::kChunk)) return st;
     }
-    int st;
+    int st = first();
+    if (st != KO_OK) return st;
     if (plan.pair) st = launch_product_pair<Epi>(map_a, map_b, map_d, p, s);
     else if (!tma) st = launch_product_tile<Epi, 128, false>(map_a, map_b, map_d, p, info.sm_count, s);
     else if (plan.bn == 128) st = launch_product_tile<Epi, 128, true>(map_a, map_b, map_d, p, info.sm_count, s);
     else st = launch_product_tile<Epi, 256, true>(map_a, map_b, map_d, p, info.sm_count, s);
+    if (st == KO_OK) st = beside();
     if (st != KO_OK || plan.split <= 1) return st;
     const long long chunks = plan.tiles * 4 * (plan.bn / 32);
     return launch_overlapped(linear_slice_sum_kernel<kMode, kOut16>, (unsigned)chunks, 256u, (size_t)0, s, p, plan.bn);

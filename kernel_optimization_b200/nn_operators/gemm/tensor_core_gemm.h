@@ -250,6 +250,7 @@ struct PlainEpilogue {
     static constexpr int kWarps = 4;  // epilogue warps, a multiple of 4: each quadrant of TMEM lanes is shared by kWarps / 4
     static constexpr bool kTransA = false;
     static constexpr bool kFused = false;
+    static constexpr bool kShares = false;  // true: launch_dependents only after the wait for the previous kernel; registers and memory left over
 };
 
 template <class Epi, bool kFused = Epi::kFused>
@@ -480,7 +481,7 @@ __device__ __forceinline__ void publish_block(float *slot_chunks, uint32_t t_row
 // kTmaStore: D is written by TMA stores staged through shared memory (needs a 16-byte row pitch and base for D
 // and no C operand); otherwise every thread stores its row segment directly (and adds C when given)
 template <int BN, bool kTmaStore, int MT = 1, int kBoxes = 2, class Epi = PlainEpilogue>
-__global__ void __launch_bounds__(64 + 32 * Epi::kWarps, 1)
+__global__ void __launch_bounds__(64 + 32 * Epi::kWarps, Epi::kShares ? 2 : 1)
 gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                     const __grid_constant__ CUtensorMap map_b_narrow, const __grid_constant__ CUtensorMap map_d,
                     const __grid_constant__ typename Epi::Params p) {
@@ -540,7 +541,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         if (p.tiles_n) prefetch_tensormap(&map_b_narrow);
         if (kTmaStore) prefetch_tensormap(&map_d);
     }
-    grid_launch_dependents();  // the stream's next kernel may set up while this one drains
+    if (!Epi::kShares) grid_launch_dependents();  // the stream's next kernel may set up while this one drains
     if (warp == 1) tmem_alloc(smem_u32(tmem_slot), Cfg::kTmemCols);
     tc_fence_before();
     __syncthreads();
@@ -549,6 +550,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     // launched with programmatic stream serialization: barriers, tensor memory and descriptor prefetch above
     // overlap the previous kernel's tail; operands and D are touched only after its writes are visible
     grid_dependency_wait();
+    if (Epi::kShares) grid_launch_dependents();
 
     if (warp == 0) {
         // ------------------------------------------------------------------ TMA producer

@@ -118,7 +118,7 @@ __device__ __forceinline__ bool mbar_wait_remote(uint32_t bar, uint32_t parity, 
 
 // map_b / map_b_narrow: boxes of bn_wide / 2 and bn_narrow / 2 rows (128 rows when the tiles are uniform)
 template <bool kTmaStore, class Epi = PlainEpilogue>
-__global__ void __launch_bounds__(64 + 32 * Epi::kWarps, 1)
+__global__ void __launch_bounds__(64 + 32 * Epi::kWarps, Epi::kShares ? 2 : 1)
 gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                          const __grid_constant__ CUtensorMap map_b_narrow, const __grid_constant__ CUtensorMap map_d,
                          const __grid_constant__ typename Epi::Params p) {
@@ -168,7 +168,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         if (p.tiles_n) prefetch_tensormap(&map_b_narrow);
         if (kTmaStore) prefetch_tensormap(&map_d);
     }
-    grid_launch_dependents();
+    if (!Epi::kShares) grid_launch_dependents();
     if (warp == 1) tmem_alloc_pair(smem_u32(tmem_slot), Cfg::kTmemCols);
     tc_fence_before();
     __syncthreads();
@@ -176,6 +176,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     grid_dependency_wait();
+    if (Epi::kShares) grid_launch_dependents();
 
     if (warp == 0) {
         // ------------------------------------------------------------------ TMA producer (both CTAs)

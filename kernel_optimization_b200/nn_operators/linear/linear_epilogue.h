@@ -8,7 +8,10 @@
 // first chunk's while the tile is still being multiplied -- so neither direction takes issue slots or L1 from the warps.
 // Everything is FP32 until one rounding to the stored type.  Eight epilogue warps, two per quadrant of TMEM lanes: an
 // activation costs about ten issue slots an element, which four warps alone could not hide behind the next tile's MMAs.
+// (Four for the weight gradient, which only stores.)
 #pragma once
+
+#include <cooperative_groups.h>
 
 #include "../gemm/tensor_core_gemm.h"
 #include "activation.h"
@@ -79,9 +82,13 @@ __device__ __forceinline__ void linear_store_one(const LinearParams &p, float v,
 template <LinearMode kMode, bool kOut16>
 struct LinearEpilogue {
     using Params = LinearParams;
-    static constexpr int kWarps = 8;
     static constexpr bool kTransA = kMode == LinearMode::kWeightGrad;
+    static constexpr int kWarps = kTransA ? 4 : 8;
     static constexpr bool kFused = true;
+    // The weight gradient shares its SMs with the column sums of the bias gradient: it asks for dependents only once its own
+    // inputs are there (see column_sum_kernel), and leaves registers (at most 168 a thread, as for two blocks) and the little
+    // shared memory that the sums need.
+    static constexpr bool kShares = kTransA;
     static constexpr bool kExtra16 = kMode == LinearMode::kInputGrad || kOut16;
     static constexpr int kChunk = kOut16 ? 64 : 32;           // columns
     static constexpr int kStep = kChunk * (kWarps / 4);        // from one chunk of a warp to its next
@@ -154,13 +161,55 @@ private:
 #pragma unroll
         for (int c = 0; c < 32; ++c) asm volatile("st.shared.b32 [%0], %1;" ::"r"(box + (uint32_t)(lane * 32 + (c ^ lane)) * 4u), "r"(r[c]) : "memory");
         __syncwarp();
-        if (col + lane >= p.N) return;
-        const int rows = min(32, p.M - row_base);
-#pragma unroll 4
-        for (int i = 0; i < rows; ++i) {
-            float v;
-            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(box + (uint32_t)(i * 32 + (lane ^ i)) * 4u) : "memory");
-            linear_store_one<kBf16, kOut16>(p, linear_finish_one<kMode, kBf16, kOut16>(p, v, row_base + i, col + lane), row_base + i, col + lane);
+        const int c = col + lane, rows = min(32, p.M - row_base);
+        if (c >= p.N) return;
+        float bias = 0.f;
+        if (kMode == LinearMode::kForward && p.bias) bias = widen16_at<kBf16>(p.bias, (size_t)c);
+        constexpr int kRows = 8;  // rows whose operands are on their way together
+#pragma unroll 1
+        for (int i0 = 0; i0 < rows; i0 += kRows) {
+            const size_t at = (size_t)(row_base + i0) * p.N + c;
+            float x[kRows], v[kRows];
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+                x[i] = 0.f;
+                if (p.extra && i0 + i < rows) {
+                    if constexpr (kExtra16) x[i] = widen16_at<kBf16>(p.extra, at + (size_t)i * p.N);
+                    else x[i] = static_cast<const float *>(p.extra)[at + (size_t)i * p.N];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[i]) : "r"(box + (uint32_t)((i0 + i) * 32 + (lane ^ (i0 + i))) * 4u) : "memory");
+                if (kMode == LinearMode::kForward && p.bias) v[i] += bias;
+            }
+            if (kMode == LinearMode::kForward && p.pre)
+#pragma unroll
+                for (int i = 0; i < kRows; ++i)
+                    if (i0 + i < rows) static_cast<uint16_t *>(p.pre)[at + (size_t)i * p.N] = (uint16_t)tc::pack16(v[i], 0.f, kBf16 ? 2 : 1);
+            if (p.activation != kActNone)
+                with_activation(p.activation, [&](auto act) {
+#pragma unroll
+                    for (int i = 0; i < kRows; i += 2) {
+                        if constexpr (kMode == LinearMode::kInputGrad) {
+                            float s0 = 0.f, s1 = 0.f;
+                            if constexpr (kOut16) pair_split(slope_pair<act.value>(pair_of(x[i], x[i + 1])), s0, s1);
+                            else s0 = slope_exact<act.value>(x[i]), s1 = slope_exact<act.value>(x[i + 1]);
+                            v[i] *= s0;
+                            v[i + 1] *= s1;
+                        } else if constexpr (kOut16) {
+                            pair_split(activate_pair<act.value>(pair_of(v[i], v[i + 1])), v[i], v[i + 1]);
+                        } else {
+                            v[i] = activate_exact<act.value>(v[i]);
+                            v[i + 1] = activate_exact<act.value>(v[i + 1]);
+                        }
+                    }
+                });
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+                if (kMode != LinearMode::kInputGrad && p.extra) v[i] = __fadd_rn(v[i], x[i]);
+                if (i0 + i < rows) linear_store_one<kBf16, kOut16>(p, v[i], row_base + i0 + i, c);
+            }
         }
     }
 
@@ -398,65 +447,75 @@ __global__ void __launch_bounds__(256) linear_slice_sum_kernel(const LinearParam
     }
 }
 
-// Column sums of a 16-bit [rows, cols] matrix (the bias gradient), cols a multiple of 8: a warp takes 256 columns of every
-// (8 * gridDim.y)-th row, the block's warps add through shared memory, one partial row per block; with a single block
-// along the rows the partial row is the result.
-template <bool kBf16>
-__global__ void __launch_bounds__(256) column_sum_kernel(const uint16_t *in, long long rows, int cols, float *partials) {
-    constexpr int E = 8;
-    __shared__ float fold[8][32 * E + 1];
+// Column sums of a 16-bit [rows, cols] matrix, cols a multiple of 8: the bias gradient, beside the weight gradient's product.
+// A cluster of blocks shares 64 columns (a 128-byte line of each row, eight threads wide) and splits the rows; the blocks'
+// sums are added in rank order through distributed shared memory, so there is no workspace and no second kernel.  The
+// product keeps the SMs' ports to the L2 busy: with one block per 32 columns the sums of 16384 x 4096 crawled along for 229 us
+// beside a product of 100 us; many blocks with many lines in flight get through.
+//
+// Launched behind the product with programmatic serialization, it runs while the product does: the product's blocks ask
+// for their dependents only after their own grid_dependency_wait(), so everything enqueued before the product is complete
+// and visible when this kernel starts, and it reads and writes nothing the product writes.  It waits for the product before
+// it ends, so whatever follows it in the stream also follows the product.  (Loads past the L1, which may hold lines of an
+// earlier kernel.)
+template <bool kBf16, int kWarps = 8>
+__global__ void __launch_bounds__(32 * kWarps, 32 / kWarps) column_sum_kernel(const uint16_t *in, long long rows, int cols, float *out) {
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    __shared__ float sums[64];  // little enough to fit beside a product's block
     grid_launch_dependents();
-    grid_dependency_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int c = (int)(blockIdx.x * 32 + lane) * E;
-    float sum[E];
+    const int c0 = (int)(blockIdx.x / ranks) * 64, c = c0 + (lane & 7) * 8;
+    f32x2 sum[4];
 #pragma unroll
-    for (int e = 0; e < E; ++e) sum[e] = 0.f;
+    for (int i = 0; i < 4; ++i) sum[i] = pair_of(0.f, 0.f);
     if (c < cols) {
-#pragma unroll 4
-        for (long long r = (long long)blockIdx.y * 8 + warp; r < rows; r += (long long)gridDim.y * 8) {
-            const uint16_t *at = in + (size_t)r * cols + c;
-            const uint4 v = *reinterpret_cast<const uint4 *>(at);
-            float f[8];
-            widen16<kBf16>(v.x, f[0], f[1]);
-            widen16<kBf16>(v.y, f[2], f[3]);
-            widen16<kBf16>(v.z, f[4], f[5]);
-            widen16<kBf16>(v.w, f[6], f[7]);
+        constexpr int kAhead = 8;
+        const long long step = (long long)ranks * kWarps * 4;
+        for (long long r = (rank * kWarps + warp) * 4 + (lane >> 3); r < rows; r += step * kAhead) {
+            uint4 v[kAhead];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sum[e] += f[e];
+            for (int i = 0; i < kAhead; ++i)
+                v[i] = r + i * step < rows ? __ldcg(reinterpret_cast<const uint4 *>(in + (size_t)(r + i * step) * cols + c)) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float lo, hi;
+                    widen16<kBf16>(w[j], lo, hi);
+                    sum[j] = pair_add(sum[j], pair_of(lo, hi));
+                }
+            }
         }
     }
+    float column[8];
 #pragma unroll
-    for (int e = 0; e < E; ++e) fold[warp][lane * E + e] = sum[e];
-    __syncthreads();
-    for (int i = threadIdx.x; i < 32 * E; i += 256) {
-        const int col = (int)blockIdx.x * 32 * E + i;
-        float total = 0.f;
+    for (int j = 0; j < 4; ++j) {
+        float v[2];
+        pair_split(sum[j], v[0], v[1]);
 #pragma unroll
-        for (int w = 0; w < 8; ++w) total += fold[w][i];
-        if (col < cols) partials[(size_t)blockIdx.y * cols + col] = total;
+        for (int h = 0; h < 2; ++h) {
+            v[h] += __shfl_xor_sync(kFullMask, v[h], 16);
+            v[h] += __shfl_xor_sync(kFullMask, v[h], 8);
+            column[2 * j + h] = v[h];
+        }
     }
-}
-// out = the partial rows added in order: a block takes 32 columns, warp w the partial rows w, w + 8, ...
-template <int kWarps = 8>
-__global__ void __launch_bounds__(32 * kWarps) column_fold_kernel(const float *partials, int partial_rows, int cols, float *out) {
-    __shared__ float fold[kWarps][32];
-    grid_launch_dependents();
+    for (int w = 0; w < kWarps; ++w) {  // the warps in turn
+        if (warp == w && lane < 8)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sums[lane * 8 + i] = w ? sums[lane * 8 + i] + column[i] : column[i];
+        __syncthreads();
+    }
+    if (ranks > 1) cluster.sync();
+    if (rank == 0 && threadIdx.x < 64 && c0 + (int)threadIdx.x < cols) {
+        float total = sums[threadIdx.x];
+        for (int r = 1; r < ranks; ++r) total += *cluster.map_shared_rank(sums + threadIdx.x, r);
+        out[c0 + threadIdx.x] = total;
+    }
+    if (ranks > 1) cluster.sync();  // nobody leaves while its sums may still be read
     grid_dependency_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int col = (int)blockIdx.x * 32 + lane;
-    float sum = 0.f;
-    if (col < cols)
-#pragma unroll 4
-        for (int p = warp; p < partial_rows; p += kWarps) sum += __ldcg(partials + (size_t)p * cols + col);
-    fold[warp][lane] = sum;
-    __syncthreads();
-    if (warp == 0 && col < cols) {
-        sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) sum += fold[w][lane];
-        out[col] = sum;
-    }
 }
 
 }  // namespace ko

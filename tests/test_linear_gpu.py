@@ -222,6 +222,24 @@ def test_no_tokens(cuda, ko):
     assert cuda.equal(ko.linear_backward_weight(dy, x, c, return_bias=False), c)
 
 
+def test_no_input_features(cuda, ko):
+    """k = 0: dw is empty, the bias gradient is still the column sums."""
+    for m, n in ((5, 64), (3000, 200)):
+        dy, x = _randn(cuda, (m, n), cuda.bfloat16, 1), cuda.empty(m, 0, device="cuda", dtype=cuda.bfloat16)
+        dw, db = ko.linear_backward_weight(dy, x)
+        assert dw.shape == (n, 0) and ((db.double() - dy.double().sum(0)).abs() <= (m / 8 + 64) * 2.0 ** -24 * dy.double().abs().sum(0)).all()
+
+
+def test_bias_gradient_of_a_large_batch(cuda, ko):
+    """dY beyond the size up to which its column sums run beside the product."""
+    dy, x = _randn(cuda, (6500, 4104), cuda.float16, 1, 0.1), _randn(cuda, (6500, 72), cuda.float16, 2)
+    dw, db = ko.linear_backward_weight(dy, x)
+    _close(cuda, dw, dy.double().t() @ x.double(), _sum_error(dy.t(), x, 6500), "dw")
+    _close(cuda, db, dy.double().sum(0), (6500 / 8 + 64) * 2.0 ** -24 * dy.double().abs().sum(0), "dbias")
+    again = ko.linear_backward_weight(dy, x)
+    assert cuda.equal(dw, again[0]) and cuda.equal(db, again[1])
+
+
 def _np16(cuda, t):
     return t.contiguous().view(cuda.int16).cpu().numpy()
 
