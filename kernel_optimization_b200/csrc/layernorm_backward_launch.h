@@ -88,7 +88,7 @@ int launch_resident(const ko::LayerNormBackwardArgs<T> &a, const ko::DeviceInfo 
     if (E > 1) {
         // the SM's shared memory, shared by its blocks; 3 KB of each share cover static shared memory and the system's 1 KB
         const size_t share = ((size_t)info.max_smem_optin + 1024) / kBlocks - 3072;
-        const size_t stage = (size_t)kRows * a.cols * sizeof(T) * (a.residual ? 3 : 2);
+        const size_t stage = (size_t)kRows * backward_pitch<T, E, kVecs, kLanes>(a.cols) * (a.residual ? 3 : 2);
         stages = (int)std::min<size_t>(share / stage, kBackwardMaxStages);
         KO_REQUIRE(stages >= 2, KO_ERR_SHAPE, "layernorm backward: %d columns leave no room for two stages", a.cols);  // 8192 FP32 columns do
         smem = std::max(smem, stages * stage);

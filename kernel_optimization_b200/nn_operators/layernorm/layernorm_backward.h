@@ -81,14 +81,19 @@ __device__ __forceinline__ void block_allreduce_sums(float (&v)[N], float *scrat
 // leave once per block.  Per row two reductions of two values each: sum x and sum w, then, with the mean, sum dev^2 and
 // sum w dev.
 //
-// Consecutive rows are consecutive bytes: one thread brings a step's rows of x, dy and the residual into a shared-memory
-// ring by one bulk copy each (cp.async.bulk, counted in bytes on an mbarrier), several steps ahead, so the bytes in flight
-// depend neither on registers nor on how many warps the row's reductions keep waiting.  Bulk copies want 16-byte
-// boundaries: rows of single elements (E == 1: odd widths, unaligned operands) come by plain loads instead.
+// Rows are consecutive bytes: the first warp brings a step's rows of x, dy and the residual into a shared-memory ring by bulk
+// copies (cp.async.bulk, counted in bytes on an mbarrier), several steps ahead, so the bytes in flight depend neither on
+// registers nor on how many warps the row's reductions keep waiting.  Bulk copies want 16-byte boundaries: rows of single
+// elements (E == 1: odd widths, unaligned operands) come by plain loads instead.
 //
 // 16-bit rows leave about 34 instruction slots per element at full bandwidth (6 bytes an element, 22 bytes per clock and
 // SM), so arithmetic runs on packed FP32 pairs, elements are unpacked once, and a thread holds 16 columns to spread the
 // reductions' shuffles over many elements.
+//
+// Measured (B200, with the kernel that adds the partial rows; copy bandwidth 6447 GB/s): BF16 [32768, 4096] with residual
+// 185 us = 5.80 TB/s (173 us = 4.66 TB/s without: there the instruction slots bind, 70 % of them taken), FP32 [16384, 768]
+// 30 us = 5.0 TB/s of which the second kernel is 3, FP32 [8192, 5120] with residual 103 us = 6.5 TB/s, FP16 [30000, 1001]
+// 62 us = 2.9 TB/s (two-byte loads).
 constexpr int kBackwardWarpsPerSm = 16;  // at 128 registers a thread
 constexpr int kBackwardMaxStages = 8;
 
@@ -134,7 +139,17 @@ struct RowReduce {
     }
 };
 
-// stages: steps of kRows rows in the ring (dynamic shared memory: [stages][x, dy(, residual)][kRows][cols], at least
+// Rows of more than a warp have a place of their own in the ring, as wide as the columns their threads cover: every address is
+// then a constant away from the stage's, and the columns past the row's end read zeros that are written once.  Each row is a
+// copy of its own then, which shorter rows do not bear (131072 x 256 BF16 60 us against 47 with one copy for a step's rows).
+template <int kLanes>
+constexpr bool kBackwardPadded = kLanes >= 64;
+template <typename T, int E, int kVecs, int kLanes>
+__host__ __device__ constexpr uint32_t backward_pitch(int cols) {
+    return (uint32_t)((kBackwardPadded<kLanes> ? kLanes * kVecs * E : cols) * (int)sizeof(T));
+}
+
+// stages: steps of kRows rows in the ring (dynamic shared memory: [stages][x, dy(, residual)][kRows][pitch], at least
 // 2 * kCapacity floats for the column sums at the end); status: the staged row operators' device status word
 template <typename T, int E, int kVecs, int kLanes>
 __global__ void __launch_bounds__(32 * backward_warps(kLanes), backward_blocks_per_sm(kLanes))
@@ -144,6 +159,8 @@ layernorm_backward_resident_kernel(const LayerNormBackwardArgs<T> a, int stages,
     constexpr int kWarps = backward_warps(kLanes), kRows = 32 * kWarps / kLanes;
     constexpr int kCapacity = kLanes * kVecs * E, kPairs = kVecs * E / 2;
     constexpr bool kSingles = E == 1;  // a pair then spans two chunks, and rows come by plain loads
+    constexpr bool kPadded = kBackwardPadded<kLanes>;
+    const uint32_t pitch = backward_pitch<T, E, kVecs, kLanes>(a.cols);
     extern __shared__ __align__(16) uint8_t ring[];
     __shared__ __align__(16) float scratch[kLanes > 32 ? kRows : 1][kLanes > 32 ? 4 * (kLanes / 32) : 1];
     __shared__ uint64_t full[kBackwardMaxStages], empty[kBackwardMaxStages];
@@ -153,6 +170,8 @@ layernorm_backward_resident_kernel(const LayerNormBackwardArgs<T> a, int stages,
     const float inv_n = 1.0f / (float)a.cols, inv_d = a.cols > a.ddof ? 1.0f / (float)(a.cols - a.ddof) : 0.f;
     f32x2 gamma[kPairs], dgamma[kPairs], dbeta[kPairs];
     bool active[kVecs];
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) active[v] = (t + v * kLanes) * E < a.cols;
 
     auto unpack = [](const Raw (&raw)[kVecs], f32x2 (&p)[kPairs]) {
         if constexpr (kSingles) {
@@ -163,52 +182,77 @@ layernorm_backward_resident_kernel(const LayerNormBackwardArgs<T> a, int stages,
             for (int v = 0; v < kVecs; ++v) RowIo<T>::unpack_pairs(raw[v], p + v * (E / 2));
         }
     };
-    // the thread's chunks of a row; zeros past the row's end, or everywhere in a row that is not there
-    auto load = [&](const T *row, bool there, f32x2 (&p)[kPairs]) {
+    // the thread's chunks of a row in global memory; zeros past the row's end
+    auto load = [&](const T *row, f32x2 (&p)[kPairs]) {
         Raw raw[kVecs];
 #pragma unroll
-        for (int v = 0; v < kVecs; ++v) raw[v] = active[v] && there ? Chunk::load(row + (t + v * kLanes) * E) : Chunk::zero();
+        for (int v = 0; v < kVecs; ++v) raw[v] = active[v] ? Chunk::load(row + (t + v * kLanes) * E) : Chunk::zero();
         unpack(raw, p);
     };
+    // the same of a row in the ring, at the address of the thread's first chunk
+    auto staged = [&](uint32_t at, bool there, f32x2 (&p)[kPairs]) {
+        if constexpr (!kSingles) {
+            Raw raw[kVecs];
+#pragma unroll
+            for (int v = 0; v < kVecs; ++v) {
+                uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                if (kPadded || (active[v] && there))
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                                 : "r"(at + (uint32_t)(v * kLanes * 16)));
+                raw[v] = *reinterpret_cast<const Raw *>(&w);
+            }
+            unpack(raw, p);
+        }
+    };
 
-    // ring: step i of this block (rows step_row(i) .. + kRows - 1) lives in stage i % stages
-    const uint32_t tensor_bytes = (uint32_t)(kRows * a.cols * (int)sizeof(T)), stage_bytes = tensor_bytes * (a.residual ? 3u : 2u);
-    const long long steps = (a.rows - 1 - (long long)blockIdx.x * kRows) / ((long long)gridDim.x * kRows) + 1;  // the grid has no idle block
-    auto step_row = [&](long long i) { return ((long long)blockIdx.x + i * gridDim.x) * kRows; };
-    auto bring = [&](long long i) {
-        const int s = (int)(i % stages);
-        const long long first = step_row(i);
-        const uint32_t bytes = (uint32_t)(a.rows - first < kRows ? a.rows - first : kRows) * (uint32_t)a.cols * (uint32_t)sizeof(T);
-        const uint32_t bar = smem_u32(full + s), dst = smem_u32(ring) + (uint32_t)s * stage_bytes;
-        mbar_expect_tx(bar, a.residual ? 3u * bytes : 2u * bytes);
-        bulk_load_1d(dst, a.x + (size_t)first * a.cols, bytes, bar);
-        bulk_load_1d(dst + tensor_bytes, a.dy + (size_t)first * a.cols, bytes, bar);
-        if (a.residual) bulk_load_1d(dst + 2 * tensor_bytes, a.residual + (size_t)first * a.cols, bytes, bar);
+    // ring: step s of this block, rows first_row + s * stride .. + kRows - 1, lives in stage s % stages
+    const uint32_t tensor_bytes = kRows * pitch, stage_bytes = tensor_bytes * (a.residual ? 3u : 2u);
+    const long long first_row = (long long)blockIdx.x * kRows, stride = (long long)gridDim.x * kRows;
+    const int steps = (int)((a.rows - 1 - first_row) / stride) + 1;  // the grid has no idle block
+    auto bring = [&](long long row, uint32_t stage) {  // whole warp 0: one copy per tensor, or padded a lane per row
+        const int lane = threadIdx.x, rows = (int)(a.rows - row < kRows ? a.rows - row : kRows);
+        const uint32_t row_bytes = (uint32_t)a.cols * (uint32_t)sizeof(T), bar = smem_u32(full + stage);
+        if (lane == 0) mbar_expect_tx(bar, (a.residual ? 3u : 2u) * (uint32_t)rows * row_bytes);
+        __syncwarp();
+        if (lane < (kPadded ? rows : 1)) {
+            const uint32_t bytes = kPadded ? row_bytes : (uint32_t)rows * row_bytes;
+            const size_t at = (size_t)(row + lane) * a.cols;
+            const uint32_t dst = smem_u32(ring) + stage * stage_bytes + (uint32_t)lane * pitch;
+            bulk_load_1d(dst, a.x + at, bytes, bar);
+            bulk_load_1d(dst + tensor_bytes, a.dy + at, bytes, bar);
+            if (a.residual) bulk_load_1d(dst + 2 * tensor_bytes, a.residual + at, bytes, bar);
+        }
     };
     auto give_up = [&](unsigned code) {  // a wait ran out: the rest runs through without waiting, the host is told
         atomicCAS(status, 0u, code);
         *(volatile int *)&abort_flag = 1;
     };
 
-    if (!kSingles && threadIdx.x == 0) {
-        for (int s = 0; s < stages; ++s) {
-            mbar_init(smem_u32(full + s), 1);
-            mbar_init(smem_u32(empty + s), kWarps);
+    if constexpr (!kSingles) {
+        if constexpr (kPadded) {  // zeros behind every row of the ring, where the copies do not reach
+            const int pad = kCapacity / E - a.cols / E, pads = stages * (a.residual ? 3 : 2) * kRows * pad;
+            for (int i = threadIdx.x; i < pads; i += 32 * kWarps)
+                *reinterpret_cast<uint4 *>(ring + (size_t)(i / pad) * pitch + (size_t)(a.cols / E + i % pad) * 16) = make_uint4(0u, 0u, 0u, 0u);
         }
-        abort_flag = 0;
-        fence_barrier_init();
-        fence_proxy_async();
+        if (threadIdx.x == 0) {
+            for (int s = 0; s < stages; ++s) {
+                mbar_init(smem_u32(full + s), 1);
+                mbar_init(smem_u32(empty + s), kWarps);
+            }
+            abort_flag = 0;
+            fence_barrier_init();
+            fence_proxy_async();
+        }
+        __syncthreads();
     }
     grid_launch_dependents();
-    if (!kSingles) __syncthreads();
-#pragma unroll
-    for (int v = 0; v < kVecs; ++v) active[v] = (t + v * kLanes) * E < a.cols;
     grid_dependency_wait();
-    if (!kSingles && threadIdx.x == 0)
-        for (long long i = 0; i < stages && i < steps; ++i) bring(i);
+    if (!kSingles && threadIdx.x < 32)
+        for (int i = 0; i < stages && i < steps; ++i) bring(first_row + i * stride, (uint32_t)i);
     // a row's columns past the last one: x = dy = gamma = 0
     if (a.gamma) {
-        load(a.gamma, true, gamma);
+        load(a.gamma, gamma);
     } else {
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) {
@@ -219,21 +263,24 @@ layernorm_backward_resident_kernel(const LayerNormBackwardArgs<T> a, int stages,
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) dgamma[i] = dbeta[i] = pair_of(0.f, 0.f);
 
-    int stage = 0;
-    uint32_t phase = 0;
-    for (long long i = 0; i < steps; ++i) {
-        // all threads of a block make the same number of steps: a row past the end is zeros and nothing is stored
-        const long long r = step_row(i) + slot;
+    uint32_t stage = 0, phase = 0;
+    long long r = first_row + slot;
+    T *dx = a.dx + (size_t)r * a.cols + t * E;
+    const uint32_t my_chunks = smem_u32(ring) + (uint32_t)slot * pitch + (uint32_t)t * 16u;
+    for (int step = 0; step < steps; ++step, r += stride, dx += (size_t)stride * a.cols) {
         const bool there = r < a.rows;
+        // Rows past the end are met in the last step only.  Whole warps leave; parts of a warp stay for its shuffles, with
+        // zeros, and store nothing.
+        if (kLanes >= 32 && !there) break;
         f32x2 x[kPairs], dy[kPairs];
-        const T *staged = reinterpret_cast<const T *>(ring + (size_t)stage * stage_bytes) + slot * a.cols;
+        const uint32_t here = my_chunks + stage * stage_bytes;
         if constexpr (kSingles) {
-            load(a.x + (size_t)r * a.cols, there, x);
-            load(a.dy + (size_t)r * a.cols, there, dy);
+            load(a.x + (size_t)r * a.cols, x);
+            load(a.dy + (size_t)r * a.cols, dy);
         } else {
             if (!mbar_wait(smem_u32(full + stage), phase, &abort_flag)) give_up(2u);
-            load(staged, there, x);
-            load(staged + kRows * a.cols, there, dy);
+            staged(here, there, x);
+            staged(here + tensor_bytes, there, dy);
         }
         f32x2 sum_x2 = x[0], sum_w2 = pair_mul(dy[0], gamma[0]);
 #pragma unroll
@@ -248,10 +295,10 @@ layernorm_backward_resident_kernel(const LayerNormBackwardArgs<T> a, int stages,
         sum_w = lo + hi;
         reduce(sum_x, sum_w);
         // the stage of the step before: by now every warp of this row is done with it
-        if (!kSingles && threadIdx.x == 0 && i > 0 && i - 1 + stages < steps) {
-            const int before = stage ? stage - 1 : stages - 1;
+        if (!kSingles && threadIdx.x < 32 && step > 0 && step - 1 + stages < steps) {
+            const uint32_t before = stage ? stage - 1 : (uint32_t)stages - 1;
             if (!mbar_wait(smem_u32(empty + before), stage ? phase : phase ^ 1u, &abort_flag)) give_up(3u);
-            else bring(i - 1 + stages);
+            else bring(r - slot + (stages - 1) * stride, before);
         }
         const float mean = sum_x * inv_n;
         f32x2 minus_mean[kSingles ? kPairs : kVecs];  // 0 past the row's end: the deviation is 0 there
@@ -285,28 +332,29 @@ layernorm_backward_resident_kernel(const LayerNormBackwardArgs<T> a, int stages,
         }
         if (a.residual) {
             f32x2 add[kPairs];
-            load(kSingles ? a.residual + (size_t)r * a.cols : staged + 2 * kRows * a.cols, there, add);
+            if constexpr (kSingles) load(a.residual + (size_t)r * a.cols, add);
+            else staged(here + 2 * tensor_bytes, there, add);
 #pragma unroll
-            for (int i = 0; i < kPairs; ++i) x[i] = pair_add(x[i], add[i]);
+            for (int j = 0; j < kPairs; ++j) x[j] = pair_add(x[j], add[j]);
         }
         if constexpr (!kSingles) {
             __syncwarp();
             if ((threadIdx.x & 31) == 0) mbar_arrive(smem_u32(empty + stage));
-            if (++stage == stages) {
+            if (++stage == (uint32_t)stages) {
                 stage = 0;
                 phase ^= 1u;
             }
         }
-        if (there) {
-            T *out = a.dx + (size_t)r * a.cols + t * E;
+        if (kLanes >= 32 || there) {
 #pragma unroll
             for (int v = 0; v < kVecs; ++v)
                 if (active[v]) {
                     if constexpr (kSingles) {
+                        float lo, hi;
                         pair_split(x[v / 2], lo, hi);
-                        out[v * kLanes] = RowIo<T>::from_float(v & 1 ? hi : lo);
+                        dx[v * kLanes] = RowIo<T>::from_float(v & 1 ? hi : lo);
                     } else {
-                        Chunk::store(out + v * kLanes * E, RowIo<T>::pack_pairs(x + v * (E / 2)));
+                        Chunk::store(dx + v * kLanes * E, RowIo<T>::pack_pairs(x + v * (E / 2)));
                     }
                 }
         }
