@@ -134,9 +134,18 @@ int launch_product_pair(const CUtensorMap &ma, const CUtensorMap &mb, const CUte
 // Runs the product that `p` describes (M, N, K, D, fmt, out_fmt, b_row_major, bias, extra, pre, activation set by the
 // caller; the rest filled in here).  A: [M, K], or [K, M] for the weight gradient; B: [N, K], or [K, N] with b_row_major.
 // Everything has been checked but the workspace.  `first` launches what goes ahead of the product once nothing is left to
-// refuse, `beside` what may run beside it, between it and the sum of its slices.
+// refuse, `beside` what may run beside it, between it and the sum of its slices (both are told whether sums are promoted).
+template <class Epi>
+int launch_product(const ProductPlan &plan, bool tma, const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &md, const LinearParams &p,
+                   int sms, cudaStream_t s) {
+    if (plan.pair) return launch_product_pair<Epi>(ma, mb, md, p, s);
+    if (!tma) return launch_product_tile<Epi, 128, false>(ma, mb, md, p, sms, s);
+    if (plan.bn == 128) return launch_product_tile<Epi, 128, true>(ma, mb, md, p, sms, s);
+    return launch_product_tile<Epi, 256, true>(ma, mb, md, p, sms, s);
+}
+
 struct Nothing {
-    int operator()() const { return KO_OK; }
+    int operator()(bool) const { return KO_OK; }
 };
 template <LinearMode kMode, bool kOut16, class First = Nothing, class Beside = Nothing>
 int run_product(LinearParams p, const void *A, const void *B, void *workspace, size_t workspace_bytes, cudaStream_t s, const DeviceInfo &info,
@@ -179,13 +188,18 @@ int run_product(LinearParams p, const void *A, const void *B, void *workspace, s
         if (p.extra)
             if (int st = make_store_map(encode, &p.map_extra, Epi::kExtra16 ? p.fmt + 1 : 0, const_cast<void *>(p.extra), p.M, p.N, Epi::kChunk)) return st;
     }
-    int st = first();
+    // FP32 results of more than two periods of K a work unit: partial sums are promoted (see LinearEpilogue)
+    const long long unit_blocks = ((p.K + tc::kBK - 1) / tc::kBK + plan.split - 1) / plan.split;
+    const bool promote = !kOut16 && unit_blocks > 2 * tc::kPeriod;
+    int st = first(promote);
     if (st != KO_OK) return st;
-    if (plan.pair) st = launch_product_pair<Epi>(map_a, map_b, map_d, p, s);
-    else if (!tma) st = launch_product_tile<Epi, 128, false>(map_a, map_b, map_d, p, info.sm_count, s);
-    else if (plan.bn == 128) st = launch_product_tile<Epi, 128, true>(map_a, map_b, map_d, p, info.sm_count, s);
-    else st = launch_product_tile<Epi, 256, true>(map_a, map_b, map_d, p, info.sm_count, s);
-    if (st == KO_OK) st = beside();
+    if constexpr (!kOut16) {
+        if (promote) st = launch_product<LinearEpilogue<kMode, false, true>>(plan, tma, map_a, map_b, map_d, p, info.sm_count, s);
+        else st = launch_product<Epi>(plan, tma, map_a, map_b, map_d, p, info.sm_count, s);
+    } else {
+        st = launch_product<Epi>(plan, tma, map_a, map_b, map_d, p, info.sm_count, s);
+    }
+    if (st == KO_OK) st = beside(promote);
     if (st != KO_OK || plan.split <= 1) return st;
     const long long chunks = plan.tiles * 4 * (plan.bn / 32);
     return launch_overlapped(linear_slice_sum_kernel<kMode, kOut16>, (unsigned)chunks, 256u, (size_t)0, s, p, plan.bn);

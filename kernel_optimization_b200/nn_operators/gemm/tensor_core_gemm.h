@@ -49,6 +49,7 @@ constexpr int kBM = 128;          // rows of D per tile = TMEM lanes
 constexpr int kBK = 64;           // K elements per stage: 64 * 2 B = one 128-byte swizzle row
 constexpr int kUmmaK = 16;        // K per tcgen05.mma for 16-bit inputs
 constexpr int kThreads = 192;     // 6 warps: producer, MMA, 4 x epilogue
+constexpr int kPeriod = 32;       // K-blocks per accumulator where partial sums are promoted (2048 values of K)
 
 // codes written to the status word (first failure wins)
 enum : unsigned { kStatusOk = 0, kTimeoutProducer = 1, kTimeoutMma = 2, kTimeoutEpilogue = 3, kTimeoutDrain = 4 };
@@ -180,6 +181,18 @@ __device__ __forceinline__ void tmem_ld_32x32_issue(uint32_t taddr, uint32_t (&r
         : "r"(taddr)
         : "memory");
 }
+// 32 lanes x 32 consecutive FP32 columns from registers: thread t holds row (lane base + t)
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const float (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(taddr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]),
+        "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]), "f"(v[19]), "f"(v[20]), "f"(v[21]),
+        "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]), "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // Shared-memory matrix descriptor of a K-major operand tile stored as rows of 128 bytes with the
@@ -250,6 +263,7 @@ struct PlainEpilogue {
     static constexpr int kWarps = 4;  // epilogue warps, a multiple of 4: each quadrant of TMEM lanes is shared by kWarps / 4
     static constexpr bool kTransA = false;
     static constexpr bool kFused = false;
+    static constexpr bool kPromote = false; // true: partial sums of kPeriod K-blocks are added outside the tensor cores (see there)
     static constexpr bool kShares = false;  // true: launch_dependents only after the wait for the previous kernel; registers and memory left over
 };
 
@@ -507,6 +521,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int tiles_m = (p.M + kTileM - 1) / kTileM, tiles_n = p.tiles_n ? p.tiles_n : (p.N + BN - 1) / BN;
     const int k_blocks = (p.K + kBK - 1) / kBK;
+    [[maybe_unused]] const int period = Epi::kPromote ? kPeriod : k_blocks;  // K-blocks that share an accumulator
     // work units: (tile, K slice), the slices of a tile next to each other so that they run at the same time
     const int split = p.split_k > 1 ? p.split_k : 1;
     const long long num_units = (long long)tiles_m * tiles_n * split;
@@ -627,30 +642,35 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 column_tile<BN>(p, tn, col0, bn);
                 // bit 15: A is MN-major, bit 16: B is MN-major
                 const uint32_t idesc = make_idesc(p.fmt, kBM, bn) | (p.b_row_major ? 1u << 16 : 0u) | (Epi::kTransA ? 1u << 15 : 0u);
-                // MT = 1: two accumulators used in turn; MT = 2: one accumulator per half, both busy with every tile
-                const uint32_t acc = MT == 1 ? (local_tile & 1u) : 0u, acc_phase = (MT == 1 ? (local_tile >> 1) : local_tile) & 1u;
-                if (!mbar_wait(acc_free_bar(acc), acc_phase ^ 1u, abort_flag)) { ok = false; break; }
-                tc_fence_after();
-                const uint32_t d_tmem = tmem_base + acc * BN;
-                for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    if (!mbar_wait(full_bar(stage), phase, abort_flag)) { ok = false; break; }
+                // MT = 1: two accumulators used in turn; MT = 2: one accumulator per half, both busy with every tile.  A promoting
+                // epilogue takes a tile in periods, each with an accumulator of its own.
+                for (int k0 = kb0; k0 < kb1 && ok; k0 += period) {
+                    if (k0 != kb0) ++local_tile;
+                    const int k_end = Epi::kPromote ? min(k0 + period, kb1) : kb1;
+                    const uint32_t acc = MT == 1 ? (local_tile & 1u) : 0u, acc_phase = (MT == 1 ? (local_tile >> 1) : local_tile) & 1u;
+                    if (!mbar_wait(acc_free_bar(acc), acc_phase ^ 1u, abort_flag)) { ok = false; break; }
                     tc_fence_after();
-                    // descriptors of this stage: the ring's plus the stage's offset in 16-byte units
-                    const uint32_t a_lo = a_lo0 + stage * (uint32_t)(Cfg::kStageBytes >> 4), b_lo = b_lo0 + stage * (uint32_t)(Cfg::kStageBytes >> 4);
-                    uint32_t accumulate = kb != kb0 ? 1u : 0u;
+                    const uint32_t d_tmem = tmem_base + acc * BN;
+                    for (int kb = k0; kb < k_end; ++kb, ++it) {
+                        if (!mbar_wait(full_bar(stage), phase, abort_flag)) { ok = false; break; }
+                        tc_fence_after();
+                        // descriptors of this stage: the ring's plus the stage's offset in 16-byte units
+                        const uint32_t a_lo = a_lo0 + stage * (uint32_t)(Cfg::kStageBytes >> 4), b_lo = b_lo0 + stage * (uint32_t)(Cfg::kStageBytes >> 4);
+                        uint32_t accumulate = kb != k0 ? 1u : 0u;
 #pragma unroll
-                    for (int k = 0; k < kBK / kUmmaK; ++k) {
-                        // advancing K inside the swizzled row: +32 bytes per 16 elements (K-major); row-major B: 16 K-rows
-                        // further = two 8-row atoms = 2048 bytes
-                        umma_f16_words(d_tmem, a_lo + k * a_kstep, desc_hi, b_lo + k * b_kstep, desc_hi, idesc, accumulate);
-                        if (MT == 2)  // rows 128..255 of the tile: 16 KB further in the stage, accumulator columns BN..2BN-1
-                            umma_f16_words(d_tmem + BN, a_lo + (kBM * kBK * 2 >> 4) + k * a_kstep, desc_hi, b_lo + k * b_kstep, desc_hi, idesc, accumulate);
-                        accumulate = 1u;
+                        for (int k = 0; k < kBK / kUmmaK; ++k) {
+                            // advancing K inside the swizzled row: +32 bytes per 16 elements (K-major); row-major B: 16 K-rows
+                            // further = two 8-row atoms = 2048 bytes
+                            umma_f16_words(d_tmem, a_lo + k * a_kstep, desc_hi, b_lo + k * b_kstep, desc_hi, idesc, accumulate);
+                            if (MT == 2)  // rows 128..255 of the tile: 16 KB further in the stage, accumulator columns BN..2BN-1
+                                umma_f16_words(d_tmem + BN, a_lo + (kBM * kBK * 2 >> 4) + k * a_kstep, desc_hi, b_lo + k * b_kstep, desc_hi, idesc, accumulate);
+                            accumulate = 1u;
+                        }
+                        umma_commit(empty_bar(stage));  // the stage is reusable once these MMAs have read it
+                        if (++stage == (uint32_t)Cfg::kStages) { stage = 0; phase ^= 1u; }
                     }
-                    umma_commit(empty_bar(stage));  // the stage is reusable once these MMAs have read it
-                    if (++stage == (uint32_t)Cfg::kStages) { stage = 0; phase ^= 1u; }
+                    if (ok) umma_commit(acc_ready_bar(acc));
                 }
-                if (ok) umma_commit(acc_ready_bar(acc));
             }
             if (!ok) {
                 if (!*abort_flag) atomicCAS(p.status, kStatusOk, kTimeoutMma);
@@ -682,10 +702,16 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             unit_of(u, t, slice, kb0, kb1);
             tile_of(p, t, tiles_m, tiles_n, tm, tn);
             column_tile<BN>(p, tn, col0, bn);
-            const uint32_t acc = MT == 1 ? (local_tile & 1u) : 0u, acc_phase = (MT == 1 ? (local_tile >> 1) : local_tile) & 1u;
             if constexpr (Epi::kFused)  // the first chunk's operand arrives while the tile is still being computed
                 if (kTmaStore && split == 1) Epi::bring(fused, p, tm * kTileM + quad * 32, col0 + share * Epi::kChunk, lane);
-            if (!mbar_wait(acc_ready_bar(acc), acc_phase, abort_flag)) {
+            if constexpr (Epi::kPromote) {
+                const int periods = (kb1 - kb0 + kPeriod - 1) / kPeriod;
+                ok = Epi::template promote<BN, false>(tmem_base + ((uint32_t)(quad * 32) << 16), share, periods, local_tile, acc_ready_bar(0),
+                                                      acc_free_bar(0), abort_flag);
+                local_tile += (uint32_t)periods - 1;  // the accumulator that holds the sums
+            }
+            const uint32_t acc = MT == 1 ? (local_tile & 1u) : 0u, acc_phase = (MT == 1 ? (local_tile >> 1) : local_tile) & 1u;
+            if (!ok || (!Epi::kPromote && !mbar_wait(acc_ready_bar(acc), acc_phase, abort_flag))) {
                 if (lane == 0 && !*abort_flag) atomicCAS(p.status, kStatusOk, kTimeoutEpilogue);
                 *abort_flag = 1;
                 ok = false;

@@ -146,6 +146,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     const int tiles_m = (p.M + kTileM - 1) / kTileM, tiles_n = p.tiles_n ? p.tiles_n : (p.N + BN - 1) / BN;
     const long long num_tiles = (long long)tiles_m * tiles_n;
     const int k_blocks = (p.K + kBK - 1) / kBK;
+    [[maybe_unused]] const int period = Epi::kPromote ? kPeriod : k_blocks;  // K-blocks that share an accumulator
     const long long pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
     if (threadIdx.x == 0) {
@@ -248,28 +249,32 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                 column_tile<BN>(p, tn, col0, bn);
                 // bit 15: A is MN-major, bit 16: B is MN-major
                 const uint32_t idesc = make_idesc(p.fmt, kTileM, bn) | (p.b_row_major ? 1u << 16 : 0u) | (Epi::kTransA ? 1u << 15 : 0u);
-                const uint32_t acc = local_tile & 1u, acc_phase = (local_tile >> 1) & 1u;
-                if (!mbar_wait_remote(acc_free_bar(acc), acc_phase ^ 1u, abort_flag)) { ok = false; break; }
-                tc_fence_after();
-                const uint32_t d_tmem = tmem_base + acc * BN;
-                for (int kb = 0; kb < k_blocks; ++kb, ++it) {
-                    if (!mbar_wait(full_bar(stage), phase, abort_flag)) { ok = false; break; }
+                for (int k0 = 0; k0 < k_blocks && ok; k0 += period) {
+                    if (k0 != 0) ++local_tile;
+                    const int k_end = Epi::kPromote ? min(k0 + period, k_blocks) : k_blocks;
+                    const uint32_t acc = local_tile & 1u, acc_phase = (local_tile >> 1) & 1u;
+                    if (!mbar_wait_remote(acc_free_bar(acc), acc_phase ^ 1u, abort_flag)) { ok = false; break; }
                     tc_fence_after();
-                    const uint32_t a_lo = a_lo0 + stage * (uint32_t)(Cfg::kStageBytes >> 4), b_lo = b_lo0 + stage * (uint32_t)(Cfg::kStageBytes >> 4);
-                    uint32_t accumulate = kb != 0 ? 1u : 0u;
+                    const uint32_t d_tmem = tmem_base + acc * BN;
+                    for (int kb = k0; kb < k_end; ++kb, ++it) {
+                        if (!mbar_wait(full_bar(stage), phase, abort_flag)) { ok = false; break; }
+                        tc_fence_after();
+                        const uint32_t a_lo = a_lo0 + stage * (uint32_t)(Cfg::kStageBytes >> 4), b_lo = b_lo0 + stage * (uint32_t)(Cfg::kStageBytes >> 4);
+                        uint32_t accumulate = kb != k0 ? 1u : 0u;
 #pragma unroll
-                    for (int k = 0; k < kBK / kUmmaK; ++k) {
-                        umma_f16_pair_words(d_tmem, a_lo + k * a_kstep, desc_hi, b_lo + k * b_kstep, desc_hi, idesc, accumulate);
-                        accumulate = 1u;
+                        for (int k = 0; k < kBK / kUmmaK; ++k) {
+                            umma_f16_pair_words(d_tmem, a_lo + k * a_kstep, desc_hi, b_lo + k * b_kstep, desc_hi, idesc, accumulate);
+                            accumulate = 1u;
+                        }
+                        // the stage is reusable once these MMAs have read it (in both CTAs: the commit tracks both SMs); the
+                        // leader's producer passes the release on to the peer
+                        umma_commit_pair(own_empty0 + 8u * stage);
+                        if (++stage == (uint32_t)Cfg::kStages) { stage = 0; phase ^= 1u; }
                     }
-                    // the stage is reusable once these MMAs have read it (in both CTAs: the commit tracks both SMs); the
-                    // leader's producer passes the release on to the peer
-                    umma_commit_pair(own_empty0 + 8u * stage);
-                    if (++stage == (uint32_t)Cfg::kStages) { stage = 0; phase ^= 1u; }
-                }
-                if (ok) {
-                    umma_commit_pair(own_ready0 + 8u * acc);
-                    umma_commit_pair(peer_ready0 + 8u * acc);
+                    if (ok) {
+                        umma_commit_pair(own_ready0 + 8u * acc);
+                        umma_commit_pair(peer_ready0 + 8u * acc);
+                    }
                 }
             }
             if (!ok) {
@@ -298,10 +303,16 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
             int tm, tn, col0, bn;
             tile_of(p, t, tiles_m, tiles_n, tm, tn);
             column_tile<BN>(p, tn, col0, bn);
-            const uint32_t acc = local_tile & 1u, acc_phase = (local_tile >> 1) & 1u;
             const int row_base = tm * kTileM + (int)rank * kBM + quad * 32;
             if constexpr (Epi::kFused) Epi::bring(fused, p, row_base, col0 + share * Epi::kChunk, lane);  // while the tile is being computed
-            if (!mbar_wait(acc_ready_bar(acc), acc_phase, abort_flag)) {
+            if constexpr (Epi::kPromote) {
+                const int periods = (k_blocks + kPeriod - 1) / kPeriod;
+                ok = Epi::template promote<BN, true>(tmem_base + ((uint32_t)(quad * 32) << 16), share, periods, local_tile, acc_ready_bar(0),
+                                                     map_to_cluster_rank(acc_free_bar(0), 0), abort_flag);
+                local_tile += (uint32_t)periods - 1;  // the accumulator that holds the sums
+            }
+            const uint32_t acc = local_tile & 1u, acc_phase = (local_tile >> 1) & 1u;
+            if (!ok || (!Epi::kPromote && !mbar_wait(acc_ready_bar(acc), acc_phase, abort_flag))) {
                 if (lane == 0 && !*abort_flag) atomicCAS(p.status, kStatusOk, kTimeoutEpilogue);
                 *abort_flag = 1;
                 ok = false;

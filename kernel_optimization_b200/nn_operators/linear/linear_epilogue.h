@@ -79,16 +79,23 @@ __device__ __forceinline__ void linear_store_one(const LinearParams &p, float v,
     else static_cast<float *>(p.D)[at] = v;
 }
 
-template <LinearMode kMode, bool kOut16>
+// kPromote (FP32 results of long sums): the tensor cores cut their accumulator off at every addition instead of rounding it, so an
+// error grows with K on the side of smaller magnitudes -- 1.9e-5 of the result (2-norm) for 16384 tokens, where a blocked FP32
+// sum is off by 1.5e-6.  A tile is then taken in periods of 2048 values of K, each into the other of the two
+// accumulators, and the epilogue warps add the periods' sums, rounded to nearest, in registers (128 a thread for a tile 256
+// columns wide) while the next period is being multiplied: as exact as a period, and hidden.
+template <LinearMode kMode, bool kOut16, bool kPromoteSums = false>
 struct LinearEpilogue {
     using Params = LinearParams;
     static constexpr bool kTransA = kMode == LinearMode::kWeightGrad;
-    static constexpr int kWarps = kTransA ? 4 : 8;
+    static constexpr bool kPromote = kPromoteSums;
+    static constexpr int kWarps = kTransA && !kPromote ? 4 : 8;
+    static_assert(!kPromote || !kOut16, "what is rounded to 16 bits does not show it");
     static constexpr bool kFused = true;
     // The weight gradient shares its SMs with the column sums of the bias gradient: it asks for dependents only once its own
     // inputs are there (see column_sum_kernel), and leaves registers (at most 168 a thread, as for two blocks) and the little
     // shared memory that the sums need.
-    static constexpr bool kShares = kTransA;
+    static constexpr bool kShares = kTransA && !kPromote;
     static constexpr bool kExtra16 = kMode == LinearMode::kInputGrad || kOut16;
     static constexpr int kChunk = kOut16 ? 64 : 32;           // columns
     static constexpr int kStep = kChunk * (kWarps / 4);        // from one chunk of a warp to its next
@@ -103,6 +110,51 @@ struct LinearEpilogue {
         bool coming = false;  // an extra load has been issued and not waited for
     };
 
+    // The promoted sums of a tile's `periods` accumulators, the first of them number `first` of the CTA's sequence: all but the
+    // last are added up in registers -- this warp's 32 rows of the chunks share * 32, share * 32 + 64, ... -- and given
+    // back; the last receives the total, for the rest of the epilogue to find there.  t_rows: TMEM address of the warp's
+    // rows in accumulator 0; ready, free: the accumulators' mbarriers (free as a shared::cluster address where the MMAs are
+    // issued by another CTA).  False when a wait ran out.  A function of its own, so that its registers and those of the
+    // code around it do not add up.
+    template <int BN, bool kRemote>
+    __device__ __noinline__ static bool promote(uint32_t t_rows, int share, int periods, uint32_t first, uint32_t ready, uint32_t free,
+                                                volatile int *abort_flag) {
+        constexpr int kChunks = BN / 64;
+        f32x2 sums[kChunks][16];
+        for (uint32_t n = first; n < first + (uint32_t)periods; ++n) {
+            const uint32_t acc = n & 1u, t_row = t_rows + acc * BN + share * 32;
+            if (!mbar_wait(ready + 8u * acc, (n >> 1) & 1u, abort_flag)) return false;
+            tc::tc_fence_after();
+            const bool last = n + 1 == first + (uint32_t)periods;
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) {
+                float f[32];
+                tc::tmem_ld_32x32(t_row + j * 64, f);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const f32x2 part = pair_of(f[2 * i], f[2 * i + 1]);
+                    sums[j][i] = n == first ? part : pair_add(sums[j][i], part);
+                }
+                if (last) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) pair_split(sums[j][i], f[2 * i], f[2 * i + 1]);
+                    tc::tmem_st_32x32(t_row + j * 64, f);
+                }
+            }
+            if (last) {
+                tc::tmem_st_wait();
+            } else {
+                tc::tc_fence_before();
+                __syncwarp();
+                if ((threadIdx.x & 31) == 0) {
+                    if constexpr (kRemote) mbar_arrive_cluster(free + 8u * acc);
+                    else mbar_arrive(free + 8u * acc);
+                }
+            }
+        }
+        return true;
+    }
+
     // the extra operand's chunk at (row_base, col) on its way into box 1
     __device__ __forceinline__ static void bring(State &st, const Params &p, int row_base, int col, int lane) {
         if (p.extra == nullptr || row_base >= p.M || col >= p.N) return;
@@ -114,11 +166,11 @@ struct LinearEpilogue {
         st.coming = true;
     }
 
-    // rows row_base .. + 31 of a tile (accumulator at TMEM address t_row), this warp's chunks c_begin, c_begin + kStep, ...
-    // to D and Z; false when a wait ran out
+    // rows row_base .. + 31 of a tile, this warp's chunks c_begin, c_begin + kStep, ... of the accumulator at TMEM address t_row, to
+    // D and Z; false when a wait ran out
     template <bool kTmaStore>
-    __device__ __forceinline__ static bool block(const CUtensorMap *map_d, const Params &p, State &st, uint32_t t_row, int row_base, int col0,
-                                                 int bn, int c_begin, int lane, volatile int *abort_flag) {
+    __device__ __forceinline__ static bool block(const CUtensorMap *map_d, const Params &p, State &st, uint32_t t_row, int row_base,
+                                                 int col0, int bn, int c_begin, int lane, volatile int *abort_flag) {
 #pragma unroll 1
         for (int c0 = c_begin; c0 < bn; c0 += kStep) {
             if (row_base >= p.M || col0 + c0 >= p.N) break;
@@ -133,9 +185,8 @@ struct LinearEpilogue {
             } else {
 #pragma unroll 1
                 for (int h = 0; h < kChunk; h += 32) {
-                    uint32_t r[32];
-                    tc::tmem_ld_32x32_issue(t_row + c0 + h, r);
-                    tc::tmem_ld_wait();
+                    f32x2 r[16];
+                    sums_at(t_row + c0 + h, r);
                     if (p.fmt) chunk_by_rows<true>(p, r, row_base, col0 + c0 + h, lane, st.boxes);
                     else chunk_by_rows<false>(p, r, row_base, col0 + c0 + h, lane, st.boxes);
                 }
@@ -156,10 +207,14 @@ private:
     // c ^ r: no bank conflict either way) so that a lane has one column, and every access is 32 neighbouring elements of
     // a row.  Written straight from a lane's own row, each store touched 32 sectors: 1021 x 2053 x 1096 FP32 22 us.
     template <bool kBf16>
-    __device__ __forceinline__ static void chunk_by_rows(const Params &p, const uint32_t (&r)[32], int row_base, int col, int lane, uint32_t box) {
+    __device__ __forceinline__ static void chunk_by_rows(const Params &p, const f32x2 (&r)[16], int row_base, int col, int lane, uint32_t box) {
         __syncwarp();
 #pragma unroll
-        for (int c = 0; c < 32; ++c) asm volatile("st.shared.b32 [%0], %1;" ::"r"(box + (uint32_t)(lane * 32 + (c ^ lane)) * 4u), "r"(r[c]) : "memory");
+        for (int c = 0; c < 32; ++c) {
+            float lo, hi;
+            pair_split(r[c / 2], lo, hi);
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(box + (uint32_t)(lane * 32 + (c ^ lane)) * 4u), "f"(c & 1 ? hi : lo) : "memory");
+        }
         __syncwarp();
         const int c = col + lane, rows = min(32, p.M - row_base);
         if (c >= p.N) return;
@@ -269,11 +324,16 @@ private:
         }
         ++st.stores;
     }
-    // 32 accumulator columns plus the bias
-    template <bool kBf16>
-    __device__ __forceinline__ static void accumulators(const Params &p, uint32_t taddr, int col, f32x2 (&v)[16]) {
+    __device__ __forceinline__ static void sums_at(uint32_t taddr, f32x2 (&v)[16]) {
         uint32_t r[32];
         tc::tmem_ld_32x32_issue(taddr, r);
+        tc::tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = pair_of(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+    }
+    // 32 sums (columns col .. of the matrix) plus the bias
+    template <bool kBf16>
+    __device__ __forceinline__ static void biased(const Params &p, uint32_t taddr, int col, f32x2 (&v)[16]) {
         uint4 bias[4];
         if constexpr (kMode == LinearMode::kForward) {
             if (p.bias) {
@@ -282,9 +342,7 @@ private:
                 for (int j = 0; j < 4; ++j) bias[j] = col + j * 8 < p.N ? at[j] : make_uint4(0u, 0u, 0u, 0u);
             }
         }
-        tc::tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = pair_of(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+        sums_at(taddr, v);
         if constexpr (kMode == LinearMode::kForward) {
             if (p.bias) {
 #pragma unroll
@@ -304,12 +362,12 @@ private:
         constexpr int kHalves = kChunk / 32;
         constexpr int kRow16 = kOut16 ? 128 : 64;  // bytes of a 16-bit tensor's box row
         const bool keep_z = kMode == LinearMode::kForward && p.pre != nullptr;
-        if (keep_z && p.extra) {  // box 1 is taken: Z goes ahead through box 0, from a reading of the accumulators of its own
+        if (keep_z && p.extra) {  // box 1 is taken: Z goes ahead through box 0, from a reading of the sums of its own
             const uint32_t box = free_box(st, p, lane);
 #pragma unroll 1
             for (int h = 0; h < kHalves; ++h) {
                 f32x2 v[16];
-                accumulators<kBf16>(p, taddr + h * 32, col + h * 32, v);
+                biased<kBf16>(p, taddr + h * 32, col + h * 32, v);
                 put16<kBf16, kRow16>(v, box, lane, h * 4);
             }
             send(st, &p.map_pre, box, row_base, col, lane);
@@ -324,7 +382,7 @@ private:
                     for (int j = 0; j < 4; ++j) extra[j] = get_piece(piece<128>(z_box, lane, h * 4 + j));
                 if (h == 1) next_extra(st, p, row_base, col, more, lane);
                 f32x2 v[16];
-                accumulators<kBf16>(p, taddr + h * 32, col + h * 32, v);
+                biased<kBf16>(p, taddr + h * 32, col + h * 32, v);
                 if constexpr (kMode == LinearMode::kForward) {
                     if (keep_z && !p.extra) put16<kBf16, 128>(v, z_box, lane, h * 4);
                     with_activation(p.activation, [&](auto act) {
@@ -357,7 +415,7 @@ private:
             // FP32 results: the accumulators go to the box as they are; activation, slope or addition (library functions of
             // some 40 instructions) then work on the lane's row of it, four values at a time
             f32x2 v[16];
-            accumulators<kBf16>(p, taddr, col, v);
+            biased<kBf16>(p, taddr, col, v);
             if (keep_z && !p.extra) put16<kBf16, 64>(v, z_box, lane, 0);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -458,7 +516,7 @@ __global__ void __launch_bounds__(256) linear_slice_sum_kernel(const LinearParam
 // and visible when this kernel starts, and it reads and writes nothing the product writes.  It waits for the product before
 // it ends, so whatever follows it in the stream also follows the product.  (Loads past the L1, which may hold lines of an
 // earlier kernel.)
-template <bool kBf16, int kWarps = 8>
+template <bool kBf16, int kWarps>
 __global__ void __launch_bounds__(32 * kWarps, 32 / kWarps) column_sum_kernel(const uint16_t *in, long long rows, int cols, float *out) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();

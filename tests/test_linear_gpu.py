@@ -222,6 +222,62 @@ def test_no_tokens(cuda, ko):
     assert cuda.equal(ko.linear_backward_weight(dy, x, c, return_bias=False), c)
 
 
+@pytest.mark.parametrize("n,k", [(256, 512), (1032, 264), (2048, 2048)])
+def test_fp32_results_of_long_sums(cuda, lib, ko, n, k):
+    """Tensor cores cut an accumulator off at every addition: up to 2^-23 of it per instruction (16 terms), half of that on
+    average, always towards zero.  Sums kept in FP32 are therefore taken in periods of 2048 terms, 128 instructions, and the
+    periods' sums added with rounding: off by 128 * 2^-24 plus half a step per period, relative to the sums' size (2-norm over
+    all results, whose partial sums are no larger than the results on the whole).  A single accumulator over all 16384 terms
+    is off by 1.9e-5."""
+    m = 16384
+    bound = 128 * 2.0 ** -24 + m / 2048 * 2.0 ** -24
+
+    def off(got, want):
+        return ((got.double() - want).norm() / want.norm()).item()
+
+    dt = cuda.bfloat16
+    dy, x = _randn(cuda, (m, n), dt, 1), _randn(cuda, (m, k), dt, 2)
+    c = _randn(cuda, (n, k), cuda.float32, 3)
+    want = dy.double().t() @ x.double()
+    dw, db = ko.linear_backward_weight(dy, x)
+    assert off(dw, want) <= bound and off(db, dy.double().sum(0)) <= bound
+    assert off(ko.linear_backward_weight(dy, x, c, return_bias=False), want + c.double()) <= bound
+    a, w = dy.t().contiguous(), x.t().contiguous()      # the same sums as a forward product and as an input gradient
+    assert off(ko.linear(a, w, out_dtype=cuda.float32), want) <= bound
+    assert off(ko.linear_backward_input(a, x, out_dtype=cuda.float32), want) <= bound
+    assert lib.ko_poll_device_status() == 0
+
+
+@pytest.mark.parametrize("tile,slices", [(128, 0), (128, 3), (256, 0), (256, 2), (2048, 0)])
+def test_every_plan_of_the_three_products(cuda, lib, ko, tile, slices):
+    """Pinned tiles and K slices, with short and long sums, FP32 and 16-bit results."""
+    P = lambda t: None if t is None else t.data_ptr()
+    dt, s = cuda.bfloat16, cuda.cuda.current_stream().cuda_stream
+    ws = cuda.empty(1 << 27, dtype=cuda.uint8, device="cuda")
+    for m, n, k in ((300, 264, 392), (520, 392, 4104), (4104, 520, 264)):
+        x, w, z = _randn(cuda, (m, k), dt, 1), _randn(cuda, (n, k), dt, 2, k ** -0.5), _randn(cuda, (m, k), dt, 3, 1.5)
+        dy, bias = _randn(cuda, (m, n), dt, 4), _randn(cuda, (n,), dt, 5)
+        for odt, fmt in ((dt, 2), (cuda.float32, 0)):
+            r, c = _randn(cuda, (m, n), odt, 6), _randn(cuda, (n, k), odt, 7)
+            y, pre = cuda.full((m, n), float("nan"), dtype=odt, device="cuda"), cuda.empty(m, n, dtype=dt, device="cuda")
+            dx, dw = cuda.full((m, k), float("nan"), dtype=odt, device="cuda"), cuda.full((n, k), float("nan"), dtype=odt, device="cuda")
+            db = cuda.empty(n, device="cuda")
+            assert lib.ko_linear_tuned(1, fmt, 4, m, n, k, P(x), P(w), P(bias), P(r), P(y), P(pre), P(ws), ws.numel(), tile, slices, s) == 0
+            assert lib.ko_linear_backward_input_tuned(1, fmt, 2, m, n, k, P(dy), P(w), P(z), P(dx), P(ws), ws.numel(), tile, slices, s) == 0
+            assert lib.ko_linear_backward_weight_tuned(1, fmt, m, n, k, P(dy), P(x), P(c), P(dw), P(db), P(ws), ws.numel(), tile, slices, s) == 0
+            assert lib.ko_poll_device_status() == 0
+            z0 = x.double() @ w.double().t() + bias.double()
+            err = _sum_error(x, w.t(), k) + 2.0 ** -23 * z0.abs()
+            _close(cuda, pre, z0, err, "pre")
+            _close(cuda, y, _act(cuda, z0, "silu") + r.double(), 1.13 * err + _own_error(z0, not fmt) + 2.0 ** -23 * (z0.abs() + r.double().abs()), "y")
+            plain = dy.double() @ w.double()
+            _close(cuda, dx, plain * _slope(cuda, z.double(), "gelu"),
+                   1.13 * _sum_error(dy, w, n) + plain.abs() * (_own_error(z.double(), not fmt) + 2.0 ** -23), "dx")
+            want = dy.double().t() @ x.double() + c.double()
+            _close(cuda, dw, want, _sum_error(dy.t(), x, m) + 2.0 ** -23 * want.abs(), "dw")
+            _close(cuda, db, dy.double().sum(0), (m / 8 + 64) * 2.0 ** -24 * dy.double().abs().sum(0), "db")
+
+
 def test_no_input_features(cuda, ko):
     """k = 0: dw is empty, the bias gradient is still the column sums."""
     for m, n in ((5, 64), (3000, 200)):
