@@ -11,7 +11,8 @@ int check_linear(const char *name, int in_fmt, int out_fmt, int activation, int6
     KO_REQUIRE(out_fmt == 0 || out_fmt == in_fmt + 1, KO_ERR_INVALID_ARG, "%s: out_fmt must be 0 (f32) or the input type's %d", name, in_fmt + 1);
     KO_REQUIRE(activation >= 0 && activation < kActCount, KO_ERR_INVALID_ARG, "%s: unknown activation %d", name, activation);
     KO_REQUIRE(M >= 0 && N >= 0 && K >= 0, KO_ERR_INVALID_ARG, "%s: negative shape {%lld,%lld,%lld}", name, (long long)M, (long long)N, (long long)K);
-    KO_REQUIRE(M <= 0x7fffff00 && N <= 0x7fffff00 && K <= 0x7fffff00, KO_ERR_SHAPE, "%s: a dimension exceeds 2^31-256", name);
+    // room for a last step past the end in 32-bit counters
+    KO_REQUIRE(M <= 0x7fff0000 && N <= 0x7fff0000 && K <= 0x7fff0000, KO_ERR_SHAPE, "%s: a dimension exceeds 2^31-65536", name);
     return KO_OK;
 }
 

@@ -319,7 +319,7 @@ layernorm_backward_resident_kernel(const LayerNormBackwardArgs<T> a, int stages,
         pair_split(sum_wd2, lo, hi);
         sum_wd = lo + hi;
         reduce(m2, sum_wd);
-        const float rstd = rsqrtf(fmaf(m2, inv_d, a.eps));
+        const float rstd = there ? rsqrtf(fmaf(m2, inv_d, a.eps)) : 0.f;  // (eps may be 0, and then 0 * rstd no longer is)
         // dx = rstd w - rstd c1 - xhat rstd c2, c1 = sum(w) / n, c2 = sum(w xhat) / d
         const float offset = -rstd * sum_w * inv_n, slope = -rstd * (sum_wd * rstd * inv_d);
         const f32x2 rstd2 = pair_of(rstd, rstd), offset2 = pair_of(offset, offset), slope2 = pair_of(slope, slope);

@@ -15,8 +15,9 @@
 //               in Phi up to there, and it falls on below the FP32 range, so a gelu is off by at most 6e-7
 //   its slope   g(-a) = Phi(-a) - a phi(a) = e^(-a^2 / 2) r(a), g(a) = 1 - g(-a), r of degree 8 fitted the same way on [0, 5]
 //               with the weight e^(-a^2 / 2): 1.1e-6
-//   logistic    two reciprocals from one: 1 / u = v / (u v).  2^x is cut off at 2^60, so that u v stays finite; the logistic
-//               is then 1e-18 instead of less
+//   logistic    two reciprocals from one: 1 / u = v / (u v).  Arguments are held above -41 (silu) or where the cubic reaches that
+//               (gelu_tanh: z = -7.4), so that u v stays finite; the results there are 1e-16 in magnitude instead of less
+// Limits are put with max.NaN / min.NaN: a NaN stays one.
 // Half a step of FP16 is 2.4e-4 of a value.
 #pragma once
 
@@ -63,11 +64,33 @@ __device__ __forceinline__ float slope_exact(float z) {
 // ---- fast forms, two values ----
 __device__ __forceinline__ f32x2 both(float v) { return pair_of(v, v); }
 
-// 1 / (1 + 2^x), x = -v log2(e) for the logistic function of v
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 at_least_pair(f32x2 z, float limit) {
+    float a, b;
+    pair_split(z, a, b);
+    return pair_of(max_nan(a, limit), max_nan(b, limit));
+}
+__device__ __forceinline__ f32x2 at_most_pair(f32x2 z, float limit) {
+    float a, b;
+    pair_split(z, a, b);
+    return pair_of(min_nan(a, limit), min_nan(b, limit));
+}
+
+// 1 / (1 + 2^x), x = -v log2(e) for the logistic function of v, x <= 62.  (fminf takes the 62 for a NaN, which would reach the
+// other value through the common reciprocal; the callers multiply by what is still a NaN.)
 __device__ __forceinline__ f32x2 logistic_pair(f32x2 x) {
     float x0, x1, u, v;
     pair_split(x, x0, x1);
-    const f32x2 d = pair_add(pair_of(exp2_approx(fminf(x0, 60.f)), exp2_approx(fminf(x1, 60.f))), both(1.f));
+    const f32x2 d = pair_add(pair_of(exp2_approx(fminf(x0, 62.f)), exp2_approx(fminf(x1, 62.f))), both(1.f));
     pair_split(d, u, v);
     return pair_mul(pair_of(v, u), both(rcp_approx(u * v)));
 }
@@ -99,10 +122,12 @@ __device__ __forceinline__ f32x2 activate_pair(f32x2 z) {
         pair_split(p, p0, p1);
         return pair_mul(z, reflect_pair(z, pair_of(exp2_approx(p0), exp2_approx(p1))));
     } else if constexpr (kAct == kActGeluTanh) {
-        const f32x2 u = pair_fma(both(-kLog2e * kTwoRoot2OverPi * 0.044715f), pair_mul(z, z), both(-kLog2e * kTwoRoot2OverPi));
-        return pair_mul(z, logistic_pair(pair_mul(z, u)));
+        const f32x2 t = at_least_pair(z, -7.4f);
+        const f32x2 u = pair_fma(both(-kLog2e * kTwoRoot2OverPi * 0.044715f), pair_mul(t, t), both(-kLog2e * kTwoRoot2OverPi));
+        return pair_mul(t, logistic_pair(pair_mul(t, u)));
     } else if constexpr (kAct == kActSilu) {
-        return pair_mul(z, logistic_pair(pair_mul(z, both(-kLog2e))));
+        const f32x2 t = at_least_pair(z, -41.f);
+        return pair_mul(t, logistic_pair(pair_mul(t, both(-kLog2e))));
     }
     return z;
 }
@@ -114,9 +139,8 @@ __device__ __forceinline__ f32x2 slope_pair(f32x2 z) {
         pair_split(z, a, b);
         return pair_of(a > 0.f ? 1.f : 0.f, b > 0.f ? 1.f : 0.f);
     } else if constexpr (kAct == kActGelu) {
-        float a0, a1, e0, e1;
-        pair_split(magnitude_pair(z), a0, a1);
-        const f32x2 a = pair_of(fminf(a0, 16.f), fminf(a1, 16.f));  // e^-128 = 0; the polynomial stays finite
+        float e0, e1;
+        const f32x2 a = at_most_pair(magnitude_pair(z), 16.f);  // e^-128 = 0; the polynomial stays finite
         pair_split(pair_mul(pair_mul(a, a), both(-0.5f * kLog2e)), e0, e1);
         f32x2 r = pair_fma(a, both(3.7967514795e-05f), both(-6.1627244577e-04f));
         r = pair_fma(a, r, both(4.4045890681e-03f));
@@ -128,17 +152,15 @@ __device__ __forceinline__ f32x2 slope_pair(f32x2 z) {
         r = pair_fma(a, r, both(4.9999898672e-01f));
         return reflect_pair(z, pair_mul(r, pair_of(exp2_approx(e0), exp2_approx(e1))));
     } else if constexpr (kAct == kActGeluTanh) {
-        float z0, z1;
-        pair_split(z, z0, z1);
-        // the slope is 0 or 1 beyond 16 in magnitude; held there, z^2 times nothing stays nothing
-        const f32x2 t = pair_of(fminf(fmaxf(z0, -16.f), 16.f), fminf(fmaxf(z1, -16.f), 16.f)), t2 = pair_mul(t, t);
+        // the slope is 1 beyond 16; held there, z^2 times nothing stays nothing
+        const f32x2 t = at_most_pair(at_least_pair(z, -7.4f), 16.f), t2 = pair_mul(t, t);
         const f32x2 u = pair_fma(both(-kLog2e * kTwoRoot2OverPi * 0.044715f), t2, both(-kLog2e * kTwoRoot2OverPi));
         const f32x2 s = logistic_pair(pair_mul(t, u));
         const f32x2 bend = pair_mul(t, pair_fma(pair_mul(s, both(-1.f)), s, s));
         return pair_fma(bend, pair_fma(both(3.0f * kTwoRoot2OverPi * 0.044715f), t2, both(kTwoRoot2OverPi)), s);
     } else if constexpr (kAct == kActSilu) {
-        const f32x2 s = logistic_pair(pair_mul(z, both(-kLog2e)));
-        return pair_mul(s, pair_fma(z, pair_fma(s, both(-1.f), both(1.f)), both(1.f)));
+        const f32x2 t = at_least_pair(z, -41.f), s = logistic_pair(pair_mul(t, both(-kLog2e)));
+        return pair_mul(s, pair_fma(t, pair_fma(s, both(-1.f), both(1.f)), both(1.f)));
     }
     return both(1.f);
 }

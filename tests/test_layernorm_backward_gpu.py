@@ -137,6 +137,16 @@ def test_constant_rows_and_a_single_column(cuda, ko):
         assert not dx.any() and not dgamma.any()
 
 
+def test_no_eps(cuda, ko):
+    """eps = 0, with every number of rows left over by the blocks."""
+    for cols in (24, 64, 100, 200, 512, 1001):
+        for rows in (1, 3, 31, 33):
+            a = _inputs(cuda, cuda.float32, rows, cols, seed=rows)
+            got = ko.layernorm_backward(a["dy"], a["x"], 0.0, a["gamma"])
+            want, scale = _reference(cuda, a["dy"], a["x"], 0.0, a["gamma"])
+            _check(cuda, got, want, scale, cuda.float32)
+
+
 def test_a_bad_row_stays_in_its_row(cuda, ko):
     for cols in (256, 1001, 20480):
         a = _inputs(cuda, cuda.float16, 40, cols)

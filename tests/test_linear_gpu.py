@@ -296,6 +296,31 @@ def test_bias_gradient_of_a_large_batch(cuda, ko):
     assert cuda.equal(dw, again[0]) and cuda.equal(db, again[1])
 
 
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+@pytest.mark.parametrize("act", ACTS)
+def test_activations_of_huge_and_bad_values(cuda, ko, out, act):
+    """Far out every activation is its argument or nothing, and its slope 1 or 0; a NaN stays a NaN and its neighbours are spared."""
+    big = cuda.tensor([1e3, 1e10, 3e18, 1e30], device="cuda")
+    row = cuda.cat([big, -big, cuda.tensor([float("nan"), 1.0, -1.0, float("nan"), 2.0, -60.0, 60.0, float("nan")], device="cuda")]).bfloat16()
+    ok = ~row.isnan()
+    eye = cuda.eye(16, device="cuda").bfloat16()
+    for m in (4, 64, 4096):
+        z = row.repeat(m, 1)
+        clean = cuda.where(ok, z, cuda.zeros_like(z))
+        bias = cuda.where(ok, cuda.zeros_like(row), row)                 # the NaNs arrive with the bias: a product would spread them
+        y = ko.linear(clean, eye, bias, act, out_dtype=_dtype(cuda, out)).double()
+        dx = ko.linear_backward_input(cuda.ones_like(z), eye, None if act == "none" else z, act, out_dtype=_dtype(cuda, out)).double()
+        assert (y.isnan() == ~ok).all() and (act in ("none", "relu") or (dx.isnan() == ~ok).all())
+        tame = z.double().clamp(-1e3, 1e3)                               # the formulas overflow beyond
+        want, slope = _act(cuda, tame, act), _slope(cuda, tame, act)
+        want = cuda.where((z.double().abs() > 1e3) & (z.double() > 0), z.double(), want)
+        if act == "none":
+            want = z.double()
+        step = cuda.finfo(_dtype(cuda, out)).eps
+        assert ((y - want).abs()[:, ok] <= (step * want.abs() + 2e-6 * 61)[:, ok]).all()
+        assert ((dx - slope).abs()[:, ok] <= (step * slope.abs() + 2e-6 * 61)[:, ok]).all()
+
+
 def _np16(cuda, t):
     return t.contiguous().view(cuda.int16).cpu().numpy()
 
