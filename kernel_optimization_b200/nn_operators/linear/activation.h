@@ -85,6 +85,13 @@ __device__ __forceinline__ f32x2 at_most_pair(f32x2 z, float limit) {
     return pair_of(min_nan(a, limit), min_nan(b, limit));
 }
 
+// |z|, at most `limit`
+__device__ __forceinline__ f32x2 magnitude_pair(f32x2 z, float limit) {
+    float a, b;
+    pair_split(z, a, b);
+    return pair_of(min_nan(fabsf(a), limit), min_nan(fabsf(b), limit));
+}
+
 // 1 / (1 + 2^x), x = -v log2(e) for the logistic function of v, x <= 62.  (fminf takes the 62 for a NaN, which would reach the
 // other value through the common reciprocal; the callers multiply by what is still a NaN.)
 __device__ __forceinline__ f32x2 logistic_pair(f32x2 x) {
@@ -94,7 +101,6 @@ __device__ __forceinline__ f32x2 logistic_pair(f32x2 x) {
     pair_split(d, u, v);
     return pair_mul(pair_of(v, u), both(rcp_approx(u * v)));
 }
-__device__ __forceinline__ f32x2 magnitude_pair(f32x2 z) { return z & 0x7fffffff7fffffffull; }
 // f(-|z|) where z is negative, else 1 - f(-|z|)
 __device__ __forceinline__ f32x2 reflect_pair(f32x2 z, f32x2 low) {
     float z0, z1, a, b;
@@ -110,7 +116,8 @@ __device__ __forceinline__ f32x2 activate_pair(f32x2 z) {
         pair_split(z, a, b);
         return pair_of(a < 0.f ? 0.f : a, b < 0.f ? 0.f : b);
     } else if constexpr (kAct == kActGelu) {
-        const f32x2 a = magnitude_pair(z);
+        // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
+        const f32x2 a = magnitude_pair(z, 32.f);
         f32x2 p = pair_fma(a, both(-1.7937167058e-06f), both(6.0908834712e-05f));
         p = pair_fma(a, p, both(-9.2606159160e-04f));
         p = pair_fma(a, p, both(8.4938677028e-03f));
@@ -118,9 +125,10 @@ __device__ __forceinline__ f32x2 activate_pair(f32x2 z) {
         p = pair_fma(a, p, both(-4.5848044753e-01f));
         p = pair_fma(a, p, both(-1.1512467861e+00f));
         p = pair_fma(a, p, both(-9.9999547005e-01f));
-        float p0, p1;
+        float p0, p1, z0, z1;
         pair_split(p, p0, p1);
-        return pair_mul(z, reflect_pair(z, pair_of(exp2_approx(p0), exp2_approx(p1))));
+        pair_split(z, z0, z1);
+        return pair_fma(a, pair_of(-exp2_approx(p0), -exp2_approx(p1)), pair_of(fmaxf(z0, 0.f), fmaxf(z1, 0.f)));
     } else if constexpr (kAct == kActGeluTanh) {
         const f32x2 t = at_least_pair(z, -7.4f);
         const f32x2 u = pair_fma(both(-kLog2e * kTwoRoot2OverPi * 0.044715f), pair_mul(t, t), both(-kLog2e * kTwoRoot2OverPi));
@@ -140,7 +148,7 @@ __device__ __forceinline__ f32x2 slope_pair(f32x2 z) {
         return pair_of(a > 0.f ? 1.f : 0.f, b > 0.f ? 1.f : 0.f);
     } else if constexpr (kAct == kActGelu) {
         float e0, e1;
-        const f32x2 a = at_most_pair(magnitude_pair(z), 16.f);  // e^-128 = 0; the polynomial stays finite
+        const f32x2 a = magnitude_pair(z, 16.f);  // e^-128 = 0; the polynomial stays finite
         pair_split(pair_mul(pair_mul(a, a), both(-0.5f * kLog2e)), e0, e1);
         f32x2 r = pair_fma(a, both(3.7967514795e-05f), both(-6.1627244577e-04f));
         r = pair_fma(a, r, both(4.4045890681e-03f));
