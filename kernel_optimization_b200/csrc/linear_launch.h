@@ -25,11 +25,12 @@ struct ProductPlan {
 
 // tma: D can be stored by TMA; without it only the 128 x 128 tile is built.  element_bytes: what the epilogue moves per element
 // of D (D itself, Z, the extra operand).  Modelled microseconds per candidate: start, then rounds of work units x (K-blocks
-// of 64 x time per K-block + epilogue time that the next tile does not hide); slices add a second kernel and the partial
-// tiles' way through the L2 (written once, read once) at 5 TB/s.  Fitted to forced plans, BF16, measured (modelled):
+// of 64 x time per K-block + epilogue time that the next tile does not hide); slices add a second kernel (2 us of the
+// device, 4 of the host with the workspace; 5 is what they have to gain) and the partial tiles' way through the L2 (written once,
+// read once) at 5 TB/s.  Fitted to forced plans, BF16, measured (modelled):
 // 16384 x 4096 x 1024 pair 103 (103), 128 x 256 110 (112), 128 x 128 164 (165); 4096^3 93 (97), 102 (103), 142 (139);
 // 8192 x 768 x 768 16.6 (15.9), 17.4 (16.3), 18.2 (17.1); 2048 x 1024 x 1024 13.6 (11.6), 14.0 (11.8), 11.1 (8.8); 4096 x 4096 x 64
-// to FP32 19.0 (17.7), 15.5 (17.3), 14.0 (17.3); 768 x 768 x 8192 in four slices of 128-wide tiles 20.2 (19.9).
+// to FP32 19.0 (17.7), 15.5 (17.3), 14.0 (17.3); 768 x 768 x 8192 in four slices of 128-wide tiles 20.2 (22.7 with the 5).
 inline ProductPlan plan_product(int64_t M, int64_t N, int64_t K, bool tma, int element_bytes, int sms) {
     const long long k_blocks = (K + tc::kBK - 1) / tc::kBK;
     ProductPlan best{false, 128, 1, 0};
@@ -51,7 +52,7 @@ inline ProductPlan plan_product(int64_t M, int64_t N, int64_t K, bool tma, int e
             double cost = start + (double)rounds * ((double)((k_blocks + split - 1) / split) * per_block + per_tile(split > 1 ? 4 : element_bytes));
             if (split > 1) {
                 const double written = (double)((M + 31) / 32 * 32) * (double)N * split, read = (double)M * (double)N * split;
-                cost += 2.2 + ((written + read) * 4.0 + (double)M * (double)N * element_bytes) / 5e6;
+                cost += 5.0 + ((written + read) * 4.0 + (double)M * (double)N * element_bytes) / 5e6;
             }
             if (cost < best_cost) {
                 best_cost = cost;

@@ -6,7 +6,6 @@ a page-locked host buffer plus a device buffer with copies in both directions.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import functools
 
@@ -168,18 +167,16 @@ def _operand(t, name: str, device, dtypes, shape) -> int | None:
     raise ValueError(f"{name} must be contiguous")
 
 
-_HERE = contextlib.nullcontext()
-
-
-def _on(device, stream: int | None):
-    """Context in which `device` and the stream with handle `stream` (None: the device's current one) are current, so that
-    outputs and workspaces come from the pool of the stream that uses them."""
+def _elsewhere(device, stream: int | None):
+    """None when `device` is the current one and `stream` is not given; else a context in which `device` and the stream with
+    handle `stream` (None: the device's current one) are current, so that outputs and workspaces come from the pool of the
+    stream that uses them."""
     import torch
 
     if device.type != "cuda":
         raise ValueError("operator inputs must live on a CUDA device (there is no CPU path)")
     if stream is None:
-        return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+        return None if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
     if stream == 0:
         return torch.cuda.stream(torch.cuda.default_stream(device))
     return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device))
@@ -221,16 +218,27 @@ def layernorm_backward(dy, x, eps: float, gamma=None, ddof: int = 0, residual=No
     lib = native.lib()
     code, fn = {torch.float32: (DTYPE_F32, lib.ko_layernorm_backward_f32), torch.float16: (DTYPE_F16, lib.ko_layernorm_backward_f16),
                 torch.bfloat16: (DTYPE_BF16, lib.ko_layernorm_backward_bf16)}[x.dtype]
-    with _on(device, stream):
-        dx = torch.empty(rows, cols, dtype=x.dtype, device=device) if dx is None else dx
-        dgamma = torch.empty(cols, dtype=torch.float32, device=device) if dgamma is None else dgamma
-        dbeta = torch.empty(cols, dtype=torch.float32, device=device) if dbeta is None else dbeta
-        ws, ws_at, ws_bytes = _workspace(_layernorm_backward_bytes(device.index, code, rows, cols), device)
-        native.check(fn(_operand(dy, "dy", device, same, (rows, cols)), _ptr(x), _operand(dx, "dx", device, same, (rows, cols)), rows,
-                        cols, eps, _operand(gamma, "gamma", device, same, (cols,)),
-                        _operand(residual, "residual", device, same, (rows, cols)),
-                        _operand(dgamma, "dgamma", device, vector, (cols,)), _operand(dbeta, "dbeta", device, vector, (cols,)), ddof,
-                        ws_at, ws_bytes, _current_stream_ptr(device.index)), "ko_layernorm_backward")
+    place = _elsewhere(device, stream)
+    if place is not None:
+        with place:
+            return layernorm_backward(dy, x, eps, gamma, ddof, residual, dx, dgamma, dbeta)
+    matrix, row = (rows, cols), (cols,)
+    x_at, dy_at = _ptr(x), _operand(dy, "dy", device, same, matrix)
+    gamma_at, residual_at = _operand(gamma, "gamma", device, same, row), _operand(residual, "residual", device, same, matrix)
+    dx_at, dgamma_at, dbeta_at = (_operand(dx, "dx", device, same, matrix), _operand(dgamma, "dgamma", device, vector, row),
+                                  _operand(dbeta, "dbeta", device, vector, row))
+    if dx is None:
+        dx = torch.empty(rows, cols, dtype=x.dtype, device=device)
+        dx_at = dx.data_ptr()
+    if dgamma is None:
+        dgamma = torch.empty(cols, dtype=torch.float32, device=device)
+        dgamma_at = dgamma.data_ptr()
+    if dbeta is None:
+        dbeta = torch.empty(cols, dtype=torch.float32, device=device)
+        dbeta_at = dbeta.data_ptr()
+    ws, ws_at, ws_bytes = _workspace(_layernorm_backward_bytes(device.index, code, rows, cols), device)
+    native.check(fn(dy_at, x_at, dx_at, rows, cols, eps, gamma_at, residual_at, dgamma_at, dbeta_at, ddof, ws_at, ws_bytes,
+                    _current_stream_ptr(device.index)), "ko_layernorm_backward")
     return dx, dgamma, dbeta
 
 
@@ -305,14 +313,17 @@ def _linear_types(a, out, out_dtype, default):
     """(in_fmt, out_fmt, out_dtype) of a product whose inputs have `a`'s type."""
     import torch
 
-    if a.dim() != 2 or a.dtype not in (torch.float16, torch.bfloat16):
-        raise ValueError(f"the inputs must be 2-D FP16 or BF16 tensors, got {a.dtype} with {a.dim()} dimensions")
+    dtype = a.dtype
+    if a.dim() != 2 or (dtype is not torch.bfloat16 and dtype is not torch.float16):
+        raise ValueError(f"the inputs must be 2-D FP16 or BF16 tensors, got {dtype} with {a.dim()} dimensions")
     if out_dtype is None:
         out_dtype = default if out is None else out.dtype
-    if out_dtype not in (torch.float32, a.dtype):
-        raise ValueError(f"the output is FP32 or the inputs' {a.dtype}, not {out_dtype}")
-    in_fmt = 0 if a.dtype == torch.float16 else 1
-    return in_fmt, 0 if out_dtype == torch.float32 else in_fmt + 1, out_dtype
+    in_fmt = 0 if dtype is torch.float16 else 1
+    if out_dtype is dtype:
+        return in_fmt, in_fmt + 1, out_dtype
+    if out_dtype is not torch.float32:
+        raise ValueError(f"the output is FP32 or the inputs' {dtype}, not {out_dtype}")
+    return in_fmt, 0, out_dtype
 
 
 @functools.lru_cache(maxsize=4096)
@@ -339,15 +350,23 @@ def linear(x, w, bias=None, activation: str = "none", residual=None, out=None, o
     if w.dim() != 2:
         raise ValueError(f"w must have 2 dimensions, got {w.dim()}")
     (m, k), n = x.shape, w.shape[0]
-    with _on(device, stream):
-        out = torch.empty(m, n, dtype=out_dtype, device=device) if out is None else out
-        if return_pre and pre is None:
-            pre = torch.empty(m, n, dtype=x.dtype, device=device)
-        ws, ws_at, ws_bytes = _workspace(_linear_bytes(device.index, "ko_linear_workspace", m, n, k), device)
-        native.check(native.lib().ko_linear(in_fmt, out_fmt, act, m, n, k, _ptr(x), _operand(w, "w", device, same, (n, k)),
-                                            _operand(bias, "bias", device, same, (n,)), _operand(residual, "residual", device, to, (m, n)),
-                                            _operand(out, "out", device, to, (m, n)), _operand(pre, "pre", device, same, (m, n)),
-                                            ws_at, ws_bytes, _current_stream_ptr(device.index)), "ko_linear")
+    place = _elsewhere(device, stream)
+    if place is not None:
+        with place:
+            return linear(x, w, bias, activation, residual, out, out_dtype, return_pre, pre)
+    matrix = (m, n)
+    x_at, w_at, bias_at = _ptr(x), _operand(w, "w", device, same, (n, k)), _operand(bias, "bias", device, same, (n,))
+    residual_at, out_at, pre_at = (_operand(residual, "residual", device, to, matrix), _operand(out, "out", device, to, matrix),
+                                   _operand(pre, "pre", device, same, matrix))
+    if out is None:
+        out = torch.empty(m, n, dtype=out_dtype, device=device)
+        out_at = out.data_ptr()
+    if return_pre and pre is None:
+        pre = torch.empty(m, n, dtype=x.dtype, device=device)
+        pre_at = pre.data_ptr()
+    ws, ws_at, ws_bytes = _workspace(_linear_bytes(device.index, "ko_linear_workspace", m, n, k), device)
+    native.check(native.lib().ko_linear(in_fmt, out_fmt, act, m, n, k, x_at, w_at, bias_at, residual_at, out_at, pre_at, ws_at, ws_bytes,
+                                        _current_stream_ptr(device.index)), "ko_linear")
     return out if pre is None else (out, pre)
 
 
@@ -366,12 +385,18 @@ def linear_backward_input(dy, w, pre=None, activation: str = "none", out=None, o
     if w.dim() != 2:
         raise ValueError(f"w must have 2 dimensions, got {w.dim()}")
     (m, n), k = dy.shape, w.shape[1]
-    with _on(device, stream):
-        out = torch.empty(m, k, dtype=out_dtype, device=device) if out is None else out
-        ws, ws_at, ws_bytes = _workspace(_linear_bytes(device.index, "ko_linear_backward_input_workspace", m, n, k), device)
-        native.check(native.lib().ko_linear_backward_input(
-            in_fmt, out_fmt, act, m, n, k, _ptr(dy), _operand(w, "w", device, same, (n, k)), _operand(pre, "pre", device, same, (m, k)),
-            _operand(out, "out", device, (out_dtype,), (m, k)), ws_at, ws_bytes, _current_stream_ptr(device.index)), "ko_linear_backward_input")
+    place = _elsewhere(device, stream)
+    if place is not None:
+        with place:
+            return linear_backward_input(dy, w, pre, activation, out, out_dtype)
+    dy_at, w_at, pre_at = _ptr(dy), _operand(w, "w", device, same, (n, k)), _operand(pre, "pre", device, same, (m, k))
+    out_at = _operand(out, "out", device, (out_dtype,), (m, k))
+    if out is None:
+        out = torch.empty(m, k, dtype=out_dtype, device=device)
+        out_at = out.data_ptr()
+    ws, ws_at, ws_bytes = _workspace(_linear_bytes(device.index, "ko_linear_backward_input_workspace", m, n, k), device)
+    native.check(native.lib().ko_linear_backward_input(in_fmt, out_fmt, act, m, n, k, dy_at, w_at, pre_at, out_at, ws_at, ws_bytes,
+                                                       _current_stream_ptr(device.index)), "ko_linear_backward_input")
     return out
 
 
@@ -389,13 +414,19 @@ def linear_backward_weight(dy, x, c=None, out=None, out_dtype=None, return_bias:
     if x.dim() != 2:
         raise ValueError(f"x must have 2 dimensions, got {x.dim()}")
     (m, n), k = dy.shape, x.shape[1]
-    with _on(device, stream):
-        out = torch.empty(n, k, dtype=out_dtype, device=device) if out is None else out
-        if return_bias and dbias is None:
-            dbias = torch.empty(n, dtype=torch.float32, device=device)
-        ws, ws_at, ws_bytes = _workspace(_linear_bytes(device.index, "ko_linear_backward_weight_workspace", m, n, k), device)
-        native.check(native.lib().ko_linear_backward_weight(
-            in_fmt, out_fmt, m, n, k, _ptr(dy), _operand(x, "x", device, (dy.dtype,), (m, k)), _operand(c, "c", device, to, (n, k)),
-            _operand(out, "out", device, to, (n, k)), _operand(dbias, "dbias", device, (torch.float32,), (n,)),
-            ws_at, ws_bytes, _current_stream_ptr(device.index)), "ko_linear_backward_weight")
+    place = _elsewhere(device, stream)
+    if place is not None:
+        with place:
+            return linear_backward_weight(dy, x, c, out, out_dtype, return_bias, dbias)
+    dy_at, x_at, c_at = _ptr(dy), _operand(x, "x", device, (dy.dtype,), (m, k)), _operand(c, "c", device, to, (n, k))
+    out_at, dbias_at = _operand(out, "out", device, to, (n, k)), _operand(dbias, "dbias", device, (torch.float32,), (n,))
+    if out is None:
+        out = torch.empty(n, k, dtype=out_dtype, device=device)
+        out_at = out.data_ptr()
+    if return_bias and dbias is None:
+        dbias = torch.empty(n, dtype=torch.float32, device=device)
+        dbias_at = dbias.data_ptr()
+    ws, ws_at, ws_bytes = _workspace(_linear_bytes(device.index, "ko_linear_backward_weight_workspace", m, n, k), device)
+    native.check(native.lib().ko_linear_backward_weight(in_fmt, out_fmt, m, n, k, dy_at, x_at, c_at, out_at, dbias_at, ws_at, ws_bytes,
+                                                        _current_stream_ptr(device.index)), "ko_linear_backward_weight")
     return out if dbias is None else (out, dbias)

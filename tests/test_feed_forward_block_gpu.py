@@ -91,6 +91,37 @@ def test_captured_training_step(cuda, lib, ko):
     assert lib.ko_poll_device_status() == 0
 
 
+def test_first_calls_of_a_process_inside_a_capture():
+    """Nothing has to be called once before: the first use of every kernel may be the captured one."""
+    import os
+    import subprocess
+    import sys
+
+    code = '''
+import torch, kernel_optimization_b200 as ko
+from test_feed_forward_block_gpu import _block, _block_backward, _parameters
+p = _parameters(torch, torch.bfloat16, 512, 2048, 3)
+x, dy = (torch.randn(1000, 512, device="cuda").bfloat16() for _ in range(2))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y, saved = _block(ko, p, x)
+    grads = _block_backward(ko, p, dy, saved)
+    token = _block(ko, p, x[:1])[0]
+graph.replay()
+want, saved = _block(ko, p, x)
+again = _block_backward(ko, p, dy, saved)
+torch.cuda.synchronize()
+assert torch.equal(y, want) and all(torch.equal(grads[n], again[n]) for n in grads) and torch.equal(token, _block(ko, p, x[:1])[0])
+assert ko.lib().ko_poll_device_status() == 0
+print("captured")
+'''
+    here = os.path.dirname(os.path.abspath(__file__))
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([os.path.dirname(here), here, os.environ.get("PYTHONPATH", "")]))
+    out = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "captured" in out.stdout, out.stderr[-2000:]
+
+
 def test_tokens_one_by_one(cuda, ko):
     """Serving: each token alone gives what it gives in a batch, to the rounding of the steps' results."""
     p = _parameters(cuda, cuda.float16, 768, 2048, 4)
