@@ -4,23 +4,6 @@
 
 namespace {
 
-// beside: right behind the product's launch, which keeps the order with earlier work (see column_sum_kernel); else in its turn
-template <bool kBf16>
-int column_sums(bool beside, const void *in, int64_t rows, int cols, float *out, cudaStream_t s) {
-    const unsigned strips = (unsigned)((cols + 63) / 64);
-    const uint16_t *dy = static_cast<const uint16_t *>(in);
-    unsigned cluster = 1;
-    while (cluster < 8 && rows > 256LL * cluster) cluster *= 2;  // about 256 rows a block, one round of its loads
-    if (beside)
-        return ko::launch_clustered_overlapped(ko::column_sum_kernel<kBf16, 8>, strips * cluster, 256u, cluster, (size_t)0, s, dy, (long long)rows, cols,
-                                               out);
-    // With the device to itself: 16384 rows of 4096 / 2048 columns take 24 / 15 us in blocks of 8 warps and 33 / 31 in blocks of 32,
-    // which pay while there are few of them (32768 x 512 beside a product: 18 against 13 us).
-    if (strips * cluster >= 128 || rows <= 2048)
-        return ko::launch_clustered(ko::column_sum_kernel<kBf16, 8>, strips * cluster, 256u, cluster, s, dy, (long long)rows, cols, out);
-    return ko::launch_clustered(ko::column_sum_kernel<kBf16, 32>, strips * cluster, 1024u, cluster, s, dy, (long long)rows, cols, out);
-}
-
 int dispatch(int in_fmt, int out_fmt, int64_t M, int64_t N, int64_t K, const void *dY, const void *X, const void *C,
                               void *dW, float *dbias, void *workspace, size_t workspace_bytes, void *stream, const ko::PinnedPlan &pin) {
     const char *name = "linear backward weight";
@@ -48,20 +31,18 @@ int dispatch(int in_fmt, int out_fmt, int64_t M, int64_t N, int64_t K, const voi
     p.M = (int)N; p.N = (int)K; p.K = (int)M;  // the product's shape
     p.D = dW; p.fmt = in_fmt; p.out_fmt = out_fmt; p.b_row_major = 1;
     p.extra = C;
-    // The column sums go beside the product, unless dY is large: then their reads throw out of the L2 what the product would
-    // read again, and it is quicker to let them go first.  Measured with / without dbias (us): 16384 x 1024 x 4096 102 / 100,
-    // 16384 x 768 x 768 29.3 / 27.6, 777 x 1000 x 520 10.5 / 10.0; 16384 x 4096 x 1024 126 beside, 121 ahead / 101.
-    // Ahead as well where the product promotes its sums, which takes all of an SM's registers.
-    const bool large = (size_t)M * (size_t)N * 2 > ((size_t)48 << 20);
-    const auto sums = [&](bool now, bool as_beside) -> int {
-        if (dbias == nullptr || !now) return KO_OK;
-        return in_fmt ? column_sums<true>(as_beside, dY, M, (int)N, dbias, s) : column_sums<false>(as_beside, dY, M, (int)N, dbias, s);
-    };
-    if (K == 0) return sums(true, false);
-    const auto first = [&](bool promoted) { return sums(large || promoted, false); };
-    const auto beside = [&](bool promoted) { return sums(!large && !promoted, true); };
-    return out_fmt ? ko::run_product<ko::LinearMode::kWeightGrad, true>(p, dY, X, workspace, workspace_bytes, s, info, name, pin, first, beside)
-                   : ko::run_product<ko::LinearMode::kWeightGrad, false>(p, dY, X, workspace, workspace_bytes, s, info, name, pin, first, beside);
+    p.dbias = dbias;
+    if (K == 0) {  // no dW, only the column sums
+        if (dbias == nullptr) return KO_OK;
+        const uint16_t *dy = static_cast<const uint16_t *>(dY);
+        const unsigned blocks = (unsigned)((N + 63) / 64);
+        if (in_fmt) ko::column_sum_kernel<true><<<blocks, 256, 0, s>>>(dy, (long long)M, (int)N, dbias);
+        else ko::column_sum_kernel<false><<<blocks, 256, 0, s>>>(dy, (long long)M, (int)N, dbias);
+        KO_CUDA(cudaGetLastError());
+        return KO_OK;
+    }
+    return out_fmt ? ko::run_product<ko::LinearMode::kWeightGrad, true>(p, dY, X, workspace, workspace_bytes, s, info, name, pin)
+                   : ko::run_product<ko::LinearMode::kWeightGrad, false>(p, dY, X, workspace, workspace_bytes, s, info, name, pin);
 }
 
 }  // namespace
@@ -75,7 +56,7 @@ int ko_linear_backward_weight_workspace(int64_t M, int64_t N, int64_t K, size_t 
     if (M == 0 || N == 0) return KO_OK;
     ko::DeviceInfo info;
     if (int st = ko::current_device_info(&info)) return st;
-    *bytes = ko::product_workspace(N, K, M, info.sm_count);
+    *bytes = ko::product_workspace(N, K, M, info.sm_count, true);
     return KO_OK;
 }
 

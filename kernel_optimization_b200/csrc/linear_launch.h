@@ -83,12 +83,26 @@ inline int pin_product(const PinnedPlan &pin, int64_t M, int64_t N, int64_t K, b
     return KO_OK;
 }
 
-// room for whatever plan a call of this shape may take: with or without TMA, any operands
-inline size_t product_workspace(int64_t M, int64_t N, int64_t K, int sms) {
+// Tiles of a row of tiles that share the column sums of dY (see ColumnSums): one, whose sums are dbias, or four, whose parts
+// have to be added.  One that takes all K-blocks is 35 ns a K-block behind the others (16384 x 4096 x 1024: 111 us, four 104, without
+// the sums 102); adding parts is a launch, 1.3 us of the device (777 x 1000 x 520: one 9.5 us, four 10.8), where K is not cut anyway.
+inline int sum_shares(const ProductPlan &plan, int64_t N, int64_t K) {
+    const long long tiles_n = (N + plan.bn - 1) / plan.bn, unit_blocks = ((K + tc::kBK - 1) / tc::kBK + plan.split - 1) / plan.split;
+    return unit_blocks < 64 ? 1 : (int)std::min<long long>(tiles_n, 4);
+}
+inline size_t sum_bytes(const ProductPlan &plan, int64_t M, int64_t N, int64_t K) {
+    return (size_t)sum_shares(plan, N, K) * plan.split * (size_t)M * sizeof(float);
+}
+
+// room for whatever plan a call of this shape may take: with or without TMA, any operands, column sums
+inline size_t product_workspace(int64_t M, int64_t N, int64_t K, int sms, bool sums = false) {
     if (M == 0 || N == 0 || K == 0) return 0;
     size_t most = 0;
     for (int element_bytes = 2; element_bytes <= 10; element_bytes += 2)
-        most = std::max({most, plan_product(M, N, K, true, element_bytes, sms).bytes(), plan_product(M, N, K, false, element_bytes, sms).bytes()});
+        for (bool tma : {true, false}) {
+            const ProductPlan plan = plan_product(M, N, K, tma, element_bytes, sms);
+            most = std::max(most, plan.bytes() + (sums ? sum_bytes(plan, M, N, K) : 0));
+        }
     return most;
 }
 
@@ -115,7 +129,8 @@ int launch_product_tile(const CUtensorMap &ma, const CUtensorMap &mb, const CUte
     auto kernel = tc::gemm_tcgen05_kernel<BN, kTmaStore, 1, 2, Epi>;
     if (int st = ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), Cfg::kSmemBytes)) return st;
     const long long units = (long long)((p.M + 127) / 128) * ((p.N + BN - 1) / BN) * p.split_k;
-    return launch_overlapped(kernel, (unsigned)std::min<long long>(units, sms), 64u + 32u * Epi::kWarps, (size_t)Cfg::kSmemBytes, s, ma, mb, mb, md, p);
+    return launch_overlapped(kernel, (unsigned)std::min<long long>(units, sms), 64u + 32u * (Epi::kWarps + Epi::kSumWarps), (size_t)Cfg::kSmemBytes, s, ma,
+                             mb, mb, md, p);
 }
 
 template <class Epi>
@@ -123,7 +138,7 @@ int launch_product_pair(const CUtensorMap &ma, const CUtensorMap &mb, const CUte
     using Cfg = typename tc::PairConfigFor<Epi>::type;
     auto kernel = tc::gemm_tcgen05_pair_kernel<true, Epi>;
     const void *id = reinterpret_cast<const void *>(kernel);
-    constexpr unsigned threads = 64u + 32u * Epi::kWarps;
+    constexpr unsigned threads = 64u + 32u * (Epi::kWarps + Epi::kSumWarps);
     if (int st = ensure_dynamic_smem(id, Cfg::kSmemBytes)) return st;
     int resident = 0;
     if (int st = resident_pairs_of(id, threads, Cfg::kSmemBytes, &resident)) return st;
@@ -134,8 +149,7 @@ int launch_product_pair(const CUtensorMap &ma, const CUtensorMap &mb, const CUte
 
 // Runs the product that `p` describes (M, N, K, D, fmt, out_fmt, b_row_major, bias, extra, pre, activation set by the
 // caller; the rest filled in here).  A: [M, K], or [K, M] for the weight gradient; B: [N, K], or [K, N] with b_row_major.
-// Everything has been checked but the workspace.  `first` launches what goes ahead of the product once nothing is left to
-// refuse, `beside` what may run beside it, between it and the sum of its slices (both are told whether sums are promoted).
+// Everything has been checked but the workspace.
 template <class Epi>
 int launch_product(const ProductPlan &plan, bool tma, const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &md, const LinearParams &p,
                    int sms, cudaStream_t s) {
@@ -145,12 +159,9 @@ int launch_product(const ProductPlan &plan, bool tma, const CUtensorMap &ma, con
     return launch_product_tile<Epi, 256, true>(ma, mb, md, p, sms, s);
 }
 
-struct Nothing {
-    int operator()(bool) const { return KO_OK; }
-};
-template <LinearMode kMode, bool kOut16, class First = Nothing, class Beside = Nothing>
+template <LinearMode kMode, bool kOut16>
 int run_product(LinearParams p, const void *A, const void *B, void *workspace, size_t workspace_bytes, cudaStream_t s, const DeviceInfo &info,
-                const char *name, const PinnedPlan &pin = {}, const First &first = {}, const Beside &beside = {}) {
+                const char *name, const PinnedPlan &pin = {}) {
     using Epi = LinearEpilogue<kMode, kOut16>;
     EncodeTiledFn encode = nullptr;
     if (int st = get_encode_fn(&encode)) return st;
@@ -160,13 +171,17 @@ int run_product(LinearParams p, const void *A, const void *B, void *workspace, s
     const int element_bytes = (kOut16 ? 2 : 4) + (p.pre ? 2 : 0) + (p.extra ? (Epi::kExtra16 ? 2 : 4) : 0);
     ProductPlan plan = plan_product(p.M, p.N, p.K, tma, element_bytes, info.sm_count);
     if (int st = pin_product(pin, p.M, p.N, p.K, tma, name, &plan)) return st;
-    KO_REQUIRE(plan.bytes() == 0 || (workspace != nullptr && workspace_bytes >= plan.bytes()), KO_ERR_INVALID_ARG,
-               "%s: the workspace needs %zu bytes, got %zu", name, plan.bytes(), workspace ? workspace_bytes : (size_t)0);
+    p.sum_shares = p.dbias ? sum_shares(plan, p.N, p.K) : 0;
+    const bool fold = p.sum_shares * plan.split > 1;
+    const size_t bytes = plan.bytes() + (fold ? sum_bytes(plan, p.M, p.N, p.K) : 0);
+    KO_REQUIRE(bytes == 0 || (workspace != nullptr && workspace_bytes >= bytes), KO_ERR_INVALID_ARG,
+               "%s: the workspace needs %zu bytes, got %zu", name, bytes, workspace ? workspace_bytes : (size_t)0);
     KO_REQUIRE(aligned16(workspace), KO_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", name);
     p.C = nullptr;
     p.tiles_n = p.wide_tiles_n = p.bn_wide = p.bn_narrow = 0;
     p.split_k = plan.split;
     p.partials = static_cast<float *>(workspace);
+    p.sum_parts = fold ? static_cast<float *>(workspace) + plan.bytes() / sizeof(float) : p.dbias;
     if (int st = device_status_word(0, &p.status)) return st;
 
     alignas(64) CUtensorMap map_a, map_b, map_d;
@@ -192,16 +207,17 @@ int run_product(LinearParams p, const void *A, const void *B, void *workspace, s
     // FP32 results of more than two periods of K a work unit: partial sums are promoted (see LinearEpilogue)
     const long long unit_blocks = ((p.K + tc::kBK - 1) / tc::kBK + plan.split - 1) / plan.split;
     const bool promote = !kOut16 && unit_blocks > 2 * tc::kPeriod;
-    int st = first(promote);
-    if (st != KO_OK) return st;
+    int st = KO_OK;
     if constexpr (!kOut16) {
         if (promote) st = launch_product<LinearEpilogue<kMode, false, true>>(plan, tma, map_a, map_b, map_d, p, info.sm_count, s);
         else st = launch_product<Epi>(plan, tma, map_a, map_b, map_d, p, info.sm_count, s);
     } else {
         st = launch_product<Epi>(plan, tma, map_a, map_b, map_d, p, info.sm_count, s);
     }
-    if (st == KO_OK) st = beside(promote);
-    if (st != KO_OK || plan.split <= 1) return st;
+    if (st != KO_OK) return st;
+    if constexpr (kMode == LinearMode::kWeightGrad)
+        if (fold && plan.split == 1) return launch_overlapped(linear_fold_sums_kernel<256>, (unsigned)((p.M + 255) / 256), 256u, (size_t)0, s, p);
+    if (plan.split <= 1) return KO_OK;
     const long long chunks = plan.tiles * 4 * (plan.bn / 32);
     return launch_overlapped(linear_slice_sum_kernel<kMode, kOut16>, (unsigned)chunks, 256u, (size_t)0, s, p, plan.bn);
 }

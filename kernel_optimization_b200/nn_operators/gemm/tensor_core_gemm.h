@@ -264,7 +264,7 @@ struct PlainEpilogue {
     static constexpr bool kTransA = false;
     static constexpr bool kFused = false;
     static constexpr bool kPromote = false; // true: partial sums of kPeriod K-blocks are added outside the tensor cores (see there)
-    static constexpr bool kShares = false;  // true: launch_dependents only after the wait for the previous kernel; registers and memory left over
+    static constexpr int kSumWarps = 0;  // warps that add up the columns of A as stored (kTransA), beside the product
 };
 
 template <class Epi, bool kFused = Epi::kFused>
@@ -495,7 +495,7 @@ __device__ __forceinline__ void publish_block(float *slot_chunks, uint32_t t_row
 // kTmaStore: D is written by TMA stores staged through shared memory (needs a 16-byte row pitch and base for D
 // and no C operand); otherwise every thread stores its row segment directly (and adds C when given)
 template <int BN, bool kTmaStore, int MT = 1, int kBoxes = 2, class Epi = PlainEpilogue>
-__global__ void __launch_bounds__(64 + 32 * Epi::kWarps, Epi::kShares ? 2 : 1)
+__global__ void __launch_bounds__(64 + 32 * (Epi::kWarps + Epi::kSumWarps), 1)
 gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                     const __grid_constant__ CUtensorMap map_b_narrow, const __grid_constant__ CUtensorMap map_d,
                     const __grid_constant__ typename Epi::Params p) {
@@ -539,7 +539,8 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     if (threadIdx.x == 0) {
         for (int s = 0; s < Cfg::kStages; ++s) {
             mbar_init(full_bar(s), 1);
-            mbar_init(empty_bar(s), 1);
+            if constexpr (Epi::kSumWarps != 0) mbar_init(empty_bar(s), p.sum_shares ? 1 + Epi::kSumWarps : 1);
+            else mbar_init(empty_bar(s), 1);
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(acc_ready_bar(a), 1);
@@ -556,7 +557,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         if (p.tiles_n) prefetch_tensormap(&map_b_narrow);
         if (kTmaStore) prefetch_tensormap(&map_d);
     }
-    if (!Epi::kShares) grid_launch_dependents();  // the stream's next kernel may set up while this one drains
+    grid_launch_dependents();  // the stream's next kernel may set up while this one drains
     if (warp == 1) tmem_alloc(smem_u32(tmem_slot), Cfg::kTmemCols);
     tc_fence_before();
     __syncthreads();
@@ -565,7 +566,6 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     // launched with programmatic stream serialization: barriers, tensor memory and descriptor prefetch above
     // overlap the previous kernel's tail; operands and D are touched only after its writes are visible
     grid_dependency_wait();
-    if (Epi::kShares) grid_launch_dependents();
 
     if (warp == 0) {
         // ------------------------------------------------------------------ TMA producer
@@ -681,6 +681,38 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             bool drained = false;
             for (uint32_t spin = 0; spin < kSpinLimit && !(drained = mbar_try_wait(drain_bar, 0)); ++spin) {}
             if (!drained) atomicCAS(p.status, kStatusOk, kTimeoutDrain);
+        }
+        __syncwarp();
+    } else if (Epi::kSumWarps != 0 && warp >= 2 + Epi::kWarps) {
+        // ------------------------------------------------------------------ column sums of A (behind the epilogue warps)
+        if constexpr (Epi::kSumWarps != 0) {
+            const int box = warp - 2 - Epi::kWarps;  // 64 of the CTA's 128 rows of the product
+            uint32_t stage = 0, phase = 0;
+            bool ok = true;
+            for (long long u = blockIdx.x; p.sum_shares && u < num_units && ok; u += gridDim.x) {
+                long long t;
+                int slice, kb0, kb1, tm, tn;
+                unit_of(u, t, slice, kb0, kb1);
+                tile_of(p, t, tiles_m, tiles_n, tm, tn);
+                const bool mine = tn < p.sum_shares;
+                typename Epi::Sums sums;
+                int next = kb0 + (tn - kb0 % p.sum_shares + p.sum_shares) % p.sum_shares;  // the next K-block that this tile adds
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    if (!mbar_wait(full_bar(stage), phase, abort_flag)) { ok = false; break; }
+                    if (mine && kb == next) {
+                        sums.add(p, ring + stage * (uint32_t)Cfg::kStageBytes + box * 8192u, lane);
+                        next += p.sum_shares;
+                        __syncwarp();
+                    }
+                    if (lane == 0) mbar_arrive(empty_bar(stage));
+                    if (++stage == (uint32_t)Cfg::kStages) { stage = 0; phase ^= 1u; }
+                }
+                if (ok && mine) sums.store(p, slice * p.sum_shares + tn, tm * kTileM + box * 64, lane);
+            }
+            if (!ok) {
+                if (lane == 0 && !*abort_flag) atomicCAS(p.status, kStatusOk, kTimeoutEpilogue);
+                *abort_flag = 1;
+            }
         }
         __syncwarp();
     } else {

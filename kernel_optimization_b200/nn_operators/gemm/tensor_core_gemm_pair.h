@@ -15,6 +15,7 @@
 //                the leader's barrier only -- a commit costs the MMA issue stream about 50 ns, a second one per stage
 //                measured 14 % -- and the leader's producer, once it has seen that release, passes it on to the
 //                peer's barrier with a relaxed remote arrive; each producer waits on its own barrier.
+//   arrived[s]   peer only, for the warps that add up columns of A: the leader's pass on what they saw on full[s].
 //   acc_ready[a] one per CTA, two plain commits (shared::cluster addresses) once a tile's MMAs are issued; each CTA's
 //                epilogue warps wait on their own.
 //   acc_free[a]  leader only, 8 arrivals: the four epilogue warps of both CTAs (the peer's arrive remotely).
@@ -118,7 +119,7 @@ __device__ __forceinline__ bool mbar_wait_remote(uint32_t bar, uint32_t parity, 
 
 // map_b / map_b_narrow: boxes of bn_wide / 2 and bn_narrow / 2 rows (128 rows when the tiles are uniform)
 template <bool kTmaStore, class Epi = PlainEpilogue>
-__global__ void __launch_bounds__(64 + 32 * Epi::kWarps, Epi::kShares ? 2 : 1)
+__global__ void __launch_bounds__(64 + 32 * (Epi::kWarps + Epi::kSumWarps), 1)
 gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                          const __grid_constant__ CUtensorMap map_b_narrow, const __grid_constant__ CUtensorMap map_d,
                          const __grid_constant__ typename Epi::Params p) {
@@ -139,6 +140,8 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * Cfg::kStages + 5);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     [[maybe_unused]] auto fused_bar = [&](int w) { return bar_base + 8u * (2 * Cfg::kStages + 7 + w); };  // behind the two words above
+    [[maybe_unused]] auto arrived_bar = [&](int s) { return bar_base + 8u * (2 * Cfg::kStages + 7 + Epi::kWarps + s); };
+    static_assert(Epi::kSumWarps == 0 || 8 * (3 * Cfg::kStages + 7 + Epi::kWarps) <= Cfg::kBarrierBytes, "room for the barriers");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_cta_rank();  // 0 = leader
@@ -152,7 +155,12 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     if (threadIdx.x == 0) {
         for (int s = 0; s < Cfg::kStages; ++s) {
             mbar_init(full_bar(s), 1);
-            mbar_init(empty_bar(s), 1);
+            if constexpr (Epi::kSumWarps != 0) {
+                mbar_init(empty_bar(s), p.sum_shares ? 1 + Epi::kSumWarps : 1);
+                mbar_init(arrived_bar(s), 1);
+            } else {
+                mbar_init(empty_bar(s), 1);
+            }
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(acc_ready_bar(a), 1);
@@ -169,7 +177,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         if (p.tiles_n) prefetch_tensormap(&map_b_narrow);
         if (kTmaStore) prefetch_tensormap(&map_d);
     }
-    if (!Epi::kShares) grid_launch_dependents();
+    grid_launch_dependents();
     if (warp == 1) tmem_alloc_pair(smem_u32(tmem_slot), Cfg::kTmemCols);
     tc_fence_before();
     __syncthreads();
@@ -177,7 +185,6 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     grid_dependency_wait();
-    if (Epi::kShares) grid_launch_dependents();
 
     if (warp == 0) {
         // ------------------------------------------------------------------ TMA producer (both CTAs)
@@ -286,6 +293,40 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
             bool drained = false;
             for (uint32_t spin = 0; spin < kSpinLimit && !(drained = mbar_try_wait(drain_bar, 0)); ++spin) {}
             if (!drained) atomicCAS(p.status, kStatusOk, kTimeoutDrain);
+        }
+        __syncwarp();
+    } else if (Epi::kSumWarps != 0 && warp >= 2 + Epi::kWarps) {
+        // ------------------------------------------------------------------ column sums of A (behind the epilogue warps, both CTAs)
+        if constexpr (Epi::kSumWarps != 0) {
+            const int box = warp - 2 - Epi::kWarps;  // 64 of the CTA's 128 rows of the product
+            uint32_t stage = 0, phase = 0;
+            bool ok = true;
+            for (long long t = pair; p.sum_shares && t < num_tiles && ok; t += pairs) {
+                int tm, tn;
+                tile_of(p, t, tiles_m, tiles_n, tm, tn);
+                const bool mine = tn < p.sum_shares;
+                typename Epi::Sums sums;
+                int next = tn;  // the next K-block that this tile adds
+                for (int kb = 0; kb < k_blocks; ++kb) {
+                    // The pair's loads complete on the leader's barrier; its first sum warp passes the word on.  A token (relaxed):
+                    // what the peer's sum warps read came into their own SM's shared memory before the leader's barrier heard of
+                    // it.  A releasing arrive took 0.7 us a K-block longer, which the whole ring then waited for.
+                    if (!mbar_wait_remote(leader ? full_bar(stage) : arrived_bar(stage), phase, abort_flag)) { ok = false; break; }
+                    if (leader && box == 0 && lane == 0) mbar_arrive_cluster_relaxed(map_to_cluster_rank(arrived_bar(stage), 1));
+                    if (mine && kb == next) {
+                        sums.add(p, ring + stage * (uint32_t)Cfg::kStageBytes + box * 8192u, lane);
+                        next += p.sum_shares;
+                        __syncwarp();
+                    }
+                    if (lane == 0) mbar_arrive(empty_bar(stage));
+                    if (++stage == (uint32_t)Cfg::kStages) { stage = 0; phase ^= 1u; }
+                }
+                if (ok && mine) sums.store(p, tn, tm * kTileM + (int)rank * kBM + box * 64, lane);
+            }
+            if (!ok) {
+                if (lane == 0 && !*abort_flag) atomicCAS(p.status, kStatusOk, kTimeoutEpilogue);
+                *abort_flag = 1;
+            }
         }
         __syncwarp();
     } else {

@@ -11,8 +11,6 @@
 // (Four for the weight gradient, which only stores.)
 #pragma once
 
-#include <cooperative_groups.h>
-
 #include "../gemm/tensor_core_gemm.h"
 #include "activation.h"
 
@@ -25,6 +23,10 @@ struct LinearParams : tc::GemmParams {
     const void *extra;  // forward: residual, weight grad: C (both of D's type); input grad: Z (the inputs' type); may be null
     void *pre;          // forward: Z out (the inputs' type); may be null
     int activation;
+    // weight grad, the column sums of dY (see ColumnSums): tiles of a row of tiles that share them (0: none are wanted), where
+    // their parts go, [split_k * sum_shares, M] (a single part: dbias itself), and where the parts' sum goes
+    int sum_shares;
+    float *sum_parts, *dbias;
     alignas(64) CUtensorMap map_pre, map_extra;
 };
 
@@ -79,6 +81,81 @@ __device__ __forceinline__ void linear_store_one(const LinearParams &p, float v,
     else static_cast<float *>(p.D)[at] = v;
 }
 
+// Column sums of dY, the bias gradient, by two warps beside the product: dY's tiles lie in shared memory for the matrix
+// instructions anyway, so the sums cost neither the L2 nor DRAM another reading of it.  (A kernel of their own beside or ahead
+// of the product cost 20 us in 147 at 16384 tokens of 4096 features, x 1024.)  All tiles of the same rows of dW see the same dY; the
+// first sum_shares of them take its K-blocks in turn, so that no CTA's shared memory serves much more than the others'.
+// A warp takes 64 columns, a lane eight of them in every fourth of a K-block's 64 rows; the rows of a K-block are added first,
+// then the K-blocks: chains of 16 and K / 64 FP32 additions.
+struct ColumnSums {
+    f32x2 sum[4] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f), pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
+
+    // box: shared-memory address of 64 rows x 64 columns, 128-byte rows with their 16-byte pieces swizzled by the row
+    template <bool kBf16>
+    __device__ __forceinline__ void add_box(uint32_t box, int lane) {
+        f32x2 part[4];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int row = 4 * i + (lane >> 3);
+            uint32_t w[4];
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                         : "r"(box + row * 128 + (((lane & 7) ^ (row & 7)) << 4))
+                         : "memory");
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float lo, hi;
+                widen16<kBf16>(w[j], lo, hi);
+                part[j] = i ? pair_add(part[j], pair_of(lo, hi)) : pair_of(lo, hi);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] = pair_add(sum[j], part[j]);
+    }
+    __device__ __forceinline__ void add(const LinearParams &p, uint32_t box, int lane) {
+        if (p.fmt) add_box<true>(box, lane);
+        else add_box<false>(box, lane);
+    }
+    // part: number of this part; row: first of the warp's 64 rows of the product
+    __device__ __forceinline__ void store(const LinearParams &p, int part, int row, int lane) const {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) pair_split(sum[j], v[2 * j], v[2 * j + 1]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            v[i] += __shfl_xor_sync(kFullMask, v[i], 16);
+            v[i] += __shfl_xor_sync(kFullMask, v[i], 8);
+        }
+        const int at = row + lane * 8;
+        if (lane >= 8 || at >= p.M) return;  // M is a multiple of 8
+        float *to = p.sum_parts + (size_t)part * p.M + at;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) to[i] = v[i];
+    }
+};
+
+// the parts of row `row`, added in their order
+__device__ __forceinline__ float fold_sum_parts(const LinearParams &p, int row) {
+    const int parts = p.sum_shares * p.split_k;
+    float total = 0.f;
+    for (int i0 = 0; i0 < parts; i0 += 8) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i0 + i < parts ? __ldcg(p.sum_parts + (size_t)(i0 + i) * p.M + row) : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) total += v[i];
+    }
+    return total;
+}
+// where no kernel adds slices of the product
+template <int kBlock = 256>
+__global__ void __launch_bounds__(kBlock) linear_fold_sums_kernel(const LinearParams p) {
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int row = blockIdx.x * kBlock + threadIdx.x;
+    if (row < p.M) p.dbias[row] = fold_sum_parts(p, row);
+}
+
 // kPromote (FP32 results of long sums): the tensor cores cut their accumulator off at every addition instead of rounding it, so an
 // error grows with K on the side of smaller magnitudes -- 1.9e-5 of the result (2-norm) for 16384 tokens, where a blocked FP32
 // sum is off by 1.5e-6.  A tile is then taken in periods of 2048 values of K, each into the other of the two
@@ -92,10 +169,8 @@ struct LinearEpilogue {
     static constexpr int kWarps = kTransA && !kPromote ? 4 : 8;
     static_assert(!kPromote || !kOut16, "what is rounded to 16 bits does not show it");
     static constexpr bool kFused = true;
-    // The weight gradient shares its SMs with the column sums of the bias gradient: it asks for dependents only once its own
-    // inputs are there (see column_sum_kernel), and leaves registers (at most 168 a thread, as for two blocks) and the little
-    // shared memory that the sums need.
-    static constexpr bool kShares = kTransA && !kPromote;
+    static constexpr int kSumWarps = kTransA ? 2 : 0;  // 64 columns of dY each, see ColumnSums
+    using Sums = ColumnSums;
     static constexpr bool kExtra16 = kMode == LinearMode::kInputGrad || kOut16;
     static constexpr int kChunk = kOut16 ? 64 : 32;           // columns
     static constexpr int kStep = kChunk * (kWarps / 4);        // from one chunk of a warp to its next
@@ -480,6 +555,10 @@ __global__ void __launch_bounds__(256) linear_slice_sum_kernel(const LinearParam
     const int col = tn * bn + (chunk % chunks_n) * 32 + ((int)threadIdx.x & 7) * 4;
     grid_launch_dependents();
     grid_dependency_wait();  // the slices are complete and visible
+    if constexpr (kMode == LinearMode::kWeightGrad) {  // the blocks of dW's first 32 columns fold the column sums of their rows
+        const int sum_row = tm * tc::kBM + (chunk / chunks_n) * 32 + (int)threadIdx.x;
+        if (p.sum_shares && tn == 0 && chunk % chunks_n == 0 && threadIdx.x < 32 && sum_row < p.M) p.dbias[sum_row] = fold_sum_parts(p, sum_row);
+    }
     if (row >= p.M || col >= p.N) return;
     const size_t slot_vecs = (size_t)tc::kBM * bn / 4;
     const float4 *src = reinterpret_cast<const float4 *>(p.partials) + (size_t)t * p.split_k * slot_vecs + ((size_t)chunk << 8) + threadIdx.x;
@@ -505,75 +584,37 @@ __global__ void __launch_bounds__(256) linear_slice_sum_kernel(const LinearParam
     }
 }
 
-// Column sums of a 16-bit [rows, cols] matrix, cols a multiple of 8: the bias gradient, beside the weight gradient's product.
-// A cluster of blocks shares 64 columns (a 128-byte line of each row, eight threads wide) and splits the rows; the blocks'
-// sums are added in rank order through distributed shared memory, so there is no workspace and no second kernel.  The
-// product keeps the SMs' ports to the L2 busy: with one block per 32 columns the sums of 16384 x 4096 crawled along for 229 us
-// beside a product of 100 us; many blocks with many lines in flight get through.
-//
-// Launched behind the product with programmatic serialization, it runs while the product does: the product's blocks ask
-// for their dependents only after their own grid_dependency_wait(), so everything enqueued before the product is complete
-// and visible when this kernel starts, and it reads and writes nothing the product writes.  It waits for the product before
-// it ends, so whatever follows it in the stream also follows the product.  (Loads past the L1, which may hold lines of an
-// earlier kernel.)
-template <bool kBf16, int kWarps>
-__global__ void __launch_bounds__(32 * kWarps, 32 / kWarps) column_sum_kernel(const uint16_t *in, long long rows, int cols, float *out) {
-    namespace cg = cooperative_groups;
-    cg::cluster_group cluster = cg::this_cluster();
-    const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    __shared__ float sums[64];  // little enough to fit beside a product's block
-    grid_launch_dependents();
+// Column sums of a 16-bit [rows, cols] matrix, cols a multiple of 8: the bias gradient of a layer without input features, whose
+// product has no tiles.  A block takes 64 columns, a lane eight of them; speed does not matter here.
+template <bool kBf16>
+__global__ void __launch_bounds__(256) column_sum_kernel(const uint16_t *in, long long rows, int cols, float *out) {
+    __shared__ float sums[8][64];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int c0 = (int)(blockIdx.x / ranks) * 64, c = c0 + (lane & 7) * 8;
-    f32x2 sum[4];
+    const int c0 = (int)blockIdx.x * 64, c = c0 + (lane & 7) * 8;
+    float sum[8] = {};
+    if (c < cols)
+        for (long long r = warp * 4 + (lane >> 3); r < rows; r += 32) {
+            const uint4 v = __ldcg(reinterpret_cast<const uint4 *>(in + (size_t)r * cols + c));
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] = pair_of(0.f, 0.f);
-    if (c < cols) {
-        constexpr int kAhead = 8;
-        const long long step = (long long)ranks * kWarps * 4;
-        for (long long r = (rank * kWarps + warp) * 4 + (lane >> 3); r < rows; r += step * kAhead) {
-            uint4 v[kAhead];
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i)
-                v[i] = r + i * step < rows ? __ldcg(reinterpret_cast<const uint4 *>(in + (size_t)(r + i * step) * cols + c)) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float lo, hi;
-                    widen16<kBf16>(w[j], lo, hi);
-                    sum[j] = pair_add(sum[j], pair_of(lo, hi));
-                }
+            for (int j = 0; j < 4; ++j) {
+                float lo, hi;
+                widen16<kBf16>(w[j], lo, hi);
+                sum[2 * j] += lo;
+                sum[2 * j + 1] += hi;
             }
         }
-    }
-    float column[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        float v[2];
-        pair_split(sum[j], v[0], v[1]);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            v[h] += __shfl_xor_sync(kFullMask, v[h], 16);
-            v[h] += __shfl_xor_sync(kFullMask, v[h], 8);
-            column[2 * j + h] = v[h];
-        }
+    for (int i = 0; i < 8; ++i) {
+        sum[i] += __shfl_xor_sync(kFullMask, sum[i], 16);
+        sum[i] += __shfl_xor_sync(kFullMask, sum[i], 8);
+        if (lane < 8) sums[warp][lane * 8 + i] = sum[i];
     }
-    for (int w = 0; w < kWarps; ++w) {  // the warps in turn
-        if (warp == w && lane < 8)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sums[lane * 8 + i] = w ? sums[lane * 8 + i] + column[i] : column[i];
-        __syncthreads();
-    }
-    if (ranks > 1) cluster.sync();
-    if (rank == 0 && threadIdx.x < 64 && c0 + (int)threadIdx.x < cols) {
-        float total = sums[threadIdx.x];
-        for (int r = 1; r < ranks; ++r) total += *cluster.map_shared_rank(sums + threadIdx.x, r);
-        out[c0 + threadIdx.x] = total;
-    }
-    if (ranks > 1) cluster.sync();  // nobody leaves while its sums may still be read
-    grid_dependency_wait();
+    __syncthreads();
+    if (threadIdx.x >= 64 || c0 + (int)threadIdx.x >= cols) return;
+    float total = 0.f;
+    for (int w = 0; w < 8; ++w) total += sums[w][threadIdx.x];
+    out[c0 + threadIdx.x] = total;
 }
 
 }  // namespace ko
