@@ -74,7 +74,7 @@ int ko_gemm_tc_tuned(int fmt, int out_fmt, int b_row_major, int64_t M, int64_t N
 
 /* the linear layer's calls with a pinned plan: tile 0 = choose, 128 / 256 = columns of D per 128-row tile of one CTA, 2048 = a
  * pair of CTAs per 256 x 256 tile (both only where D can be stored by TMA); slices: with a pinned tile, K slices (0 / 1 = none,
- * at most 64; not for 2048), for which the workspace must hold slices * tiles * 128 * tile floats, and for dbias 4 * max(slices, 1) * N floats
+ * at most 64), for which the workspace must hold slices * tiles * their elements floats, and for dbias 4 * max(slices, 1) * N floats
  * more; a pinned tile also takes the forward call past the few-token kernel */
 int ko_linear_tuned(int in_fmt, int out_fmt, int activation, int64_t M, int64_t N, int64_t K, const void *X, const void *W,
                     const void *bias, const void *residual, void *Y, void *Z, void *workspace, size_t workspace_bytes, int tile,

@@ -15,11 +15,12 @@
 
 namespace ko {
 
-// D[M, N] = A B over K, in 128 x bn tiles of one CTA (K cut into `split` slices), or 256 x 256 tiles of a pair of CTAs
+// D[M, N] = A B over K, in 128 x bn tiles of one CTA or 256 x 256 tiles of a pair of CTAs, K cut into `split` slices
 struct ProductPlan {
     bool pair;
     int bn, split;
-    size_t bytes() const { return split > 1 ? (size_t)tiles * split * 128 * bn * sizeof(float) : 0; }
+    int rows() const { return pair ? 256 : 128; }
+    size_t bytes() const { return split > 1 ? (size_t)tiles * split * rows() * bn * sizeof(float) : 0; }
     long long tiles;
 };
 
@@ -30,25 +31,27 @@ struct ProductPlan {
 // read once) at 5 TB/s.  Fitted to forced plans, BF16, measured (modelled):
 // 16384 x 4096 x 1024 pair 103 (103), 128 x 256 110 (112), 128 x 128 164 (165); 4096^3 93 (97), 102 (103), 142 (139);
 // 8192 x 768 x 768 16.6 (15.9), 17.4 (16.3), 18.2 (17.1); 2048 x 1024 x 1024 13.6 (11.6), 14.0 (11.8), 11.1 (8.8); 4096 x 4096 x 64
-// to FP32 19.0 (17.7), 15.5 (17.3), 14.0 (17.3); 768 x 768 x 8192 in four slices of 128-wide tiles 20.2 (22.7 with the 5).
+// to FP32 19.0 (17.7), 15.5 (17.3), 14.0 (17.3); 768 x 768 x 8192 in four slices of 128-wide tiles 20.2 (22.7 with the 5).  A pair's tile
+// in slices, where its few tiles leave most pairs idle: weight gradients of 32768 tokens, 512 x 2048 in four 67 (82 as 128 x 256 in four,
+// 176 uncut); 16384 tokens, 2048 x 1024 in two 66 (78 as 128 x 256 in two, 93 uncut).
 inline ProductPlan plan_product(int64_t M, int64_t N, int64_t K, bool tma, int element_bytes, int sms) {
     const long long k_blocks = (K + tc::kBK - 1) / tc::kBK;
     ProductPlan best{false, 128, 1, 0};
     double best_cost = 1e300;
-    if (tma && M > 128 && N > 128) {
-        const long long tiles = ((M + 255) / 256) * ((N + 255) / 256);
-        const long long rounds = (tiles + sms / 2 - 1) / (sms / 2);
-        best_cost = 4.5 + (double)rounds * ((double)k_blocks * 0.335 + 0.3 + 0.7 * element_bytes);
-        best = {true, 256, 1, tiles};
-    }
-    for (int bn : {128, 256}) {
-        if (bn == 256 && (!tma || N <= 128)) continue;
-        const double per_block = bn == 256 ? 0.36 : 0.29, start = bn == 256 ? 4.3 : 3.0;
-        const auto per_tile = [&](int bytes) { return bn == 256 ? 0.5 + 0.6 * bytes : 0.5 + 0.35 * bytes; };
-        const long long tiles = ((M + 127) / 128) * ((N + bn - 1) / bn);
-        const long long most = std::min<long long>(std::max<long long>(sms / tiles, 1), std::max<long long>(k_blocks / 4, 1));
+    struct Tile {
+        bool pair;
+        int bn;
+        double start, per_block, once, per_byte;  // us: a launch, a K-block, an epilogue and each byte of its elements
+    };
+    for (const Tile &tile : {Tile{true, 256, 4.5, 0.335, 0.3, 0.7}, Tile{false, 128, 3.0, 0.29, 0.5, 0.35}, Tile{false, 256, 4.3, 0.36, 0.5, 0.6}}) {
+        if (tile.bn == 256 && (!tma || N <= 128 || (tile.pair && M <= 128))) continue;
+        const int rows = tile.pair ? 256 : 128, bn = tile.bn, at_once = tile.pair ? sms / 2 : sms;
+        const double per_block = tile.per_block, start = tile.start;
+        const auto per_tile = [&](int bytes) { return tile.once + tile.per_byte * bytes; };
+        const long long tiles = ((M + rows - 1) / rows) * ((N + bn - 1) / bn);
+        const long long most = std::min<long long>(std::max<long long>(at_once / tiles, 1), std::max<long long>(k_blocks / 4, 1));
         for (int split = 1; split <= most && split <= 64; ++split) {
-            const long long rounds = (tiles * split + sms - 1) / sms;
+            const long long rounds = (tiles * split + at_once - 1) / at_once;
             double cost = start + (double)rounds * ((double)((k_blocks + split - 1) / split) * per_block + per_tile(split > 1 ? 4 : element_bytes));
             if (split > 1) {
                 const double written = (double)((M + 31) / 32 * 32) * (double)N * split, read = (double)M * (double)N * split;
@@ -56,7 +59,7 @@ inline ProductPlan plan_product(int64_t M, int64_t N, int64_t K, bool tma, int e
             }
             if (cost < best_cost) {
                 best_cost = cost;
-                best = {false, bn, split, tiles};
+                best = {tile.pair, bn, split, tiles};
             }
         }
     }
@@ -73,13 +76,12 @@ inline int pin_product(const PinnedPlan &pin, int64_t M, int64_t N, int64_t K, b
     KO_REQUIRE(pin.tile == 128 || pin.tile == 256 || pin.tile == 2048, KO_ERR_INVALID_ARG, "%s: tile code %d not in {128,256,2048}", name, pin.tile);
     KO_REQUIRE(tma || pin.tile == 128, KO_ERR_SHAPE, "%s: without TMA stores there is only the 128-column tile", name);
     const long long k_blocks = (K + tc::kBK - 1) / tc::kBK;
-    KO_REQUIRE(pin.slices >= 0 && pin.slices <= 64 && pin.slices <= k_blocks && (pin.tile != 2048 || pin.slices <= 1), KO_ERR_INVALID_ARG,
+    KO_REQUIRE(pin.slices >= 0 && pin.slices <= 64 && pin.slices <= k_blocks, KO_ERR_INVALID_ARG,
                "%s: %d K slices out of range", name, pin.slices);
     plan->pair = pin.tile == 2048;
     plan->bn = plan->pair ? 256 : pin.tile;
     plan->split = pin.slices > 1 ? pin.slices : 1;
-    const int rows = plan->pair ? 256 : 128;
-    plan->tiles = ((M + rows - 1) / rows) * ((N + plan->bn - 1) / plan->bn);
+    plan->tiles = ((M + plan->rows() - 1) / plan->rows()) * ((N + plan->bn - 1) / plan->bn);
     return KO_OK;
 }
 
@@ -142,8 +144,8 @@ int launch_product_pair(const CUtensorMap &ma, const CUtensorMap &mb, const CUte
     if (int st = ensure_dynamic_smem(id, Cfg::kSmemBytes)) return st;
     int resident = 0;
     if (int st = resident_pairs_of(id, threads, Cfg::kSmemBytes, &resident)) return st;
-    const long long tiles = (long long)((p.M + 255) / 256) * ((p.N + 255) / 256);
-    return launch_clustered_overlapped(kernel, 2u * (unsigned)std::min<long long>(tiles, resident), threads, 2u, (size_t)Cfg::kSmemBytes, s, ma,
+    const long long units = (long long)((p.M + 255) / 256) * ((p.N + 255) / 256) * p.split_k;
+    return launch_clustered_overlapped(kernel, 2u * (unsigned)std::min<long long>(units, resident), threads, 2u, (size_t)Cfg::kSmemBytes, s, ma,
                                        mb, mb, md, p);
 }
 
@@ -218,8 +220,8 @@ int run_product(LinearParams p, const void *A, const void *B, void *workspace, s
     if constexpr (kMode == LinearMode::kWeightGrad)
         if (fold && plan.split == 1) return launch_overlapped(linear_fold_sums_kernel<256>, (unsigned)((p.M + 255) / 256), 256u, (size_t)0, s, p);
     if (plan.split <= 1) return KO_OK;
-    const long long chunks = plan.tiles * 4 * (plan.bn / 32);
-    return launch_overlapped(linear_slice_sum_kernel<kMode, kOut16>, (unsigned)chunks, 256u, (size_t)0, s, p, plan.bn);
+    const long long chunks = plan.tiles * (plan.rows() / 32) * (plan.bn / 32);
+    return launch_overlapped(linear_slice_sum_kernel<kMode, kOut16>, (unsigned)chunks, 256u, (size_t)0, s, p, plan.rows(), plan.bn);
 }
 
 // the checks that the three entry points share; M tokens, N output features, K input features

@@ -248,7 +248,7 @@ struct GemmParams {
     // bn_narrow <= bn_wide <= BN; column-major B only): a tile count that fills the last wave of CTAs instead of
     // leaving part of it idle.  map_b then has a box of bn_wide rows and map_b_narrow one of bn_narrow rows.
     int tiles_n, wide_tiles_n, bn_wide, bn_narrow;
-    // K slices (single-CTA kernel only).  split_k > 1: every tile is computed by split_k CTAs, each over a contiguous
+    // K slices (of plain products: single-CTA kernel only).  split_k > 1: every tile is computed by split_k CTAs, each over a contiguous
     // range of K-blocks, and every CTA writes its FP32 partial tile to `partials` (one slot of kTileM x BN floats per
     // (tile, slice)) instead of D; gemm_slice_sum_kernel, launched behind this kernel, adds the slices in K order and
     // writes D.

@@ -147,10 +147,22 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     const uint32_t rank = cluster_cta_rank();  // 0 = leader
     const bool leader = rank == 0;
     const int tiles_m = (p.M + kTileM - 1) / kTileM, tiles_n = p.tiles_n ? p.tiles_n : (p.N + BN - 1) / BN;
-    const long long num_tiles = (long long)tiles_m * tiles_n;
     const int k_blocks = (p.K + kBK - 1) / kBK;
     [[maybe_unused]] const int period = Epi::kPromote ? kPeriod : k_blocks;  // K-blocks that share an accumulator
     const long long pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    // work units as in the single-CTA kernel; only fused epilogues are given K slices
+    const int split = Epi::kFused && p.split_k > 1 ? p.split_k : 1;
+    const long long num_units = (long long)tiles_m * tiles_n * split;
+    auto unit_of = [&](long long u, long long &t, int &slice, int &kb0, int &kb1) {
+        if (!Epi::kFused || split == 1) {
+            t = u; slice = 0; kb0 = 0; kb1 = k_blocks;
+        } else {
+            t = u / split;
+            slice = (int)(u - t * split);
+            kb0 = (int)((long long)k_blocks * slice / split);
+            kb1 = (int)((long long)k_blocks * (slice + 1) / split);
+        }
+    };
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < Cfg::kStages; ++s) {
@@ -191,14 +203,16 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         if (lane == 0) {
             uint32_t it = 0;
             bool ok = true;
-            for (long long t = pair; t < num_tiles && ok; t += pairs) {
-                int tm, tn, col0, bn;
+            for (long long u = pair; u < num_units && ok; u += pairs) {
+                long long t;
+                int slice, kb0, kb1, tm, tn, col0, bn;
+                unit_of(u, t, slice, kb0, kb1);
                 tile_of(p, t, tiles_m, tiles_n, tm, tn);
                 column_tile<BN>(p, tn, col0, bn);
                 const int half = bn >> 1;  // this CTA's share of the tile's columns
                 const CUtensorMap *b_map = (p.tiles_n && bn != p.bn_wide) ? &map_b_narrow : &map_b;  // box of bn / 2 rows
                 const uint32_t cta_bytes = (uint32_t)Cfg::kBytesA + (uint32_t)half * (kBK * 2);
-                for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+                for (int kb = kb0; kb < kb1; ++kb, ++it) {
                     const int s = it % Cfg::kStages;
                     const uint32_t phase = (it / Cfg::kStages) & 1u;
                     if (!mbar_wait(empty_bar(s), phase ^ 1u, abort_flag)) {
@@ -250,15 +264,17 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
             bool ok = true;
             const uint32_t own_empty0 = map_to_cluster_rank(empty_bar(0), 0);
             const uint32_t peer_ready0 = map_to_cluster_rank(acc_ready_bar(0), 1), own_ready0 = map_to_cluster_rank(acc_ready_bar(0), 0);
-            for (long long t = pair; t < num_tiles && ok; t += pairs, ++local_tile) {
-                int tm, tn, col0, bn;
+            for (long long u = pair; u < num_units && ok; u += pairs, ++local_tile) {
+                long long t;
+                int slice, kb0, kb1, tm, tn, col0, bn;
+                unit_of(u, t, slice, kb0, kb1);
                 tile_of(p, t, tiles_m, tiles_n, tm, tn);
                 column_tile<BN>(p, tn, col0, bn);
                 // bit 15: A is MN-major, bit 16: B is MN-major
                 const uint32_t idesc = make_idesc(p.fmt, kTileM, bn) | (p.b_row_major ? 1u << 16 : 0u) | (Epi::kTransA ? 1u << 15 : 0u);
-                for (int k0 = 0; k0 < k_blocks && ok; k0 += period) {
-                    if (k0 != 0) ++local_tile;
-                    const int k_end = Epi::kPromote ? min(k0 + period, k_blocks) : k_blocks;
+                for (int k0 = kb0; k0 < kb1 && ok; k0 += period) {
+                    if (k0 != kb0) ++local_tile;
+                    const int k_end = Epi::kPromote ? min(k0 + period, kb1) : kb1;
                     const uint32_t acc = local_tile & 1u, acc_phase = (local_tile >> 1) & 1u;
                     if (!mbar_wait_remote(acc_free_bar(acc), acc_phase ^ 1u, abort_flag)) { ok = false; break; }
                     tc_fence_after();
@@ -301,13 +317,15 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
             const int box = warp - 2 - Epi::kWarps;  // 64 of the CTA's 128 rows of the product
             uint32_t stage = 0, phase = 0;
             bool ok = true;
-            for (long long t = pair; p.sum_shares && t < num_tiles && ok; t += pairs) {
-                int tm, tn;
+            for (long long u = pair; p.sum_shares && u < num_units && ok; u += pairs) {
+                long long t;
+                int slice, kb0, kb1, tm, tn;
+                unit_of(u, t, slice, kb0, kb1);
                 tile_of(p, t, tiles_m, tiles_n, tm, tn);
                 const bool mine = tn < p.sum_shares;
                 typename Epi::Sums sums;
-                int next = tn;  // the next K-block that this tile adds
-                for (int kb = 0; kb < k_blocks; ++kb) {
+                int next = kb0 + (tn - kb0 % p.sum_shares + p.sum_shares) % p.sum_shares;  // the next K-block that this tile adds
+                for (int kb = kb0; kb < kb1; ++kb) {
                     // The pair's loads complete on the leader's barrier; its first sum warp passes the word on.  A token (relaxed):
                     // what the peer's sum warps read came into their own SM's shared memory before the leader's barrier heard of
                     // it.  A releasing arrive took 0.7 us a K-block longer, which the whole ring then waited for.
@@ -321,7 +339,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                     if (lane == 0) mbar_arrive(empty_bar(stage));
                     if (++stage == (uint32_t)Cfg::kStages) { stage = 0; phase ^= 1u; }
                 }
-                if (ok && mine) sums.store(p, tn, tm * kTileM + (int)rank * kBM + box * 64, lane);
+                if (ok && mine) sums.store(p, slice * p.sum_shares + tn, tm * kTileM + (int)rank * kBM + box * 64, lane);
             }
             if (!ok) {
                 if (lane == 0 && !*abort_flag) atomicCAS(p.status, kStatusOk, kTimeoutEpilogue);
@@ -340,14 +358,17 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         }
         uint32_t local_tile = 0, store_seq = 0;
         bool ok = true;
-        for (long long t = pair; t < num_tiles && ok; t += pairs, ++local_tile) {
-            int tm, tn, col0, bn;
+        for (long long u = pair; u < num_units && ok; u += pairs, ++local_tile) {
+            long long t;
+            int slice, kb0, kb1, tm, tn, col0, bn;
+            unit_of(u, t, slice, kb0, kb1);
             tile_of(p, t, tiles_m, tiles_n, tm, tn);
             column_tile<BN>(p, tn, col0, bn);
             const int row_base = tm * kTileM + (int)rank * kBM + quad * 32;
-            if constexpr (Epi::kFused) Epi::bring(fused, p, row_base, col0 + share * Epi::kChunk, lane);  // while the tile is being computed
+            if constexpr (Epi::kFused)
+                if (split == 1) Epi::bring(fused, p, row_base, col0 + share * Epi::kChunk, lane);  // while the tile is being computed
             if constexpr (Epi::kPromote) {
-                const int periods = (k_blocks + kPeriod - 1) / kPeriod;
+                const int periods = (kb1 - kb0 + kPeriod - 1) / kPeriod;
                 ok = Epi::template promote<BN, true>(tmem_base + ((uint32_t)(quad * 32) << 16), share, periods, local_tile, acc_ready_bar(0),
                                                      map_to_cluster_rank(acc_free_bar(0), 0), abort_flag);
                 local_tile += (uint32_t)periods - 1;  // the accumulator that holds the sums
@@ -362,7 +383,12 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
             tc_fence_after();
             const uint32_t t_row = tmem_base + ((uint32_t)(quad * 32) << 16) + acc * BN;
             if constexpr (Epi::kFused) {
-                if (!Epi::template block<kTmaStore>(&map_d, p, fused, t_row, row_base, col0, bn, share * Epi::kChunk, lane, abort_flag)) {
+                if (split > 1) {
+                    // a K slice: the partial tile goes to its slot, the slice-sum kernel writes D
+                    float *slot = p.partials + ((size_t)t * split + slice) * ((size_t)kTileM * BN);
+                    if (row_base < p.M)
+                        publish_block(slot + ((size_t)(((int)rank * 4 + quad) * (BN / 32)) << 10), t_row, bn, lane, share * 32, 8 * Epi::kWarps);
+                } else if (!Epi::template block<kTmaStore>(&map_d, p, fused, t_row, row_base, col0, bn, share * Epi::kChunk, lane, abort_flag)) {
                     if (lane == 0 && !*abort_flag) atomicCAS(p.status, kStatusOk, kTimeoutEpilogue);
                     *abort_flag = 1;
                     ok = false;

@@ -542,25 +542,25 @@ private:
 };
 
 // Second step of a product cut into K slices (see tc::gemm_slice_sum_kernel): the slices of a 32 x 32 chunk are added in
-// K order, then the epilogue.  One block per chunk, thread i takes columns 4 * (i % 8) .. + 3 of row i / 8.
+// K order, then the epilogue.  tile_m, bn: the product's tile.  One block per chunk, thread i takes columns 4 * (i % 8) .. + 3 of row i / 8.
 template <LinearMode kMode, bool kOut16>
-__global__ void __launch_bounds__(256) linear_slice_sum_kernel(const LinearParams p, int bn) {
-    const int chunks_n = bn / 32, chunks_per_tile = (tc::kBM / 32) * chunks_n;
+__global__ void __launch_bounds__(256) linear_slice_sum_kernel(const LinearParams p, int tile_m, int bn) {
+    const int chunks_n = bn / 32, chunks_per_tile = (tile_m / 32) * chunks_n;
     const long long t = blockIdx.x / chunks_per_tile;
     const int chunk = (int)(blockIdx.x - t * chunks_per_tile);
-    const int tiles_m = (p.M + tc::kBM - 1) / tc::kBM, tiles_n = (p.N + bn - 1) / bn;
+    const int tiles_m = (p.M + tile_m - 1) / tile_m, tiles_n = (p.N + bn - 1) / bn;
     int tm, tn;
     tc::tile_coords(t, tiles_m, tiles_n, tm, tn);
-    const int row = tm * tc::kBM + (chunk / chunks_n) * 32 + (int)threadIdx.x / 8;
+    const int row = tm * tile_m + (chunk / chunks_n) * 32 + (int)threadIdx.x / 8;
     const int col = tn * bn + (chunk % chunks_n) * 32 + ((int)threadIdx.x & 7) * 4;
     grid_launch_dependents();
     grid_dependency_wait();  // the slices are complete and visible
     if constexpr (kMode == LinearMode::kWeightGrad) {  // the blocks of dW's first 32 columns fold the column sums of their rows
-        const int sum_row = tm * tc::kBM + (chunk / chunks_n) * 32 + (int)threadIdx.x;
+        const int sum_row = tm * tile_m + (chunk / chunks_n) * 32 + (int)threadIdx.x;
         if (p.sum_shares && tn == 0 && chunk % chunks_n == 0 && threadIdx.x < 32 && sum_row < p.M) p.dbias[sum_row] = fold_sum_parts(p, sum_row);
     }
     if (row >= p.M || col >= p.N) return;
-    const size_t slot_vecs = (size_t)tc::kBM * bn / 4;
+    const size_t slot_vecs = (size_t)tile_m * bn / 4;
     const float4 *src = reinterpret_cast<const float4 *>(p.partials) + (size_t)t * p.split_k * slot_vecs + ((size_t)chunk << 8) + threadIdx.x;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int s0 = 0; s0 < p.split_k; s0 += 4) {

@@ -248,7 +248,7 @@ def test_fp32_results_of_long_sums(cuda, lib, ko, n, k):
     assert lib.ko_poll_device_status() == 0
 
 
-@pytest.mark.parametrize("tile,slices", [(128, 0), (128, 3), (256, 0), (256, 2), (2048, 0)])
+@pytest.mark.parametrize("tile,slices", [(128, 0), (128, 3), (256, 0), (256, 2), (2048, 0), (2048, 3)])
 def test_every_plan_of_the_three_products(cuda, lib, ko, tile, slices):
     """Pinned tiles and K slices, with short and long sums, FP32 and 16-bit results."""
     P = lambda t: None if t is None else t.data_ptr()
