@@ -734,8 +734,10 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             unit_of(u, t, slice, kb0, kb1);
             tile_of(p, t, tiles_m, tiles_n, tm, tn);
             column_tile<BN>(p, tn, col0, bn);
-            if constexpr (Epi::kFused)  // the first chunk's operand arrives while the tile is still being computed
+            if constexpr (Epi::kFused) {  // the first chunk's operand arrives while the tile is still being computed
                 if (kTmaStore && split == 1) Epi::bring(fused, p, tm * kTileM + quad * 32, col0 + share * Epi::kChunk, lane);
+                if (!kTmaStore && split == 1) Epi::bring_rows(fused, p, tm * kTileM + quad * 32, col0 + share * Epi::kChunk, lane);
+            }
             if constexpr (Epi::kPromote) {
                 const int periods = (kb1 - kb0 + kPeriod - 1) / kPeriod;
                 ok = Epi::template promote<BN, false>(tmem_base + ((uint32_t)(quad * 32) << 16), share, periods, local_tile, acc_ready_bar(0),

@@ -11,6 +11,8 @@
 // (Four for the weight gradient, which only stores.)
 #pragma once
 
+#include <type_traits>
+
 #include "../gemm/tensor_core_gemm.h"
 #include "activation.h"
 
@@ -260,14 +262,27 @@ struct LinearEpilogue {
             } else {
 #pragma unroll 1
                 for (int h = 0; h < kChunk; h += 32) {
+                    const int c = c0 + h, next = h + 32 < kChunk ? c + 32 : c0 + kStep;
+                    const bool more = p.extra && next < bn && col0 + next < p.N;
+                    float coming[32];  // the extra operand of the next chunk, on its way meanwhile
+                    if (more) fetch_rows(p, coming, row_base, col0 + next + lane);
                     f32x2 r[16];
-                    sums_at(t_row + c0 + h, r);
-                    if (p.fmt) chunk_by_rows<true>(p, r, row_base, col0 + c0 + h, lane, st.boxes);
-                    else chunk_by_rows<false>(p, r, row_base, col0 + c0 + h, lane, st.boxes);
+                    sums_at(t_row + c, r);
+                    if (p.fmt) chunk_by_rows<true>(p, r, row_base, col0 + c, lane, st.boxes);
+                    else chunk_by_rows<false>(p, r, row_base, col0 + c, lane, st.boxes);
+                    if (more) keep_rows(st, coming, lane);
                 }
             }
         }
         return true;
+    }
+
+    // the first chunk's extra operand for the row-wise form
+    __device__ __forceinline__ static void bring_rows(State &st, const Params &p, int row_base, int col, int lane) {
+        if (p.extra == nullptr || row_base >= p.M || col >= p.N) return;
+        float x[32];
+        fetch_rows(p, x, row_base, col + lane);
+        keep_rows(st, x, lane);
     }
 
     // before the block leaves: nothing may still arrive in its shared memory or be read from it
@@ -281,42 +296,50 @@ private:
     // Rows that start anywhere (odd N, unaligned operands): the chunk is turned in shared memory (4 KB, column c of row r at
     // c ^ r: no bank conflict either way) so that a lane has one column, and every access is 32 neighbouring elements of
     // a row.  Written straight from a lane's own row, each store touched 32 sectors: 1021 x 2053 x 1096 FP32 22 us.
+    // Instructions count: with 46 of them for a row's 32 elements the same call took 17.2 us, now 14.0 (30 -> 15.2 with a residual).
     template <bool kBf16>
     __device__ __forceinline__ static void chunk_by_rows(const Params &p, const f32x2 (&r)[16], int row_base, int col, int lane, uint32_t box) {
+        using Stored = std::conditional_t<kOut16, uint16_t, float>;
         __syncwarp();
+        const uint32_t own = box + (uint32_t)lane * 132u;  // boxes are aligned to their size
 #pragma unroll
         for (int c = 0; c < 32; ++c) {
             float lo, hi;
             pair_split(r[c / 2], lo, hi);
-            asm volatile("st.shared.f32 [%0], %1;" ::"r"(box + (uint32_t)(lane * 32 + (c ^ lane)) * 4u), "f"(c & 1 ? hi : lo) : "memory");
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(own ^ (uint32_t)(c * 4)), "f"(c & 1 ? hi : lo) : "memory");
         }
         __syncwarp();
         const int c = col + lane, rows = min(32, p.M - row_base);
         if (c >= p.N) return;
         float bias = 0.f;
         if (kMode == LinearMode::kForward && p.bias) bias = widen16_at<kBf16>(p.bias, (size_t)c);
-        constexpr int kRows = 8;  // rows whose operands are on their way together
+        const size_t at = (size_t)row_base * p.N + c;
+        Stored *out = static_cast<Stored *>(p.D) + at;
+        uint16_t *pre = kMode == LinearMode::kForward && p.pre ? static_cast<uint16_t *>(p.pre) + at : nullptr;
+        const uint32_t column = box + (uint32_t)lane * 4u;
+        constexpr int kRows = 8;
 #pragma unroll 1
         for (int i0 = 0; i0 < rows; i0 += kRows) {
-            const size_t at = (size_t)(row_base + i0) * p.N + c;
-            float x[kRows], v[kRows];
+            const uint32_t from = (column + (uint32_t)i0 * 128u) ^ (uint32_t)(i0 * 4), extra = column + kBoxBytes + (uint32_t)i0 * 128u;
+            const int left = rows - i0;
+            float v[kRows];
 #pragma unroll
             for (int i = 0; i < kRows; ++i) {
-                x[i] = 0.f;
-                if (p.extra && i0 + i < rows) {
-                    if constexpr (kExtra16) x[i] = widen16_at<kBf16>(p.extra, at + (size_t)i * p.N);
-                    else x[i] = static_cast<const float *>(p.extra)[at + (size_t)i * p.N];
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[i]) : "r"((from ^ (uint32_t)(i * 4)) + (uint32_t)i * 128u) : "memory");
+                if constexpr (kMode == LinearMode::kForward)
+                    if (p.bias) v[i] += bias;
+            }
+            if constexpr (kMode == LinearMode::kForward)
+                if (pre) {
+                    uint16_t z[kRows];
+#pragma unroll
+                    for (int i = 0; i < kRows; ++i) z[i] = (uint16_t)tc::pack16(v[i], 0.f, kBf16 ? 2 : 1);
+                    put_rows(pre, z, p.N, left);
                 }
-            }
+            float x[kRows];
+            if (p.extra)
 #pragma unroll
-            for (int i = 0; i < kRows; ++i) {
-                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v[i]) : "r"(box + (uint32_t)((i0 + i) * 32 + (lane ^ (i0 + i))) * 4u) : "memory");
-                if (kMode == LinearMode::kForward && p.bias) v[i] += bias;
-            }
-            if (kMode == LinearMode::kForward && p.pre)
-#pragma unroll
-                for (int i = 0; i < kRows; ++i)
-                    if (i0 + i < rows) static_cast<uint16_t *>(p.pre)[at + (size_t)i * p.N] = (uint16_t)tc::pack16(v[i], 0.f, kBf16 ? 2 : 1);
+                for (int i = 0; i < kRows; ++i) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x[i]) : "r"(extra + (uint32_t)i * 128u) : "memory");
             if (p.activation != kActNone)
                 with_activation(p.activation, [&](auto act) {
 #pragma unroll
@@ -335,12 +358,58 @@ private:
                         }
                     }
                 });
+            if (kMode != LinearMode::kInputGrad && p.extra)
+#pragma unroll
+                for (int i = 0; i < kRows; ++i) v[i] = __fadd_rn(v[i], x[i]);
+            Stored y[kRows];
 #pragma unroll
             for (int i = 0; i < kRows; ++i) {
-                if (kMode != LinearMode::kInputGrad && p.extra) v[i] = __fadd_rn(v[i], x[i]);
-                if (i0 + i < rows) linear_store_one<kBf16, kOut16>(p, v[i], row_base + i0 + i, c);
+                if constexpr (kOut16) y[i] = (uint16_t)tc::pack16(v[i], 0.f, kBf16 ? 2 : 1);
+                else y[i] = v[i];
+            }
+            put_rows(out, y, p.N, left);
+        }
+    }
+    // v[i] to row i of the rows that are left, `to` moved past them
+    template <class T, int kRows>
+    __device__ __forceinline__ static void put_rows(T *&to, const T (&v)[kRows], int pitch, int left) {
+        if (left >= kRows) {
+#pragma unroll
+            for (int i = 0; i < kRows; ++i, to += pitch) *to = v[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < kRows; ++i, to += pitch)
+                if (i < left) *to = v[i];
+        }
+    }
+    // The extra operand of 32 rows in column c, by plain loads that are all on their way together (in batches of eight, each
+    // batch's between two batches of stores, 1021 x 2053 x 1096 with a residual took 30 us), kept as FP32 in the warp's
+    // second box, where each lane finds its own column again.
+    __device__ __forceinline__ static void fetch_rows(const Params &p, float (&x)[32], int row_base, int c) {
+        const int rows = min(32, p.M - row_base);
+        const size_t at = (size_t)row_base * p.N + c;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            x[i] = 0.f;
+            if (c < p.N && i < rows) {
+                if constexpr (kExtra16) x[i] = __uint_as_float(static_cast<const uint16_t *>(p.extra)[at + (size_t)i * p.N]);
+                else x[i] = static_cast<const float *>(p.extra)[at + (size_t)i * p.N];
             }
         }
+        if constexpr (kExtra16) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                float lo, hi;
+                if (p.fmt) widen16<true>(__float_as_uint(x[i]), lo, hi);
+                else widen16<false>(__float_as_uint(x[i]), lo, hi);
+                x[i] = lo;
+            }
+        }
+    }
+    __device__ __forceinline__ static void keep_rows(State &st, const float (&x)[32], int lane) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(st.boxes + kBoxBytes + (uint32_t)(i * 128 + lane * 4)), "f"(x[i]) : "memory");
     }
 
     // address of 16-byte piece j of row `lane` of a box: rows of 128 bytes with the 128-byte swizzle, or of 64 bytes with the
