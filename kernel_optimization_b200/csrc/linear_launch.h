@@ -28,12 +28,11 @@ struct ProductPlan {
 // of D (D itself, Z, the extra operand).  Modelled microseconds per candidate: start, then rounds of work units x (K-blocks
 // of 64 x time per K-block + epilogue time that the next tile does not hide); slices add a second kernel (2 us of the
 // device, 4 of the host with the workspace; 5 is what they have to gain) and the partial tiles' way through the L2 (written once,
-// read once) at 5 TB/s.  Fitted to forced plans, BF16, measured (modelled):
-// 16384 x 4096 x 1024 pair 103 (103), 128 x 256 110 (112), 128 x 128 164 (165); 4096^3 93 (97), 102 (103), 142 (139);
-// 8192 x 768 x 768 16.6 (15.9), 17.4 (16.3), 18.2 (17.1); 2048 x 1024 x 1024 13.6 (11.6), 14.0 (11.8), 11.1 (8.8); 4096 x 4096 x 64
-// to FP32 19.0 (17.7), 15.5 (17.3), 14.0 (17.3); 768 x 768 x 8192 in four slices of 128-wide tiles 20.2 (22.7 with the 5).  A pair's tile
-// in slices, where its few tiles leave most pairs idle: weight gradients of 32768 tokens, 512 x 2048 in four 67 (82 as 128 x 256 in four,
-// 176 uncut); 16384 tokens, 2048 x 1024 in two 66 (78 as 128 x 256 in two, 93 uncut).
+// read once) at 5 TB/s.  Fitted to forced plans, BF16, measured (modelled), pair / 128 x 128 / 128 x 256:
+// 16384 x 4096 x 1024 101 (100), 135 (135), 114 (107); 4096^3 96 (93), 118 (110), 117 (101); 8192 x 768 x 768 18.8 (15.6), 18.1
+// (14.5), 20.2 (16.1); 1024 x 1024 x 4096 26 (27), 19.8 (18.3), 33 (28), 128 x 128 in two slices 20.2 (20.7).  Slices, where a few
+// tiles leave most SMs idle: 512 x 2048 x 32768 (a weight gradient) pair in four 65 (61), 128 x 256 in four 77 (65), uncut 156 (171);
+// 768 x 768 x 16384 128 x 128 in four 24.5, uncut 53.
 inline ProductPlan plan_product(int64_t M, int64_t N, int64_t K, bool tma, int element_bytes, int sms) {
     const long long k_blocks = (K + tc::kBK - 1) / tc::kBK;
     ProductPlan best{false, 128, 1, 0};
@@ -43,7 +42,7 @@ inline ProductPlan plan_product(int64_t M, int64_t N, int64_t K, bool tma, int e
         int bn;
         double start, per_block, once, per_byte;  // us: a launch, a K-block, an epilogue and each byte of its elements
     };
-    for (const Tile &tile : {Tile{true, 256, 4.5, 0.335, 0.3, 0.7}, Tile{false, 128, 3.0, 0.29, 0.5, 0.35}, Tile{false, 256, 4.3, 0.36, 0.5, 0.6}}) {
+    for (const Tile &tile : {Tile{true, 256, 4.5, 0.32, 0.3, 0.7}, Tile{false, 128, 3.0, 0.22, 0.5, 0.35}, Tile{false, 256, 4.3, 0.35, 0.5, 0.6}}) {
         if (tile.bn == 256 && (!tma || N <= 128 || (tile.pair && M <= 128))) continue;
         const int rows = tile.pair ? 256 : 128, bn = tile.bn, at_once = tile.pair ? sms / 2 : sms;
         const double per_block = tile.per_block, start = tile.start;

@@ -145,6 +145,19 @@ __device__ __forceinline__ void umma_f16_words(uint32_t d_tmem, uint32_t a_lo, u
         ::"r"(d_tmem), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// One lane of a converged warp, the same at every call.  The warps that issue MMAs and TMA loads run their loops as a whole and
+// let this lane issue: what the instructions take is then computed alike in all lanes, and a K-block costs the issuing
+// lane far less than in a loop of one lane alone, which bound the smaller tiles: a K-block of the 128 x 128 tile 310 -> 217 ns, with
+// an MN-major A (four loads) 318 -> 213; 128 x 256 389 -> 345; the pair with an MN-major A 335 -> 296, else 302 -> 296.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t yes;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(yes));
+    return yes != 0;
+}
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
@@ -569,7 +582,8 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
 
     if (warp == 0) {
         // ------------------------------------------------------------------ TMA producer
-        if (lane == 0) {
+        {
+            const bool issuer = elect_one();
             uint32_t it = 0, stage = 0, fill = 0;  // K-blocks issued, ring position of the next one, times the ring went round
             bool ok = true;
             for (long long u = blockIdx.x; u < num_units && ok; u += gridDim.x) {
@@ -590,8 +604,9 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                         ok = false;
                         break;
                     }
-                    mbar_expect_tx(full_bar(s), stage_bytes);
                     const uint32_t dst = ring + s * Cfg::kStageBytes;
+                    if (!issuer) continue;
+                    mbar_expect_tx(full_bar(s), stage_bytes);
                     if constexpr (Epi::kTransA) {
 #pragma unroll
                         for (int mb = 0; mb < kTileM / 64; ++mb)
@@ -621,9 +636,10 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------------------------ MMA issuer
-        if (lane == 0) {
-            uint32_t it = 0, local_tile = 0;
-            uint32_t stage = 0, phase = 0;  // ring position of K-block `it` and the parity of its fill
+        {
+            const bool issuer = elect_one();
+            uint32_t local_tile = 0;
+            uint32_t stage = 0, phase = 0;  // ring position of the next K-block and the parity of its fill
             // Shared-memory descriptors as two words (smem_desc_k_major_sw128 / smem_desc_mn_major_sw128 of the ring's
             // first stage): the high word (stride 1024 bytes, version, 128-byte swizzle) is the same for every operand,
             // the low word is the address in 16-byte units plus the leading offset (1 for K-major, 8192 bytes for a
@@ -651,25 +667,27 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     if (!mbar_wait(acc_free_bar(acc), acc_phase ^ 1u, abort_flag)) { ok = false; break; }
                     tc_fence_after();
                     const uint32_t d_tmem = tmem_base + acc * BN;
-                    for (int kb = k0; kb < k_end; ++kb, ++it) {
+                    for (int kb = k0; kb < k_end; ++kb) {
                         if (!mbar_wait(full_bar(stage), phase, abort_flag)) { ok = false; break; }
                         tc_fence_after();
                         // descriptors of this stage: the ring's plus the stage's offset in 16-byte units
                         const uint32_t a_lo = a_lo0 + stage * (uint32_t)(Cfg::kStageBytes >> 4), b_lo = b_lo0 + stage * (uint32_t)(Cfg::kStageBytes >> 4);
                         uint32_t accumulate = kb != k0 ? 1u : 0u;
+                        if (issuer) {
 #pragma unroll
-                        for (int k = 0; k < kBK / kUmmaK; ++k) {
-                            // advancing K inside the swizzled row: +32 bytes per 16 elements (K-major); row-major B: 16 K-rows
-                            // further = two 8-row atoms = 2048 bytes
-                            umma_f16_words(d_tmem, a_lo + k * a_kstep, desc_hi, b_lo + k * b_kstep, desc_hi, idesc, accumulate);
-                            if (MT == 2)  // rows 128..255 of the tile: 16 KB further in the stage, accumulator columns BN..2BN-1
-                                umma_f16_words(d_tmem + BN, a_lo + (kBM * kBK * 2 >> 4) + k * a_kstep, desc_hi, b_lo + k * b_kstep, desc_hi, idesc, accumulate);
-                            accumulate = 1u;
+                            for (int k = 0; k < kBK / kUmmaK; ++k) {
+                                // advancing K inside the swizzled row: +32 bytes per 16 elements (K-major); row-major B: 16 K-rows
+                                // further = two 8-row atoms = 2048 bytes
+                                umma_f16_words(d_tmem, a_lo + k * a_kstep, desc_hi, b_lo + k * b_kstep, desc_hi, idesc, accumulate);
+                                if (MT == 2)  // rows 128..255 of the tile: 16 KB further in the stage, accumulator columns BN..2BN-1
+                                    umma_f16_words(d_tmem + BN, a_lo + (kBM * kBK * 2 >> 4) + k * a_kstep, desc_hi, b_lo + k * b_kstep, desc_hi, idesc, accumulate);
+                                accumulate = 1u;
+                            }
+                            umma_commit(empty_bar(stage));  // the stage is reusable once these MMAs have read it
                         }
-                        umma_commit(empty_bar(stage));  // the stage is reusable once these MMAs have read it
                         if (++stage == (uint32_t)Cfg::kStages) { stage = 0; phase ^= 1u; }
                     }
-                    if (ok) umma_commit(acc_ready_bar(acc));
+                    if (ok && issuer) umma_commit(acc_ready_bar(acc));
                 }
             }
             if (!ok) {
@@ -677,10 +695,12 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 *abort_flag = 1;
             }
             // nothing may still be writing tensor memory when it is released
-            umma_commit(drain_bar);
-            bool drained = false;
-            for (uint32_t spin = 0; spin < kSpinLimit && !(drained = mbar_try_wait(drain_bar, 0)); ++spin) {}
-            if (!drained) atomicCAS(p.status, kStatusOk, kTimeoutDrain);
+            if (issuer) {
+                umma_commit(drain_bar);
+                bool drained = false;
+                for (uint32_t spin = 0; spin < kSpinLimit && !(drained = mbar_try_wait(drain_bar, 0)); ++spin) {}
+                if (!drained) atomicCAS(p.status, kStatusOk, kTimeoutDrain);
+            }
         }
         __syncwarp();
     } else if (Epi::kSumWarps != 0 && warp >= 2 + Epi::kWarps) {

@@ -200,7 +200,8 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
 
     if (warp == 0) {
         // ------------------------------------------------------------------ TMA producer (both CTAs)
-        if (lane == 0) {
+        {
+            const bool issuer = elect_one();
             uint32_t it = 0;
             bool ok = true;
             for (long long u = pair; u < num_units && ok; u += pairs) {
@@ -221,14 +222,15 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                         ok = false;
                         break;
                     }
+                    const uint32_t leader_full = map_to_cluster_rank(full_bar(s), 0);
+                    const uint32_t dst = ring + s * Cfg::kStageBytes;
+                    if (!issuer) continue;
                     if (leader) {
                         // the MMAs that read this stage -- in both CTAs -- have completed: tell the peer's producer (a plain
                         // remote arrive; a second tcgen05.commit per stage would cost the MMA issue stream ~50 ns each)
                         if (it >= (uint32_t)Cfg::kStages) mbar_arrive_cluster_relaxed(map_to_cluster_rank(empty_bar(s), 1));
                         mbar_expect_tx(full_bar(s), 2u * cta_bytes);  // both CTAs' loads land on this barrier
                     }
-                    const uint32_t leader_full = map_to_cluster_rank(full_bar(s), 0);
-                    const uint32_t dst = ring + s * Cfg::kStageBytes;
                     if constexpr (Epi::kTransA) {
                         // A stored [K, M]: this CTA's 128 rows of the tile as two boxes of 64 K-rows x 64 M (MN-major operand)
 #pragma unroll
@@ -252,9 +254,10 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------------------------ MMA issuer (leader CTA only)
-        if (lane == 0 && leader) {
-            uint32_t it = 0, local_tile = 0;
-            uint32_t stage = 0, phase = 0;  // ring position of K-block `it` and the parity of its fill
+        if (leader) {
+            const bool issuer = elect_one();
+            uint32_t local_tile = 0;
+            uint32_t stage = 0, phase = 0;  // ring position of the next K-block and the parity of its fill
             // descriptor words of the ring's first stage, stepped by 32-bit adds (see the single-CTA kernel)
             const uint32_t desc_hi = (uint32_t)(1024 >> 4) | (1u << 14) | (2u << 29);
             const uint32_t a_lo0 = ((ring & 0x3ffffu) >> 4) | (Epi::kTransA ? (uint32_t)(8192 >> 4) << 16 : 1u << 16);
@@ -279,22 +282,24 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                     if (!mbar_wait_remote(acc_free_bar(acc), acc_phase ^ 1u, abort_flag)) { ok = false; break; }
                     tc_fence_after();
                     const uint32_t d_tmem = tmem_base + acc * BN;
-                    for (int kb = k0; kb < k_end; ++kb, ++it) {
+                    for (int kb = k0; kb < k_end; ++kb) {
                         if (!mbar_wait(full_bar(stage), phase, abort_flag)) { ok = false; break; }
                         tc_fence_after();
                         const uint32_t a_lo = a_lo0 + stage * (uint32_t)(Cfg::kStageBytes >> 4), b_lo = b_lo0 + stage * (uint32_t)(Cfg::kStageBytes >> 4);
                         uint32_t accumulate = kb != k0 ? 1u : 0u;
+                        if (issuer) {
 #pragma unroll
-                        for (int k = 0; k < kBK / kUmmaK; ++k) {
-                            umma_f16_pair_words(d_tmem, a_lo + k * a_kstep, desc_hi, b_lo + k * b_kstep, desc_hi, idesc, accumulate);
-                            accumulate = 1u;
+                            for (int k = 0; k < kBK / kUmmaK; ++k) {
+                                umma_f16_pair_words(d_tmem, a_lo + k * a_kstep, desc_hi, b_lo + k * b_kstep, desc_hi, idesc, accumulate);
+                                accumulate = 1u;
+                            }
+                            // the stage is reusable once these MMAs have read it (in both CTAs: the commit tracks both SMs); the
+                            // leader's producer passes the release on to the peer
+                            umma_commit_pair(own_empty0 + 8u * stage);
                         }
-                        // the stage is reusable once these MMAs have read it (in both CTAs: the commit tracks both SMs); the
-                        // leader's producer passes the release on to the peer
-                        umma_commit_pair(own_empty0 + 8u * stage);
                         if (++stage == (uint32_t)Cfg::kStages) { stage = 0; phase ^= 1u; }
                     }
-                    if (ok) {
+                    if (ok && issuer) {
                         umma_commit_pair(own_ready0 + 8u * acc);
                         umma_commit_pair(peer_ready0 + 8u * acc);
                     }
@@ -305,10 +310,12 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                 *abort_flag = 1;
             }
             // nothing may still be reading the peer's shared memory or writing tensor memory when the pair parts
-            umma_commit_pair(map_to_cluster_rank(drain_bar, 0));
-            bool drained = false;
-            for (uint32_t spin = 0; spin < kSpinLimit && !(drained = mbar_try_wait(drain_bar, 0)); ++spin) {}
-            if (!drained) atomicCAS(p.status, kStatusOk, kTimeoutDrain);
+            if (issuer) {
+                umma_commit_pair(map_to_cluster_rank(drain_bar, 0));
+                bool drained = false;
+                for (uint32_t spin = 0; spin < kSpinLimit && !(drained = mbar_try_wait(drain_bar, 0)); ++spin) {}
+                if (!drained) atomicCAS(p.status, kStatusOk, kTimeoutDrain);
+            }
         }
         __syncwarp();
     } else if (Epi::kSumWarps != 0 && warp >= 2 + Epi::kWarps) {
