@@ -755,7 +755,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             tile_of(p, t, tiles_m, tiles_n, tm, tn);
             column_tile<BN>(p, tn, col0, bn);
             if constexpr (Epi::kFused) {  // the first chunk's operand arrives while the tile is still being computed
-                if (kTmaStore && split == 1) Epi::bring(fused, p, tm * kTileM + quad * 32, col0 + share * Epi::kChunk, lane);
+                if (kTmaStore && split == 1) Epi::bring(fused, p, tm * kTileM + quad * 32, col0 + share * Epi::kChunk);
                 if (!kTmaStore && split == 1) Epi::bring_rows(fused, p, tm * kTileM + quad * 32, col0 + share * Epi::kChunk, lane);
             }
             if constexpr (Epi::kPromote) {
@@ -807,7 +807,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             if (lane == 0) mbar_arrive(acc_free_bar(acc));
         }
         // shared memory must outlive the reads of the stores still in flight
-        if constexpr (Epi::kFused) Epi::finish(fused, lane);
+        if constexpr (Epi::kFused) Epi::finish(fused);
         else if (kTmaStore && lane == 0) bulk_wait_group_read<0>();
         __syncwarp();
     }

@@ -373,7 +373,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
             column_tile<BN>(p, tn, col0, bn);
             const int row_base = tm * kTileM + (int)rank * kBM + quad * 32;
             if constexpr (Epi::kFused)
-                if (split == 1) Epi::bring(fused, p, row_base, col0 + share * Epi::kChunk, lane);  // while the tile is being computed
+                if (split == 1) Epi::bring(fused, p, row_base, col0 + share * Epi::kChunk);  // while the tile is being computed
             if constexpr (Epi::kPromote) {
                 const int periods = (kb1 - kb0 + kPeriod - 1) / kPeriod;
                 ok = Epi::template promote<BN, true>(tmem_base + ((uint32_t)(quad * 32) << 16), share, periods, local_tile, acc_ready_bar(0),
@@ -411,7 +411,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(map_to_cluster_rank(acc_free_bar(acc), 0));
         }
-        if constexpr (Epi::kFused) Epi::finish(fused, lane);
+        if constexpr (Epi::kFused) Epi::finish(fused);
         else if (kTmaStore && lane == 0) bulk_wait_group_read<0>();
         __syncwarp();
     }

@@ -233,9 +233,9 @@ struct LinearEpilogue {
     }
 
     // the extra operand's chunk at (row_base, col) on its way into box 1
-    __device__ __forceinline__ static void bring(State &st, const Params &p, int row_base, int col, int lane) {
+    __device__ __forceinline__ static void bring(State &st, const Params &p, int row_base, int col) {
         if (p.extra == nullptr || row_base >= p.M || col >= p.N) return;
-        if (lane == 0) {
+        if (tc::elect_one()) {
             // a box is filled whole: what lies outside the matrix arrives as zeros and counts
             mbar_expect_tx(st.bar, kExtra16 && !kOut16 ? kBoxBytes / 2 : kBoxBytes);
             tc::tma_load_2d(st.boxes + kBoxBytes, &p.map_extra, col, row_base, st.bar);
@@ -286,10 +286,10 @@ struct LinearEpilogue {
     }
 
     // before the block leaves: nothing may still arrive in its shared memory or be read from it
-    __device__ __forceinline__ static void finish(State &st, int lane) {
+    __device__ __forceinline__ static void finish(State &st) {
         if (st.coming)
             for (uint32_t spin = 0; spin < kSpinLimit && !mbar_try_wait(st.bar, st.phase); ++spin) {}
-        if (lane == 0) tc::bulk_wait_group_read<0>();
+        if (tc::elect_one()) tc::bulk_wait_group_read<0>();
     }
 
 private:
@@ -450,19 +450,19 @@ private:
                       make_uint4(narrow<kBf16>(v[4 * j]), narrow<kBf16>(v[4 * j + 1]), narrow<kBf16>(v[4 * j + 2]), narrow<kBf16>(v[4 * j + 3])));
     }
     // the box D leaves from, free to be written: box 0 where box 1 belongs to the extra operand or to Z, else both in turn
-    __device__ __forceinline__ static uint32_t free_box(State &st, const Params &p, int lane) {
+    __device__ __forceinline__ static uint32_t free_box(State &st, const Params &p) {
         const bool turns = p.extra == nullptr && p.pre == nullptr;
-        if (lane == 0) {
+        if (tc::elect_one()) {
             if (turns) tc::bulk_wait_group_read<1>();
             else tc::bulk_wait_group_read<0>();
         }
         __syncwarp();
         return st.boxes + (turns ? (st.stores & 1u) * kBoxBytes : 0u);
     }
-    __device__ __forceinline__ static void send(State &st, const CUtensorMap *map, uint32_t box, int row_base, int col, int lane) {
+    __device__ __forceinline__ static void send(State &st, const CUtensorMap *map, uint32_t box, int row_base, int col) {
         fence_proxy_async();
         __syncwarp();
-        if (lane == 0) {
+        if (tc::elect_one()) {
             tc::tma_store_2d(map, col, row_base, box);  // rows and columns beyond the matrix are clipped by the map
             tc::bulk_commit_group();
         }
@@ -507,16 +507,16 @@ private:
         constexpr int kRow16 = kOut16 ? 128 : 64;  // bytes of a 16-bit tensor's box row
         const bool keep_z = kMode == LinearMode::kForward && p.pre != nullptr;
         if (keep_z && p.extra) {  // box 1 is taken: Z goes ahead through box 0, from a reading of the sums of its own
-            const uint32_t box = free_box(st, p, lane);
+            const uint32_t box = free_box(st, p);
 #pragma unroll 1
             for (int h = 0; h < kHalves; ++h) {
                 f32x2 v[16];
                 biased<kBf16>(p, taddr + h * 32, col + h * 32, v);
                 put16<kBf16, kRow16>(v, box, lane, h * 4);
             }
-            send(st, &p.map_pre, box, row_base, col, lane);
+            send(st, &p.map_pre, box, row_base, col);
         }
-        const uint32_t d_box = free_box(st, p, lane), z_box = st.boxes + kBoxBytes;
+        const uint32_t d_box = free_box(st, p), z_box = st.boxes + kBoxBytes;
         if constexpr (kOut16) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -524,7 +524,7 @@ private:
                 if (p.extra)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) extra[j] = get_piece(piece<128>(z_box, lane, h * 4 + j));
-                if (h == 1) next_extra(st, p, row_base, col, more, lane);
+                if (h == 1) next_extra(st, p, row_base, col, more);
                 f32x2 v[16];
                 biased<kBf16>(p, taddr + h * 32, col + h * 32, v);
                 if constexpr (kMode == LinearMode::kForward) {
@@ -593,20 +593,20 @@ private:
                     }
                 });
             }
-            next_extra(st, p, row_base, col, more, lane);
+            next_extra(st, p, row_base, col, more);
         }
         if (keep_z && !p.extra) {  // both boxes in one group of stores
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) tc::tma_store_2d(&p.map_pre, col, row_base, z_box);
+            if (tc::elect_one()) tc::tma_store_2d(&p.map_pre, col, row_base, z_box);
         }
-        send(st, map_d, d_box, row_base, col, lane);
+        send(st, map_d, d_box, row_base, col);
     }
     // the extra operand's box has been read: the next chunk's may come
-    __device__ __forceinline__ static void next_extra(State &st, const Params &p, int row_base, int col, bool more, int lane) {
+    __device__ __forceinline__ static void next_extra(State &st, const Params &p, int row_base, int col, bool more) {
         if (p.extra == nullptr) return;
         __syncwarp();
-        if (more) bring(st, p, row_base, col + kStep, lane);
+        if (more) bring(st, p, row_base, col + kStep);
     }
 };
 
