@@ -73,9 +73,22 @@ __global__ void __launch_bounds__(32 * kWarps) linear_few_tokens_kernel(const __
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) x_row[i] = static_cast<const uint16_t *>(q.X) + (size_t)min(i * 8 + g, p.M - 1) * p.K + t * 8;
     grid_launch_dependents();
+    // The previous kernel may still be running, and W may be what it writes: nothing is read yet, but a warp's first piece of W can
+    // be on its way into the L2 (1 x 4096 x 4096 9.3 -> 8.7 us, 1 x 14336 x 4096 25.3 -> 24.4).  Not where a cluster of four or
+    // eight shares few rows: the pieces are then most of K (4 x 1024 x 8192 6.1 -> 6.7), nor
+    // for 32 rows a block (32 x 8192 x 2048 13.2 either way).
+    const int first = (rank * kWarps + warp) * 32 * kChunks;
+    if (kSlabs == 1 && ranks <= 2 && t == 0)
+#pragma unroll
+        for (int c = 0; c < kChunks; c += 2)
+#pragma unroll
+            for (int s = 0; s < kSlabs; ++s)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (first + c * 32 < p.K) asm volatile("prefetch.global.L2 [%0];" ::"l"(w_row[s][h] + first + c * 32));
     grid_dependency_wait();
     const int stride = ranks * kWarps * 32 * kChunks;
-    for (int k0 = (rank * kWarps + warp) * 32 * kChunks; k0 < p.K; k0 += stride) {
+    for (int k0 = first; k0 < p.K; k0 += stride) {
         uint4 w[kChunks][kSlabs][2], x[kChunks][kTiles];
         const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
