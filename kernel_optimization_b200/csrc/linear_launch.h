@@ -85,11 +85,12 @@ inline int pin_product(const PinnedPlan &pin, int64_t M, int64_t N, int64_t K, b
 }
 
 // Tiles of a row of tiles that share the column sums of dY (see ColumnSums): one, whose sums are dbias, or four, whose parts
-// have to be added.  One that takes all K-blocks is 35 ns a K-block behind the others (16384 x 4096 x 1024: 111 us, four 104, without
-// the sums 102); adding parts is a launch, 1.3 us of the device (777 x 1000 x 520: one 9.5 us, four 10.8), where K is not cut anyway.
+// have to be added.  One that takes all K-blocks falls behind the others (a K-block's sums take longer than its MMAs in the 128 x 128
+// tile), adding parts is a launch, 1.2 us of the device, where K is not cut anyway.  One / four, without the sums (us): 777 tokens of
+// 1000 x 520 9.6 / 10.9, 9.5; 1024 tokens of 1024 x 1024 10.4 / 10.2, 8.7; 2048 tokens 16.7 / 14.2, 12.4; 16384 of 4096 x 1024 121 / 107, 105.
 inline int sum_shares(const ProductPlan &plan, int64_t N, int64_t K) {
     const long long tiles_n = (N + plan.bn - 1) / plan.bn, unit_blocks = ((K + tc::kBK - 1) / tc::kBK + plan.split - 1) / plan.split;
-    return unit_blocks < 64 ? 1 : (int)std::min<long long>(tiles_n, 4);
+    return unit_blocks < 32 ? 1 : (int)std::min<long long>(tiles_n, 4);
 }
 inline size_t sum_bytes(const ProductPlan &plan, int64_t M, int64_t N, int64_t K) {
     return (size_t)sum_shares(plan, N, K) * plan.split * (size_t)M * sizeof(float);
@@ -205,9 +206,9 @@ int run_product(LinearParams p, const void *A, const void *B, void *workspace, s
         if (p.extra)
             if (int st = make_store_map(encode, &p.map_extra, Epi::kExtra16 ? p.fmt + 1 : 0, const_cast<void *>(p.extra), p.M, p.N, Epi::kChunk)) return st;
     }
-    // FP32 results of more than two periods of K a work unit: partial sums are promoted (see LinearEpilogue)
+    // FP32 results of more than 1024 values of K a work unit: partial sums are promoted (see LinearEpilogue)
     const long long unit_blocks = ((p.K + tc::kBK - 1) / tc::kBK + plan.split - 1) / plan.split;
-    const bool promote = !kOut16 && unit_blocks > 2 * tc::kPeriod;
+    const bool promote = !kOut16 && unit_blocks > 16;
     int st = KO_OK;
     if constexpr (!kOut16) {
         if (promote) st = launch_product<LinearEpilogue<kMode, false, true>>(plan, tma, map_a, map_b, map_d, p, info.sm_count, s);

@@ -49,7 +49,7 @@ constexpr int kBM = 128;          // rows of D per tile = TMEM lanes
 constexpr int kBK = 64;           // K elements per stage: 64 * 2 B = one 128-byte swizzle row
 constexpr int kUmmaK = 16;        // K per tcgen05.mma for 16-bit inputs
 constexpr int kThreads = 192;     // 6 warps: producer, MMA, 4 x epilogue
-constexpr int kPeriod = 32;       // K-blocks per accumulator where partial sums are promoted (2048 values of K)
+constexpr int kPeriod = 14;       // K-blocks per accumulator where partial sums are promoted (896 values of K)
 
 // codes written to the status word (first failure wins)
 enum : unsigned { kStatusOk = 0, kTimeoutProducer = 1, kTimeoutMma = 2, kTimeoutEpilogue = 3, kTimeoutDrain = 4 };

@@ -88,6 +88,10 @@ __global__ void __launch_bounds__(32 * kWarps) linear_few_tokens_kernel(const __
                     if (first + c * 32 < p.K) asm volatile("prefetch.global.L2 [%0];" ::"l"(w_row[s][h] + first + c * 32));
     grid_dependency_wait();
     const int stride = ranks * kWarps * 32 * kChunks;
+    // An FP32 result is not to show how the matrix instructions cut their accumulators off (see LinearEpilogue): every 1024 values of
+    // K a warp adds them to sums of its own.
+    float sum[kOut16 ? 1 : kSlabs][kOut16 ? 1 : kTiles][4] = {};
+    int pieces = 0;
     for (int k0 = first; k0 < p.K; k0 += stride) {
         uint4 w[kChunks][kSlabs][2], x[kChunks][kTiles];
         const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
@@ -111,13 +115,28 @@ __global__ void __launch_bounds__(32 * kWarps) linear_few_tokens_kernel(const __
                     mma_16x8x16<kBf16>(acc[s][i], w[c][s][0].x, w[c][s][1].x, w[c][s][0].y, w[c][s][1].y, x[c][i].x, x[c][i].y);
                     mma_16x8x16<kBf16>(acc[s][i], w[c][s][0].z, w[c][s][1].z, w[c][s][0].w, w[c][s][1].w, x[c][i].z, x[c][i].w);
                 }
+        if constexpr (!kOut16) {
+            if (++pieces == 1024 / (32 * kChunks)) {
+                pieces = 0;
+#pragma unroll
+                for (int s = 0; s < kSlabs; ++s)
+#pragma unroll
+                    for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            sum[s][i][e] += acc[s][i][e];
+                            acc[s][i][e] = 0.f;
+                        }
+            }
+        }
     }
 #pragma unroll
     for (int s = 0; s < kSlabs; ++s)
 #pragma unroll
         for (int i = 0; i < kTiles; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) part[warp][s * 16 + (e >> 1) * 8 + g][i * 8 + 2 * t + (e & 1)] = acc[s][i][e];
+            for (int e = 0; e < 4; ++e)
+                part[warp][s * 16 + (e >> 1) * 8 + g][i * 8 + 2 * t + (e & 1)] = kOut16 ? acc[s][i][e] : sum[s * !kOut16][i * !kOut16][e] + acc[s][i][e];
     __syncthreads();
     // element i of the block: token i / kRows, W row i % kRows (stores of a token's outputs are then contiguous)
     for (int i = threadIdx.x; i < kRows * kCols; i += 32 * kWarps) {
