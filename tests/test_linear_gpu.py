@@ -383,6 +383,44 @@ def test_guards_and_unaligned_outputs(cuda, lib, ko):
         assert lib.ko_poll_device_status() == 0
 
 
+@pytest.mark.parametrize("m,n,k", [(700, 520, 1024), (700, 520, 1096), (2048, 4104, 2048), (2049, 4101, 4096), (130, 2056, 6904)])
+def test_fp32_results_of_middling_sums(cuda, lib, ko, m, n, k):
+    """As above: up to 1024 values of K in one accumulator (64 instructions), beyond that in periods of at most as many, in one tile a
+    CTA and in several, stored by TMA and row by row.  One accumulator over 4096 values would be off by 4.5e-6."""
+    bound = 64 * 2.0 ** -24 + (k / 896 + 1) * 2.0 ** -24
+    x, w = _randn(cuda, (m, k), cuda.float16, 1), _randn(cuda, (n, k), cuda.float16, 2)
+    want = x.double() @ w.double().t()
+    got = ko.linear(x, w, out_dtype=cuda.float32)
+    assert ((got.double() - want).norm() / want.norm()).item() <= bound
+    if n % 8 == 0:
+        got = ko.linear_backward_input(x, w.t().contiguous(), out_dtype=cuda.float32)
+        assert ((got.double() - want).norm() / want.norm()).item() <= bound
+    assert lib.ko_poll_device_status() == 0
+
+
+@pytest.mark.parametrize("tile,slices", [(128, 0), (128, 2), (256, 0), (256, 2), (2048, 0), (2048, 2), (0, 0)])
+@pytest.mark.parametrize("tokens", [130, 2100, 8200])
+def test_bias_gradient_of_every_plan(cuda, lib, ko, tile, slices, tokens):
+    """The column sums' way through every tile, alone or shared by tiles, with and without K slices; a workspace full of NaN."""
+    import ctypes as C
+
+    n, k, dt = 264, 1032, cuda.bfloat16
+    dy, x = _randn(cuda, (tokens, n), dt, 1), _randn(cuda, (tokens, k), dt, 2)
+    tiles = -(-n // 128) * -(-k // 128)
+    need = C.c_size_t(max(slices, 1) * (tiles * 2 * 128 * 256 + 4 * n) * 4)
+    if tile == 0:
+        assert lib.ko_linear_backward_weight_workspace(tokens, n, k, C.byref(need)) == 0
+    ws = cuda.full((need.value // 4,), float("nan"), device="cuda")
+    for out_fmt, odt in ((0, cuda.float32), (2, dt)):
+        dw, db = cuda.full((n, k), float("nan"), dtype=odt, device="cuda"), cuda.full((n,), float("nan"), device="cuda")
+        assert lib.ko_linear_backward_weight_tuned(1, out_fmt, tokens, n, k, dy.data_ptr(), x.data_ptr(), None, dw.data_ptr(), db.data_ptr(), ws.data_ptr(),
+                                                   ws.numel() * 4, tile, slices, cuda.cuda.current_stream().cuda_stream) == 0, lib.ko_last_error_string()
+        _close(cuda, dw, dy.double().t() @ x.double(), _sum_error(dy.t(), x, tokens), "dw")
+        # 16 rows added one by one, then a block's sums: at most 16 + tokens / 64 + 8 roundings on the way of a value
+        _close(cuda, db, dy.double().sum(0), (tokens / 64 + 24) * 2.0 ** -24 * dy.double().abs().sum(0), "db")
+    assert lib.ko_poll_device_status() == 0
+
+
 def test_streams_and_graphs(cuda, lib, ko):
     """Other streams, and two graphs with K slices captured on one stream and replayed side by side."""
     dt = cuda.bfloat16
