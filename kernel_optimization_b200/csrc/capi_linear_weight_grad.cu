@@ -25,6 +25,8 @@ int dispatch(int in_fmt, int out_fmt, int64_t M, int64_t N, int64_t K, const voi
     KO_REQUIRE(ko::aligned_to(dW, out_fmt ? 2 : 4) && ko::aligned_to(C, out_fmt ? 2 : 4) && ko::aligned_to(dbias, 4), KO_ERR_ALIGN,
                "%s: an operand is not aligned to its element", name);
     KO_REQUIRE(K == 0 || (dW != dY && dW != X && (const void *)dbias != dW), KO_ERR_INVALID_ARG, "%s: outputs must not alias the inputs or each other", name);
+    KO_REQUIRE(dbias == nullptr || ((const void *)dbias != dY && (K == 0 || ((const void *)dbias != X && (const void *)dbias != C))), KO_ERR_INVALID_ARG,
+               "%s: dbias must not alias an input", name);
     ko::DeviceInfo info;
     if (int st = ko::current_device_info(&info)) return st;
     ko::LinearParams p = {};

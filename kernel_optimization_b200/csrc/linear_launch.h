@@ -92,8 +92,9 @@ inline int sum_shares(const ProductPlan &plan, int64_t N, int64_t K) {
     const long long tiles_n = (N + plan.bn - 1) / plan.bn, unit_blocks = ((K + tc::kBK - 1) / tc::kBK + plan.split - 1) / plan.split;
     return unit_blocks < 32 ? 1 : (int)std::min<long long>(tiles_n, 4);
 }
-inline size_t sum_bytes(const ProductPlan &plan, int64_t M, int64_t N, int64_t K) {
-    return (size_t)sum_shares(plan, N, K) * plan.split * (size_t)M * sizeof(float);
+inline size_t sum_bytes(const ProductPlan &plan, int64_t M, int64_t N, int64_t K) {  // room for their parts; a single one is dbias
+    const size_t parts = (size_t)sum_shares(plan, N, K) * plan.split;
+    return parts > 1 ? parts * (size_t)M * sizeof(float) : 0;
 }
 
 // room for whatever plan a call of this shape may take: with or without TMA, any operands, column sums
@@ -174,8 +175,9 @@ int run_product(LinearParams p, const void *A, const void *B, void *workspace, s
     ProductPlan plan = plan_product(p.M, p.N, p.K, tma, element_bytes, info.sm_count);
     if (int st = pin_product(pin, p.M, p.N, p.K, tma, name, &plan)) return st;
     p.sum_shares = p.dbias ? sum_shares(plan, p.N, p.K) : 0;
-    const bool fold = p.sum_shares * plan.split > 1;
-    const size_t bytes = plan.bytes() + (fold ? sum_bytes(plan, p.M, p.N, p.K) : 0);
+    const size_t parts_bytes = p.dbias ? sum_bytes(plan, p.M, p.N, p.K) : 0;
+    const bool fold = parts_bytes != 0;
+    const size_t bytes = plan.bytes() + parts_bytes;
     KO_REQUIRE(bytes == 0 || (workspace != nullptr && workspace_bytes >= bytes), KO_ERR_INVALID_ARG,
                "%s: the workspace needs %zu bytes, got %zu", name, bytes, workspace ? workspace_bytes : (size_t)0);
     KO_REQUIRE(aligned16(workspace), KO_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", name);

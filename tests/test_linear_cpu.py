@@ -35,6 +35,7 @@ def test_backward_arguments(lib):
     assert dw(fmt=3) == 1 and dw(out=1) == 1 and dw(n=4) == 3 and dw(k=4) == 3 and dw(m=-1) == 1
     assert dw(dy=None) == 1 and dw(x=None) == 1 and dw(w=None) == 1 and dw(dy=P + 2) == 2 and dw(w=3 * P + 2) == 2 and dw(c=3 * P + 2) == 2
     assert dw(w=P) == 1 and dw(w=2 * P) == 1 and dw(b=3 * P) == 1 and dw(b=P + 2) == 2
+    assert dw(b=P) == 1 and dw(b=2 * P) == 1 and dw(c=4 * P, b=4 * P) == 1 and dw(k=0, b=P) == 1 and b"dbias" in lib.ko_last_error_string()
     assert dw(n=0) == 0
 
 
