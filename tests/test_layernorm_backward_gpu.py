@@ -215,6 +215,20 @@ def test_either_vector_may_be_left_out(cuda, lib):
         assert cuda.equal(dbeta, outs[0][2]) if b_wanted else bool((dbeta == -7).all())
 
 
+@pytest.mark.parametrize("rows,cols", [(540_000, 4096), (540_000, 4097), (270_000, 8200)])
+def test_offsets_past_32_bits(cuda, lib, ko, rows, cols):
+    """More than 2^31 elements a tensor (one pass, single elements, two passes): zeros but for the last rows, which are checked."""
+    a = _inputs(cuda, cuda.bfloat16, 70, cols, residual=True, seed=1)
+    big = {name: cuda.zeros(rows, cols, dtype=cuda.bfloat16, device="cuda") for name in ("dy", "x", "residual")}
+    for name, t in big.items():
+        assert t.numel() > 2 ** 31
+        t[-70:] = a[name]
+    dx, dgamma, dbeta = ko.layernorm_backward(big["dy"], big["x"], 1e-5, a["gamma"], residual=big["residual"], dx=big["dy"])
+    want, scale = _reference(cuda, a["dy"], a["x"], 1e-5, a["gamma"], residual=a["residual"])
+    _check(cuda, (dx[-70:], dgamma, dbeta), want, scale, cuda.bfloat16)
+    assert not dx[:-70].any() and lib.ko_poll_device_status() == 0
+
+
 def test_streams_and_graphs(cuda, lib, ko):
     """On another stream by context and by handle; two graphs captured on one stream and replayed side by side."""
     a, b = _inputs(cuda, cuda.bfloat16, 900, 1024, seed=1), _inputs(cuda, cuda.bfloat16, 900, 1024, seed=2)

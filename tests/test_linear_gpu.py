@@ -287,7 +287,7 @@ def test_no_input_features(cuda, ko):
 
 
 def test_bias_gradient_of_a_large_batch(cuda, ko):
-    """dY beyond the size up to which its column sums run beside the product."""
+    """A dY of more than half the L2, and its column sums."""
     dy, x = _randn(cuda, (6500, 4104), cuda.float16, 1, 0.1), _randn(cuda, (6500, 72), cuda.float16, 2)
     dw, db = ko.linear_backward_weight(dy, x)
     _close(cuda, dw, dy.double().t() @ x.double(), _sum_error(dy.t(), x, 6500), "dw")
@@ -418,6 +418,29 @@ def test_bias_gradient_of_every_plan(cuda, lib, ko, tile, slices, tokens):
         _close(cuda, dw, dy.double().t() @ x.double(), _sum_error(dy.t(), x, tokens), "dw")
         # 16 rows added one by one, then a block's sums: at most 16 + tokens / 64 + 8 roundings on the way of a value
         _close(cuda, db, dy.double().sum(0), (tokens / 64 + 24) * 2.0 ** -24 * dy.double().abs().sum(0), "db")
+    assert lib.ko_poll_device_status() == 0
+
+
+@pytest.mark.parametrize("n", [4096, 4097])
+def test_offsets_past_32_bits(cuda, lib, ko, n):
+    """More than 2^31 elements of Y, Z and dX (stored by TMA, and row by row) and of dY: the last rows are checked."""
+    m, k, dt = 540_000, 64, cuda.bfloat16
+    x, w, b = _randn(cuda, (m, k), dt, 1), _randn(cuda, (n, k), dt, 2, k ** -0.5), _randn(cuda, (n,), dt, 3)
+    y, z = ko.linear(x, w, b, "relu", return_pre=True)
+    assert y.numel() > 2 ** 31
+    for rows in (slice(0, 70), slice(m - 70, m)):
+        want = x[rows].double() @ w.double().t() + b.double()
+        err = _sum_error(x[rows], w.t(), k) + 2.0 ** -24 * want.abs()
+        _close(cuda, z[rows], want, err, "z")
+        _close(cuda, y[rows], want.clamp(min=0), err, "y")
+    if n % 8 == 0:
+        dx = ko.linear_backward_input(x, w.t().contiguous(), z, "relu", out=y)
+        rows = slice(m - 70, m)
+        _close(cuda, dx[rows], (x[rows].double() @ w.double().t()) * (z[rows] > 0), _sum_error(x[rows], w.t(), k), "dx")
+        y[:-70].zero_()
+        dw, db = ko.linear_backward_weight(y, x)
+        _close(cuda, dw, y[rows].double().t() @ x[rows].double(), _sum_error(y[rows].t(), x[rows], m), "dw")
+        _close(cuda, db, y[rows].double().sum(0), (m / 8 + 64) * 2.0 ** -24 * y[rows].double().abs().sum(0), "db")
     assert lib.ko_poll_device_status() == 0
 
 
