@@ -225,7 +225,7 @@ def test_no_tokens(cuda, ko):
 @pytest.mark.parametrize("n,k", [(256, 512), (1032, 264), (2048, 2048)])
 def test_fp32_results_of_long_sums(cuda, lib, ko, n, k):
     """Tensor cores cut an accumulator off at every addition: up to 2^-23 of it per instruction (16 terms), half of that on
-    average, always towards zero.  Sums kept in FP32 are therefore taken in periods of 2048 terms, 128 instructions, and the
+    average, always towards zero.  Sums kept in FP32 are therefore taken in periods of at most 2048 terms, 128 instructions, and the
     periods' sums added with rounding: off by 128 * 2^-24 plus half a step per period, relative to the sums' size (2-norm over
     all results, whose partial sums are no larger than the results on the whole).  A single accumulator over all 16384 terms
     is off by 1.9e-5."""
