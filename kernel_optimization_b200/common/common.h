@@ -358,6 +358,11 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     }
     return false;
 }
+// A whole warp's word on what each of its lanes saw: true where all of them say so.  For waits that a warp takes together while one
+// of its lanes issues: parities tell two neighbouring phases apart, so a lane that is still polling when the others have sent a
+// barrier two phases on would wait for a phase that is over.  Here the warp meets again after every wait: no lane releases a
+// stage before all have seen it filled (or free), and when a wait runs out all of them take the same branch.
+__device__ __forceinline__ bool warp_all(bool seen) { return __all_sync(kFullMask, seen) != 0; }
 __device__ __forceinline__ void fence_barrier_init() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 

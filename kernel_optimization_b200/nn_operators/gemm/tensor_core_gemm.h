@@ -598,7 +598,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     const int s = (int)stage;
                     const uint32_t phase = fill & 1u;
                     if (++stage == (uint32_t)Cfg::kStages) { stage = 0; ++fill; }
-                    if (!mbar_wait(empty_bar(s), phase ^ 1u, abort_flag)) {
+                    if (!warp_all(mbar_wait(empty_bar(s), phase ^ 1u, abort_flag))) {
                         if (!*abort_flag) atomicCAS(p.status, kStatusOk, kTimeoutProducer);
                         *abort_flag = 1;
                         ok = false;
@@ -664,11 +664,11 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                     if (k0 != kb0) ++local_tile;
                     const int k_end = Epi::kPromote ? min(k0 + period, kb1) : kb1;
                     const uint32_t acc = MT == 1 ? (local_tile & 1u) : 0u, acc_phase = (MT == 1 ? (local_tile >> 1) : local_tile) & 1u;
-                    if (!mbar_wait(acc_free_bar(acc), acc_phase ^ 1u, abort_flag)) { ok = false; break; }
+                    if (!warp_all(mbar_wait(acc_free_bar(acc), acc_phase ^ 1u, abort_flag))) { ok = false; break; }
                     tc_fence_after();
                     const uint32_t d_tmem = tmem_base + acc * BN;
                     for (int kb = k0; kb < k_end; ++kb) {
-                        if (!mbar_wait(full_bar(stage), phase, abort_flag)) { ok = false; break; }
+                        if (!warp_all(mbar_wait(full_bar(stage), phase, abort_flag))) { ok = false; break; }
                         tc_fence_after();
                         // descriptors of this stage: the ring's plus the stage's offset in 16-byte units
                         const uint32_t a_lo = a_lo0 + stage * (uint32_t)(Cfg::kStageBytes >> 4), b_lo = b_lo0 + stage * (uint32_t)(Cfg::kStageBytes >> 4);
@@ -718,7 +718,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 typename Epi::Sums sums;
                 int next = kb0 + (tn - kb0 % p.sum_shares + p.sum_shares) % p.sum_shares;  // the next K-block that this tile adds
                 for (int kb = kb0; kb < kb1; ++kb) {
-                    if (!mbar_wait(full_bar(stage), phase, abort_flag)) { ok = false; break; }
+                    if (!warp_all(mbar_wait(full_bar(stage), phase, abort_flag))) { ok = false; break; }
                     if (mine && kb == next) {
                         sums.add(p, ring + stage * (uint32_t)Cfg::kStageBytes + box * 8192u, lane);
                         next += p.sum_shares;
@@ -765,7 +765,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 local_tile += (uint32_t)periods - 1;  // the accumulator that holds the sums
             }
             const uint32_t acc = MT == 1 ? (local_tile & 1u) : 0u, acc_phase = (MT == 1 ? (local_tile >> 1) : local_tile) & 1u;
-            if (!ok || (!Epi::kPromote && !mbar_wait(acc_ready_bar(acc), acc_phase, abort_flag))) {
+            if (!ok || (!Epi::kPromote && !warp_all(mbar_wait(acc_ready_bar(acc), acc_phase, abort_flag)))) {
                 if (lane == 0 && !*abort_flag) atomicCAS(p.status, kStatusOk, kTimeoutEpilogue);
                 *abort_flag = 1;
                 ok = false;

@@ -216,7 +216,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                 for (int kb = kb0; kb < kb1; ++kb, ++it) {
                     const int s = it % Cfg::kStages;
                     const uint32_t phase = (it / Cfg::kStages) & 1u;
-                    if (!mbar_wait(empty_bar(s), phase ^ 1u, abort_flag)) {
+                    if (!warp_all(mbar_wait(empty_bar(s), phase ^ 1u, abort_flag))) {
                         if (!*abort_flag) atomicCAS(p.status, kStatusOk, kTimeoutProducer);
                         *abort_flag = 1;
                         ok = false;
@@ -279,11 +279,11 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                     if (k0 != kb0) ++local_tile;
                     const int k_end = Epi::kPromote ? min(k0 + period, kb1) : kb1;
                     const uint32_t acc = local_tile & 1u, acc_phase = (local_tile >> 1) & 1u;
-                    if (!mbar_wait_remote(acc_free_bar(acc), acc_phase ^ 1u, abort_flag)) { ok = false; break; }
+                    if (!warp_all(mbar_wait_remote(acc_free_bar(acc), acc_phase ^ 1u, abort_flag))) { ok = false; break; }
                     tc_fence_after();
                     const uint32_t d_tmem = tmem_base + acc * BN;
                     for (int kb = k0; kb < k_end; ++kb) {
-                        if (!mbar_wait(full_bar(stage), phase, abort_flag)) { ok = false; break; }
+                        if (!warp_all(mbar_wait(full_bar(stage), phase, abort_flag))) { ok = false; break; }
                         tc_fence_after();
                         const uint32_t a_lo = a_lo0 + stage * (uint32_t)(Cfg::kStageBytes >> 4), b_lo = b_lo0 + stage * (uint32_t)(Cfg::kStageBytes >> 4);
                         uint32_t accumulate = kb != k0 ? 1u : 0u;
@@ -336,7 +336,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                     // The pair's loads complete on the leader's barrier; its first sum warp passes the word on.  A token (relaxed):
                     // what the peer's sum warps read came into their own SM's shared memory before the leader's barrier heard of
                     // it.  A releasing arrive took 0.7 us a K-block longer, which the whole ring then waited for.
-                    if (!mbar_wait_remote(leader ? full_bar(stage) : arrived_bar(stage), phase, abort_flag)) { ok = false; break; }
+                    if (!warp_all(mbar_wait_remote(leader ? full_bar(stage) : arrived_bar(stage), phase, abort_flag))) { ok = false; break; }
                     if (leader && box == 0 && lane == 0) mbar_arrive_cluster_relaxed(map_to_cluster_rank(arrived_bar(stage), 1));
                     if (mine && kb == next) {
                         sums.add(p, ring + stage * (uint32_t)Cfg::kStageBytes + box * 8192u, lane);
@@ -381,7 +381,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                 local_tile += (uint32_t)periods - 1;  // the accumulator that holds the sums
             }
             const uint32_t acc = local_tile & 1u, acc_phase = (local_tile >> 1) & 1u;
-            if (!ok || (!Epi::kPromote && !mbar_wait(acc_ready_bar(acc), acc_phase, abort_flag))) {
+            if (!ok || (!Epi::kPromote && !warp_all(mbar_wait(acc_ready_bar(acc), acc_phase, abort_flag)))) {
                 if (lane == 0 && !*abort_flag) atomicCAS(p.status, kStatusOk, kTimeoutEpilogue);
                 *abort_flag = 1;
                 ok = false;

@@ -278,7 +278,7 @@ layernorm_backward_resident_kernel(const LayerNormBackwardArgs<T> a, int stages,
             load(a.x + (size_t)r * a.cols, x);
             load(a.dy + (size_t)r * a.cols, dy);
         } else {
-            if (!mbar_wait(smem_u32(full + stage), phase, &abort_flag)) give_up(2u);
+            if (!warp_all(mbar_wait(smem_u32(full + stage), phase, &abort_flag))) give_up(2u);
             staged(here, there, x);
             staged(here + tensor_bytes, there, dy);
         }
@@ -297,7 +297,7 @@ layernorm_backward_resident_kernel(const LayerNormBackwardArgs<T> a, int stages,
         // the stage of the step before: by now every warp of this row is done with it
         if (!kSingles && threadIdx.x < 32 && step > 0 && step - 1 + stages < steps) {
             const uint32_t before = stage ? stage - 1 : (uint32_t)stages - 1;
-            if (!mbar_wait(smem_u32(empty + before), stage ? phase : phase ^ 1u, &abort_flag)) give_up(3u);
+            if (!warp_all(mbar_wait(smem_u32(empty + before), stage ? phase : phase ^ 1u, &abort_flag))) give_up(3u);
             else bring(r - slot + (stages - 1) * stride, before);
         }
         const float mean = sum_x * inv_n;

@@ -203,7 +203,7 @@ struct LinearEpilogue {
         f32x2 sums[kChunks][16];
         for (uint32_t n = first; n < first + (uint32_t)periods; ++n) {
             const uint32_t acc = n & 1u, t_row = t_rows + acc * BN + share * 32;
-            if (!mbar_wait(ready + 8u * acc, (n >> 1) & 1u, abort_flag)) return false;
+            if (!warp_all(mbar_wait(ready + 8u * acc, (n >> 1) & 1u, abort_flag))) return false;
             tc::tc_fence_after();
             const bool last = n + 1 == first + (uint32_t)periods;
 #pragma unroll
@@ -256,7 +256,7 @@ struct LinearEpilogue {
             if (row_base >= p.M || col0 + c0 >= p.N) break;
             if constexpr (kTmaStore) {
                 if (st.coming) {
-                    if (!mbar_wait(st.bar, st.phase, abort_flag)) return false;
+                    if (!warp_all(mbar_wait(st.bar, st.phase, abort_flag))) return false;
                     st.phase ^= 1u;
                     st.coming = false;
                 }
