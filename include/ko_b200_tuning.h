@@ -73,7 +73,7 @@ int ko_gemm_tc_tuned(int fmt, int out_fmt, int b_row_major, int64_t M, int64_t N
                      const void *C, void *D, int bn, int store_mode, void *stream);
 
 /* the linear layer's calls with a pinned plan: tile 0 = choose, 128 / 256 = columns of D per 128-row tile of one CTA, 2048 = a
- * pair of CTAs per 256 x 256 tile (both only where D can be stored by TMA); slices: with a pinned tile, K slices (0 / 1 = none,
+ * pair of CTAs per 256 x 256 tile (both only where D can be stored by TMA; the pair with dbias only where K > 256); slices: with a pinned tile, K slices (0 / 1 = none,
  * at most 64), for which the workspace must hold slices * tiles * their elements floats, and for dbias 4 * max(slices, 1) * N floats
  * more; a pinned tile also takes the forward call past the few-token kernel */
 int ko_linear_tuned(int in_fmt, int out_fmt, int activation, int64_t M, int64_t N, int64_t K, const void *X, const void *W,

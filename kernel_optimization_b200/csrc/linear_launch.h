@@ -33,7 +33,8 @@ struct ProductPlan {
 // (14.5), 20.2 (16.1); 1024 x 1024 x 4096 26 (27), 19.8 (18.3), 33 (28), 128 x 128 in two slices 20.2 (20.7).  Slices, where a few
 // tiles leave most SMs idle: 512 x 2048 x 32768 (a weight gradient) pair in four 65 (61), 128 x 256 in four 77 (65), uncut 156 (171);
 // 768 x 768 x 16384 128 x 128 in four 24.5, uncut 53.
-inline ProductPlan plan_product(int64_t M, int64_t N, int64_t K, bool tma, int element_bytes, int sms) {
+// sums: column sums are wanted, which a pair can take where a row of tiles has two (see sum_shares).
+inline ProductPlan plan_product(int64_t M, int64_t N, int64_t K, bool tma, int element_bytes, int sms, bool sums) {
     const long long k_blocks = (K + tc::kBK - 1) / tc::kBK;
     ProductPlan best{false, 128, 1, 0};
     double best_cost = 1e300;
@@ -43,7 +44,7 @@ inline ProductPlan plan_product(int64_t M, int64_t N, int64_t K, bool tma, int e
         double start, per_block, once, per_byte;  // us: a launch, a K-block, an epilogue and each byte of its elements
     };
     for (const Tile &tile : {Tile{true, 256, 4.5, 0.32, 0.3, 0.7}, Tile{false, 128, 3.0, 0.22, 0.5, 0.35}, Tile{false, 256, 4.3, 0.35, 0.5, 0.6}}) {
-        if (tile.bn == 256 && (!tma || N <= 128 || (tile.pair && M <= 128))) continue;
+        if (tile.bn == 256 && (!tma || N <= 128 || (tile.pair && (M <= 128 || (sums && N <= 256))))) continue;
         const int rows = tile.pair ? 256 : 128, bn = tile.bn, at_once = tile.pair ? sms / 2 : sms;
         const double per_block = tile.per_block, start = tile.start;
         const auto per_tile = [&](int bytes) { return tile.once + tile.per_byte * bytes; };
@@ -70,10 +71,11 @@ inline ProductPlan plan_product(int64_t M, int64_t N, int64_t K, bool tma, int e
 struct PinnedPlan {
     int tile = 0, slices = 0;
 };
-inline int pin_product(const PinnedPlan &pin, int64_t M, int64_t N, int64_t K, bool tma, const char *name, ProductPlan *plan) {
+inline int pin_product(const PinnedPlan &pin, int64_t M, int64_t N, int64_t K, bool tma, bool sums, const char *name, ProductPlan *plan) {
     if (pin.tile == 0 && pin.slices == 0) return KO_OK;
     KO_REQUIRE(pin.tile == 128 || pin.tile == 256 || pin.tile == 2048, KO_ERR_INVALID_ARG, "%s: tile code %d not in {128,256,2048}", name, pin.tile);
     KO_REQUIRE(tma || pin.tile == 128, KO_ERR_SHAPE, "%s: without TMA stores there is only the 128-column tile", name);
+    KO_REQUIRE(pin.tile != 2048 || !sums || N > 256, KO_ERR_SHAPE, "%s: a pair of CTAs sums the columns of dY only where dW has more than 256", name);
     const long long k_blocks = (K + tc::kBK - 1) / tc::kBK;
     KO_REQUIRE(pin.slices >= 0 && pin.slices <= 64 && pin.slices <= k_blocks, KO_ERR_INVALID_ARG,
                "%s: %d K slices out of range", name, pin.slices);
@@ -88,9 +90,11 @@ inline int pin_product(const PinnedPlan &pin, int64_t M, int64_t N, int64_t K, b
 // have to be added.  One that takes all K-blocks falls behind the others (a K-block's sums take longer than its MMAs in the 128 x 128
 // tile), adding parts is a launch, 1.2 us of the device, where K is not cut anyway.  One / four, without the sums (us): 777 tokens of
 // 1000 x 520 9.6 / 10.9, 9.5; 1024 tokens of 1024 x 1024 10.4 / 10.2, 8.7; 2048 tokens 16.7 / 14.2, 12.4; 16384 of 4096 x 1024 121 / 107, 105.
+// Of a pair of CTAs only the leader adds, the upper rows of its tile in even columns of tiles and the lower ones in odd columns: two
+// columns of tiles for every share.
 inline int sum_shares(const ProductPlan &plan, int64_t N, int64_t K) {
     const long long tiles_n = (N + plan.bn - 1) / plan.bn, unit_blocks = ((K + tc::kBK - 1) / tc::kBK + plan.split - 1) / plan.split;
-    return unit_blocks < 32 ? 1 : (int)std::min<long long>(tiles_n, 4);
+    return unit_blocks < 32 ? 1 : (int)std::min<long long>(plan.pair ? tiles_n / 2 : tiles_n, 4);
 }
 inline size_t sum_bytes(const ProductPlan &plan, int64_t M, int64_t N, int64_t K) {  // room for their parts; a single one is dbias
     const size_t parts = (size_t)sum_shares(plan, N, K) * plan.split;
@@ -102,10 +106,11 @@ inline size_t product_workspace(int64_t M, int64_t N, int64_t K, int sms, bool s
     if (M == 0 || N == 0 || K == 0) return 0;
     size_t most = 0;
     for (int element_bytes = 2; element_bytes <= 10; element_bytes += 2)
-        for (bool tma : {true, false}) {
-            const ProductPlan plan = plan_product(M, N, K, tma, element_bytes, sms);
-            most = std::max(most, plan.bytes() + (sums ? sum_bytes(plan, M, N, K) : 0));
-        }
+        for (bool tma : {true, false})
+            for (int with = 0; with <= (sums ? 1 : 0); ++with) {
+                const ProductPlan plan = plan_product(M, N, K, tma, element_bytes, sms, with);
+                most = std::max(most, plan.bytes() + (with ? sum_bytes(plan, M, N, K) : 0));
+            }
     return most;
 }
 
@@ -172,8 +177,8 @@ int run_product(LinearParams p, const void *A, const void *B, void *workspace, s
     const bool sixteen = kOut16 || p.pre || p.bias || (p.extra && Epi::kExtra16);
     const bool tma = p.N % (sixteen ? 8 : 4) == 0 && aligned16(p.D) && aligned16(p.pre) && aligned16(p.bias) && aligned16(p.extra);
     const int element_bytes = (kOut16 ? 2 : 4) + (p.pre ? 2 : 0) + (p.extra ? (Epi::kExtra16 ? 2 : 4) : 0);
-    ProductPlan plan = plan_product(p.M, p.N, p.K, tma, element_bytes, info.sm_count);
-    if (int st = pin_product(pin, p.M, p.N, p.K, tma, name, &plan)) return st;
+    ProductPlan plan = plan_product(p.M, p.N, p.K, tma, element_bytes, info.sm_count, p.dbias != nullptr);
+    if (int st = pin_product(pin, p.M, p.N, p.K, tma, p.dbias != nullptr, name, &plan)) return st;
     p.sum_shares = p.dbias ? sum_shares(plan, p.N, p.K) : 0;
     const size_t parts_bytes = p.dbias ? sum_bytes(plan, p.M, p.N, p.K) : 0;
     const bool fold = parts_bytes != 0;

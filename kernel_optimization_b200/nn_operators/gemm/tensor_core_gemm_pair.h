@@ -15,7 +15,6 @@
 //                the leader's barrier only -- a commit costs the MMA issue stream about 50 ns, a second one per stage
 //                measured 14 % -- and the leader's producer, once it has seen that release, passes it on to the
 //                peer's barrier with a relaxed remote arrive; each producer waits on its own barrier.
-//   arrived[s]   peer only, for the warps that add up columns of A: the leader's pass on what they saw on full[s].
 //   acc_ready[a] one per CTA, two plain commits (shared::cluster addresses) once a tile's MMAs are issued; each CTA's
 //                epilogue warps wait on their own.
 //   acc_free[a]  leader only, 8 arrivals: the four epilogue warps of both CTAs (the peer's arrive remotely).
@@ -140,12 +139,19 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * Cfg::kStages + 5);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     [[maybe_unused]] auto fused_bar = [&](int w) { return bar_base + 8u * (2 * Cfg::kStages + 7 + w); };  // behind the two words above
-    [[maybe_unused]] auto arrived_bar = [&](int s) { return bar_base + 8u * (2 * Cfg::kStages + 7 + Epi::kWarps + s); };
-    static_assert(Epi::kSumWarps == 0 || 8 * (3 * Cfg::kStages + 7 + Epi::kWarps) <= Cfg::kBarrierBytes, "room for the barriers");
+    static_assert(8 * (2 * Cfg::kStages + 7 + Epi::kWarps) <= Cfg::kBarrierBytes, "room for the barriers");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_cta_rank();  // 0 = leader
     const bool leader = rank == 0;
+    // Which half of a tile's rows this CTA holds: the leader the upper one.  With column sums of A the leader alone may add, since
+    // the loads of both CTAs are counted on its barriers only: tiles of odd columns are turned over, so that half the leaders of a
+    // row of tiles hold its upper rows and half its lower ones.
+    auto half_of = [&](int tn) {
+        if constexpr (Epi::kSumWarps != 0)
+            if (p.sum_shares) return (int)rank ^ (tn & 1);
+        return (int)rank;
+    };
     const int tiles_m = (p.M + kTileM - 1) / kTileM, tiles_n = p.tiles_n ? p.tiles_n : (p.N + BN - 1) / BN;
     const int k_blocks = (p.K + kBK - 1) / kBK;
     [[maybe_unused]] const int period = Epi::kPromote ? kPeriod : k_blocks;  // K-blocks that share an accumulator
@@ -167,12 +173,8 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     if (threadIdx.x == 0) {
         for (int s = 0; s < Cfg::kStages; ++s) {
             mbar_init(full_bar(s), 1);
-            if constexpr (Epi::kSumWarps != 0) {
-                mbar_init(empty_bar(s), p.sum_shares ? 1 + Epi::kSumWarps : 1);
-                mbar_init(arrived_bar(s), 1);
-            } else {
-                mbar_init(empty_bar(s), 1);
-            }
+            if constexpr (Epi::kSumWarps != 0) mbar_init(empty_bar(s), p.sum_shares && leader ? 1 + Epi::kSumWarps : 1);
+            else mbar_init(empty_bar(s), 1);
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(acc_ready_bar(a), 1);
@@ -235,7 +237,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                         // A stored [K, M]: this CTA's 128 rows of the tile as two boxes of 64 K-rows x 64 M (MN-major operand)
 #pragma unroll
                         for (int mb = 0; mb < kBM / 64; ++mb)
-                            tma_load_2d_pair(dst + mb * 8192, &map_a, tm * kTileM + (int)rank * kBM + mb * 64, kb * kBK, leader_full);
+                            tma_load_2d_pair(dst + mb * 8192, &map_a, tm * kTileM + half_of(tn) * kBM + mb * 64, kb * kBK, leader_full);
                     } else {
                         tma_load_2d_pair(dst, &map_a, kb * kBK, tm * kTileM + (int)rank * kBM, leader_full);
                     }
@@ -319,25 +321,22 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
         }
         __syncwarp();
     } else if (Epi::kSumWarps != 0 && warp >= 2 + Epi::kWarps) {
-        // ------------------------------------------------------------------ column sums of A (behind the epilogue warps, both CTAs)
+        // ------------------------------------------------------------------ column sums of A (behind the epilogue warps, leader CTA only)
         if constexpr (Epi::kSumWarps != 0) {
             const int box = warp - 2 - Epi::kWarps;  // 64 of the CTA's 128 rows of the product
             uint32_t stage = 0, phase = 0;
             bool ok = true;
-            for (long long u = pair; p.sum_shares && u < num_units && ok; u += pairs) {
+            for (long long u = pair; leader && p.sum_shares && u < num_units && ok; u += pairs) {
                 long long t;
                 int slice, kb0, kb1, tm, tn;
                 unit_of(u, t, slice, kb0, kb1);
                 tile_of(p, t, tiles_m, tiles_n, tm, tn);
-                const bool mine = tn < p.sum_shares;
+                const int turn = tn >> 1;  // among the tiles whose leaders hold these rows
+                const bool mine = turn < p.sum_shares;
                 typename Epi::Sums sums;
-                int next = kb0 + (tn - kb0 % p.sum_shares + p.sum_shares) % p.sum_shares;  // the next K-block that this tile adds
+                int next = kb0 + (turn - kb0 % p.sum_shares + p.sum_shares) % p.sum_shares;  // the next K-block that this tile adds
                 for (int kb = kb0; kb < kb1; ++kb) {
-                    // The pair's loads complete on the leader's barrier; its first sum warp passes the word on.  A token (relaxed):
-                    // what the peer's sum warps read came into their own SM's shared memory before the leader's barrier heard of
-                    // it.  A releasing arrive took 0.7 us a K-block longer, which the whole ring then waited for.
-                    if (!warp_all(mbar_wait_remote(leader ? full_bar(stage) : arrived_bar(stage), phase, abort_flag))) { ok = false; break; }
-                    if (leader && box == 0 && lane == 0) mbar_arrive_cluster_relaxed(map_to_cluster_rank(arrived_bar(stage), 1));
+                    if (!warp_all(mbar_wait(full_bar(stage), phase, abort_flag))) { ok = false; break; }
                     if (mine && kb == next) {
                         sums.add(p, ring + stage * (uint32_t)Cfg::kStageBytes + box * 8192u, lane);
                         next += p.sum_shares;
@@ -346,7 +345,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                     if (lane == 0) mbar_arrive(empty_bar(stage));
                     if (++stage == (uint32_t)Cfg::kStages) { stage = 0; phase ^= 1u; }
                 }
-                if (ok && mine) sums.store(p, slice * p.sum_shares + tn, tm * kTileM + (int)rank * kBM + box * 64, lane);
+                if (ok && mine) sums.store(p, slice * p.sum_shares + turn, tm * kTileM + half_of(tn) * kBM + box * 64, lane);
             }
             if (!ok) {
                 if (lane == 0 && !*abort_flag) atomicCAS(p.status, kStatusOk, kTimeoutEpilogue);
@@ -371,7 +370,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
             unit_of(u, t, slice, kb0, kb1);
             tile_of(p, t, tiles_m, tiles_n, tm, tn);
             column_tile<BN>(p, tn, col0, bn);
-            const int row_base = tm * kTileM + (int)rank * kBM + quad * 32;
+            const int row_base = tm * kTileM + half_of(tn) * kBM + quad * 32;
             if constexpr (Epi::kFused)
                 if (split == 1) Epi::bring(fused, p, row_base, col0 + share * Epi::kChunk);  // while the tile is being computed
             if constexpr (Epi::kPromote) {
@@ -394,7 +393,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                     // a K slice: the partial tile goes to its slot, the slice-sum kernel writes D
                     float *slot = p.partials + ((size_t)t * split + slice) * ((size_t)kTileM * BN);
                     if (row_base < p.M)
-                        publish_block(slot + ((size_t)(((int)rank * 4 + quad) * (BN / 32)) << 10), t_row, bn, lane, share * 32, 8 * Epi::kWarps);
+                        publish_block(slot + ((size_t)((half_of(tn) * 4 + quad) * (BN / 32)) << 10), t_row, bn, lane, share * 32, 8 * Epi::kWarps);
                 } else if (!Epi::template block<kTmaStore>(&map_d, p, fused, t_row, row_base, col0, bn, share * Epi::kChunk, lane, abort_flag)) {
                     if (lane == 0 && !*abort_flag) atomicCAS(p.status, kStatusOk, kTimeoutEpilogue);
                     *abort_flag = 1;

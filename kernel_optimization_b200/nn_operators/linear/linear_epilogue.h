@@ -86,7 +86,8 @@ __device__ __forceinline__ void linear_store_one(const LinearParams &p, float v,
 // Column sums of dY, the bias gradient, by two warps beside the product: dY's tiles lie in shared memory for the matrix
 // instructions anyway, so the sums cost neither the L2 nor DRAM another reading of it.  (A kernel of their own beside or ahead
 // of the product cost 20 us in 147 at 16384 tokens of 4096 features, x 1024.)  All tiles of the same rows of dW see the same dY; the
-// first sum_shares of them take its K-blocks in turn, so that no CTA's shared memory serves much more than the others'.
+// first sum_shares of them (of a pair: of those whose leaders hold the rows) take its K-blocks in turn, so that no CTA's shared memory
+// serves much more than the others'.
 // A warp takes 64 columns, a lane eight of them in every fourth of a K-block's 64 rows; the rows of a K-block are added first,
 // then the K-blocks: chains of 16 and K / 64 FP32 additions.
 struct ColumnSums {

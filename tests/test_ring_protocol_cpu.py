@@ -70,3 +70,19 @@ def test_role_loops_wait_as_a_whole_warp():
         assert waits, name
         for at in waits:
             assert text[:at].endswith("warp_all("), (name, text[at - 40:at + 60])
+
+
+def test_tokens_hand_over_no_data():
+    """A relaxed arrive at another CTA's barrier orders nothing behind it: the one there is gives a stage back to be overwritten.
+    What is read after a wait was counted on that very barrier by the copies, or handed over by a releasing arrive."""
+    import os
+    import re
+
+    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "kernel_optimization_b200")
+    uses = []
+    for folder, _, files in os.walk(root):
+        for name in files:
+            if name.endswith((".h", ".cu")):
+                text = open(os.path.join(folder, name)).read()
+                uses += re.findall(r"mbar_arrive_cluster_relaxed\((?!uint32_t)(.*?)\);", text)
+    assert uses == ["map_to_cluster_rank(empty_bar(s), 1)"]
