@@ -93,7 +93,7 @@ __device__ __forceinline__ void block_allreduce_sums(float (&v)[N], float *scrat
 // Measured (B200, with the kernel that adds the partial rows; copy bandwidth 6447 GB/s): BF16 [32768, 4096] with residual
 // 185 us = 5.80 TB/s (173 us = 4.66 TB/s without: there the instruction slots bind, 70 % of them taken), FP32 [16384, 768]
 // 30 us = 5.0 TB/s of which the second kernel is 3, FP32 [8192, 5120] with residual 103 us = 6.5 TB/s, FP16 [30000, 1001]
-// 62 us = 2.9 TB/s (two-byte loads).
+// 54 us = 3.3 TB/s (two-byte loads).
 constexpr int kBackwardWarpsPerSm = 16;  // at 128 registers a thread
 constexpr int kBackwardMaxStages = 8;
 
@@ -182,11 +182,11 @@ layernorm_backward_resident_kernel(const LayerNormBackwardArgs<T> a, int stages,
             for (int v = 0; v < kVecs; ++v) RowIo<T>::unpack_pairs(raw[v], p + v * (E / 2));
         }
     };
-    // the thread's chunks of a row in global memory; zeros past the row's end
-    auto load = [&](const T *row, f32x2 (&p)[kPairs]) {
+    // the thread's chunks of a row in global memory; zeros past the row's end, or everywhere in a row that is not there
+    auto load = [&](const T *row, bool there, f32x2 (&p)[kPairs]) {
         Raw raw[kVecs];
 #pragma unroll
-        for (int v = 0; v < kVecs; ++v) raw[v] = active[v] ? Chunk::load(row + (t + v * kLanes) * E) : Chunk::zero();
+        for (int v = 0; v < kVecs; ++v) raw[v] = active[v] && there ? Chunk::load(row + (t + v * kLanes) * E) : Chunk::zero();
         unpack(raw, p);
     };
     // the same of a row in the ring, at the address of the thread's first chunk
@@ -252,7 +252,7 @@ layernorm_backward_resident_kernel(const LayerNormBackwardArgs<T> a, int stages,
         for (int i = 0; i < stages && i < steps; ++i) bring(first_row + i * stride, (uint32_t)i);
     // a row's columns past the last one: x = dy = gamma = 0
     if (a.gamma) {
-        load(a.gamma, gamma);
+        load(a.gamma, true, gamma);
     } else {
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) {
@@ -270,13 +270,15 @@ layernorm_backward_resident_kernel(const LayerNormBackwardArgs<T> a, int stages,
     for (int step = 0; step < steps; ++step, r += stride, dx += (size_t)stride * a.cols) {
         const bool there = r < a.rows;
         // Rows past the end are met in the last step only.  Whole warps leave; parts of a warp stay for its shuffles, with
-        // zeros, and store nothing.
-        if (kLanes >= 32 && !there) break;
+        // zeros, and store nothing.  Single elements stay as well, and find their row's address anew at the store: with the early way
+        // out, and the address carried through the loop, the 128 registers do not do (8 bytes spilled; FP16 [30000, 1001] 62.7 us
+        // against 54.5, [30000, 501] 36.2 against 29.5).
+        if (!kSingles && kLanes >= 32 && !there) break;
         f32x2 x[kPairs], dy[kPairs];
         const uint32_t here = my_chunks + stage * stage_bytes;
         if constexpr (kSingles) {
-            load(a.x + (size_t)r * a.cols, x);
-            load(a.dy + (size_t)r * a.cols, dy);
+            load(a.x + (size_t)r * a.cols, there, x);
+            load(a.dy + (size_t)r * a.cols, there, dy);
         } else {
             if (!warp_all(mbar_wait(smem_u32(full + stage), phase, &abort_flag))) give_up(2u);
             staged(here, there, x);
@@ -332,7 +334,7 @@ layernorm_backward_resident_kernel(const LayerNormBackwardArgs<T> a, int stages,
         }
         if (a.residual) {
             f32x2 add[kPairs];
-            if constexpr (kSingles) load(a.residual + (size_t)r * a.cols, add);
+            if constexpr (kSingles) load(a.residual + (size_t)r * a.cols, there, add);
             else staged(here + 2 * tensor_bytes, there, add);
 #pragma unroll
             for (int j = 0; j < kPairs; ++j) x[j] = pair_add(x[j], add[j]);
@@ -345,16 +347,17 @@ layernorm_backward_resident_kernel(const LayerNormBackwardArgs<T> a, int stages,
                 phase ^= 1u;
             }
         }
-        if (kLanes >= 32 || there) {
+        if ((!kSingles && kLanes >= 32) || there) {
+            T *out = kSingles ? a.dx + (size_t)r * a.cols + t : dx;
 #pragma unroll
             for (int v = 0; v < kVecs; ++v)
                 if (active[v]) {
                     if constexpr (kSingles) {
                         float lo, hi;
                         pair_split(x[v / 2], lo, hi);
-                        dx[v * kLanes] = RowIo<T>::from_float(v & 1 ? hi : lo);
+                        out[v * kLanes] = RowIo<T>::from_float(v & 1 ? hi : lo);
                     } else {
-                        Chunk::store(dx + v * kLanes * E, RowIo<T>::pack_pairs(x + v * (E / 2)));
+                        Chunk::store(out + v * kLanes * E, RowIo<T>::pack_pairs(x + v * (E / 2)));
                     }
                 }
         }
