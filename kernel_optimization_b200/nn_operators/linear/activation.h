@@ -167,7 +167,8 @@ __device__ __forceinline__ f32x2 slope_pair(f32x2 z) {
         const f32x2 bend = pair_mul(t, pair_fma(pair_mul(s, both(-1.f)), s, s));
         return pair_fma(bend, pair_fma(both(3.0f * kTwoRoot2OverPi * 0.044715f), t2, both(kTwoRoot2OverPi)), s);
     } else if constexpr (kAct == kActSilu) {
-        const f32x2 t = at_least_pair(z, -41.f), s = logistic_pair(pair_mul(t, both(-kLog2e)));
+        // 1 beyond 20 (to 4e-8); held there, t times the last bit of s, which the common reciprocal may leave below 1, stays 2e-6
+        const f32x2 t = at_most_pair(at_least_pair(z, -41.f), 20.f), s = logistic_pair(pair_mul(t, both(-kLog2e)));
         return pair_mul(s, pair_fma(t, pair_fma(s, both(-1.f), both(1.f)), both(1.f)));
     }
     return both(1.f);

@@ -1,0 +1,88 @@
+"""GPU: the activations of the linear layer and their slopes far out, at infinity, and in every form of the epilogue.
+
+Through an identity weight a pre-activation reaches the epilogue exactly, whatever the form sums: few tokens (up to 32 rows), tiles
+stored by TMA, tiles stored row by row (an output off the 16-byte grid), K slices."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+ACTS = ["none", "relu", "gelu", "gelu_tanh", "silu"]
+CODES = {name: i for i, name in enumerate(ACTS)}
+FORMS = ["few", "tile", "rows", "slices"]
+
+
+def _dtype(torch, kind):
+    return {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}[kind]
+
+
+def _places(torch, form, m, n, odt):
+    """An output of m x n, off the 16-byte grid where the form wants it."""
+    if form != "rows":
+        return torch.full((m, n), float("nan"), dtype=odt, device="cuda")
+    return torch.full((m * n + 1,), float("nan"), dtype=odt, device="cuda")[1:].view(m, n)
+
+
+def _act(torch, lib, z, act, odt, form, bias=None):
+    """act(z + bias) by ko_linear: z times the identity."""
+    fmt = 1 if z.dtype == torch.bfloat16 else 0
+    m, n = z.shape
+    k = 128 if form == "slices" else n      # two slices of 64, the second over zeros
+    x = torch.zeros(m, k, dtype=z.dtype, device="cuda")
+    x[:, :n] = z
+    w = torch.eye(n, k, device="cuda").to(z.dtype)
+    y = _places(torch, form, m, n, odt)
+    ws = torch.empty(1 << 24, dtype=torch.uint8, device="cuda")
+    rows = range(0, m, 32) if form == "few" else (0,)
+    size = y.element_size()
+    for r in rows:
+        part = min(32, m - r) if form == "few" else m
+        status = lib.ko_linear_tuned(fmt, 0 if odt == torch.float32 else fmt + 1, CODES[act], part, n, k, x.data_ptr() + r * k * 2, w.data_ptr(),
+                                     None if bias is None else bias.data_ptr(), None, y.data_ptr() + r * n * size, None, ws.data_ptr(), ws.numel(),
+                                     0 if form == "few" else 128, 2 if form == "slices" else 0, torch.cuda.current_stream().cuda_stream)
+        assert status == 0, lib.ko_last_error_string()
+    return y
+
+
+def _slope(torch, lib, z, act, odt, form):
+    """act'(z) by ko_linear_backward_input: ones times the identity times the slope.  No form for few tokens: it takes the tiles."""
+    fmt = 1 if z.dtype == torch.bfloat16 else 0
+    m, n = z.shape
+    k = 128 if form == "slices" else n
+    dy = torch.zeros(m, k, dtype=z.dtype, device="cuda")
+    dy[:, :n] = 1
+    w = torch.eye(k, n, device="cuda").to(z.dtype)
+    dx = _places(torch, form, m, n, odt)
+    ws = torch.empty(1 << 24, dtype=torch.uint8, device="cuda")
+    assert lib.ko_linear_backward_input_tuned(fmt, 0 if odt == torch.float32 else fmt + 1, CODES[act], m, k, n, dy.data_ptr(), w.data_ptr(), z.data_ptr(),
+                                              dx.data_ptr(), ws.data_ptr(), ws.numel(), 128, 2 if form == "slices" else 0,
+                                              torch.cuda.current_stream().cuda_stream) == 0, lib.ko_last_error_string()
+    return dx
+
+
+def _ordinary(torch, m, n, dtype, seed, scale=1.5):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(m, n, generator=gen, device="cuda") * scale).to(dtype)
+
+
+@pytest.mark.parametrize("form", FORMS[1:])
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("kind,out", [("f16", "f16"), ("bf16", "bf16"), ("bf16", "f32")])
+def test_slopes_far_out_beside_ordinary_values(cuda, lib, kind, out, act, form):
+    """Large z in even and odd columns and rows, whatever their neighbours hold: from 20 on every slope is 1 to within 5e-8, and below -30
+    nothing.  What may be off: at most 20 times the logistic function's own error of 2^-22 (its reciprocal, two roundings), 4.8e-6,
+    and half a step of the type."""
+    dtype, odt = _dtype(cuda, kind), _dtype(cuda, out)
+    far = cuda.tensor([20.0, 33.0, 1e2, 1e3, 2e4, 65504.0] + ([1e6, 1e10, 3e18, 1e30] if kind == "bf16" else []), device="cuda").to(dtype)
+    for sign in (1, -1):
+        if sign < 0:
+            far = far[1:]
+        for r0 in (0, 1):
+            for c0 in (0, 1):
+                z = _ordinary(cuda, 256, 64, dtype, 10 + r0 * 2 + c0)
+                picked = z[r0::2, c0::2]
+                picked.copy_((sign * far).repeat(-(-picked.numel() // len(far)))[:picked.numel()].view(picked.shape))
+                got = _slope(cuda, lib, z, act, odt, form)[r0::2, c0::2].double()
+                want = 1.0 if sign > 0 else 0.0
+                worst = (got - want).abs().max().item()
+                assert worst <= 6e-6 + want * cuda.finfo(odt).eps / 2, (sign, r0, c0, worst)
+    assert lib.ko_poll_device_status() == 0
