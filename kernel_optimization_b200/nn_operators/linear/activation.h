@@ -15,9 +15,9 @@
 //               in Phi up to there, and it falls on below the FP32 range, so a gelu is off by at most 6e-7
 //   its slope   g(-a) = Phi(-a) - a phi(a) = e^(-a^2 / 2) r(a), g(a) = 1 - g(-a), r of degree 8 fitted the same way on [0, 5]
 //               with the weight e^(-a^2 / 2): 1.1e-6
-//   logistic    two reciprocals from one: 1 / u = v / (u v).  Arguments are held above -41 (silu) or where the cubic reaches that
-//               (gelu_tanh: z = -7.4), so that u v stays finite; the results there are 1e-16 in magnitude instead of less
-// Limits are put with max.NaN / min.NaN: a NaN stays one.
+//   logistic    one ex2 and one reciprocal a value; arguments are held above -200 (silu) and -40 (gelu_tanh), where it is 0
+// Limits are put with max.NaN / min.NaN: a NaN stays one.  A value's result depends on nothing but the value: every form of the epilogue
+// gives the same bits for the same sums.
 // Half a step of FP16 is 2.4e-4 of a value.
 #pragma once
 
@@ -33,8 +33,10 @@ constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kTwoRoot2OverPi = 2.0f * 0.79788456080286536f;
 
 // ---- exact forms ----
-__device__ __forceinline__ float logistic_exact(float v) { return 1.0f / (1.0f + expf(-v)); }
-__device__ __forceinline__ float normal_cdf_exact(float z) { return 0.5f * erfcf(-z * 0.70710678118654752f); }
+// (__fmul_rn, __fadd_rn: no contraction with what the library functions begin or end with, so that they give the same bits
+// wherever they are expanded)
+__device__ __forceinline__ float logistic_exact(float v) { return 1.0f / __fadd_rn(1.0f, expf(-v)); }
+__device__ __forceinline__ float normal_cdf_exact(float z) { return 0.5f * erfcf(__fmul_rn(-z, 0.70710678118654752f)); }
 
 template <int kAct>
 __device__ __forceinline__ float activate_exact(float z) {
@@ -92,14 +94,15 @@ __device__ __forceinline__ f32x2 magnitude_pair(f32x2 z, float limit) {
     return pair_of(min_nan(fabsf(a), limit), min_nan(fabsf(b), limit));
 }
 
-// 1 / (1 + 2^x), x = -v log2(e) for the logistic function of v, x <= 62.  (fminf takes the 62 for a NaN, which would reach the
-// other value through the common reciprocal; the callers multiply by what is still a NaN.)
+// 1 / (1 + 2^x), x = -v log2(e) for the logistic function of v; 0 where 2^x is infinite.  Each value has a reciprocal of its own: one for
+// both, 1 / u = v / (u v), makes the last bit of a value depend on which other one it is paired with, and the forms of the epilogue
+// pair columns, rows, or a value with itself.
 __device__ __forceinline__ f32x2 logistic_pair(f32x2 x) {
     float x0, x1, u, v;
     pair_split(x, x0, x1);
-    const f32x2 d = pair_add(pair_of(exp2_approx(fminf(x0, 62.f)), exp2_approx(fminf(x1, 62.f))), both(1.f));
+    const f32x2 d = pair_add(pair_of(exp2_approx(x0), exp2_approx(x1)), both(1.f));
     pair_split(d, u, v);
-    return pair_mul(pair_of(v, u), both(rcp_approx(u * v)));
+    return pair_of(rcp_approx(u), rcp_approx(v));
 }
 // f(-|z|) where z is negative, else 1 - f(-|z|)
 __device__ __forceinline__ f32x2 reflect_pair(f32x2 z, f32x2 low) {
@@ -130,11 +133,11 @@ __device__ __forceinline__ f32x2 activate_pair(f32x2 z) {
         pair_split(z, z0, z1);
         return pair_fma(a, pair_of(-exp2_approx(p0), -exp2_approx(p1)), pair_of(fmaxf(z0, 0.f), fmaxf(z1, 0.f)));
     } else if constexpr (kAct == kActGeluTanh) {
-        const f32x2 t = at_least_pair(z, -7.4f);
+        const f32x2 t = at_least_pair(z, -40.f);
         const f32x2 u = pair_fma(both(-kLog2e * kTwoRoot2OverPi * 0.044715f), pair_mul(t, t), both(-kLog2e * kTwoRoot2OverPi));
         return pair_mul(t, logistic_pair(pair_mul(t, u)));
     } else if constexpr (kAct == kActSilu) {
-        const f32x2 t = at_least_pair(z, -41.f);
+        const f32x2 t = at_least_pair(z, -200.f);
         return pair_mul(t, logistic_pair(pair_mul(t, both(-kLog2e))));
     }
     return z;
@@ -161,14 +164,14 @@ __device__ __forceinline__ f32x2 slope_pair(f32x2 z) {
         return reflect_pair(z, pair_mul(r, pair_of(exp2_approx(e0), exp2_approx(e1))));
     } else if constexpr (kAct == kActGeluTanh) {
         // the slope is 1 beyond 16; held there, z^2 times nothing stays nothing
-        const f32x2 t = at_most_pair(at_least_pair(z, -7.4f), 16.f), t2 = pair_mul(t, t);
+        const f32x2 t = at_most_pair(at_least_pair(z, -40.f), 16.f), t2 = pair_mul(t, t);
         const f32x2 u = pair_fma(both(-kLog2e * kTwoRoot2OverPi * 0.044715f), t2, both(-kLog2e * kTwoRoot2OverPi));
         const f32x2 s = logistic_pair(pair_mul(t, u));
         const f32x2 bend = pair_mul(t, pair_fma(pair_mul(s, both(-1.f)), s, s));
         return pair_fma(bend, pair_fma(both(3.0f * kTwoRoot2OverPi * 0.044715f), t2, both(kTwoRoot2OverPi)), s);
     } else if constexpr (kAct == kActSilu) {
-        // 1 beyond 20 (to 4e-8); held there, t times the last bit of s, which the common reciprocal may leave below 1, stays 2e-6
-        const f32x2 t = at_most_pair(at_least_pair(z, -41.f), 20.f), s = logistic_pair(pair_mul(t, both(-kLog2e)));
+        // 1 beyond 20 (to 4e-8); held there, t times the last bit of s, which the reciprocal may leave below 1, stays 2e-6
+        const f32x2 t = at_most_pair(at_least_pair(z, -200.f), 20.f), s = logistic_pair(pair_mul(t, both(-kLog2e)));
         return pair_mul(s, pair_fma(t, pair_fma(s, both(-1.f), both(1.f)), both(1.f)));
     }
     return both(1.f);

@@ -577,7 +577,7 @@ private:
 #pragma unroll 1
                     for (int j = 0; j < 8; ++j) {
                         const uint4 w = get_piece(piece<128>(d_box, lane, j));
-                        float f[4] = {__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w)}, x[4] = {0.f, 0.f, 0.f, 0.f};
+                        float f[4] = {__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w)}, x[4] = {-0.f, -0.f, -0.f, -0.f};  // what adds nothing
                         if (p.extra) {
                             if constexpr (kExtra16) {
                                 const uint4 e = get_piece(piece<64>(z_box, lane, j >> 1));

@@ -86,3 +86,28 @@ def test_slopes_far_out_beside_ordinary_values(cuda, lib, kind, out, act, form):
                 worst = (got - want).abs().max().item()
                 assert worst <= 6e-6 + want * cuda.finfo(odt).eps / 2, (sign, r0, c0, worst)
     assert lib.ko_poll_device_status() == 0
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("kind,out", [("f16", "f16"), ("bf16", "bf16"), ("f16", "f32"), ("bf16", "f32")])
+def test_every_form_gives_the_same_bits(cuda, lib, kind, out, act):
+    """The same sums make the same results, wherever a value lies and whatever lies beside it."""
+    dtype, odt = _dtype(cuda, kind), _dtype(cuda, out)
+    m, n = 4096, 64
+    z = _ordinary(cuda, m, n, dtype, 5, 4.0)
+    bits = cuda.int32 if odt == cuda.float32 else cuda.int16
+    y = _act(cuda, lib, z, act, odt, "tile")
+    slope = None if act == "none" else _slope(cuda, lib, z, act, odt, "tile")
+    for form in FORMS:
+        got = _act(cuda, lib, z, act, odt, form)
+        assert cuda.equal(got.view(bits) if form != "rows" else got.contiguous().view(bits), y.view(bits)), form
+        if slope is not None and form != "few":
+            assert cuda.equal(_slope(cuda, lib, z, act, odt, form), slope), form
+    # other neighbours, in columns and in rows
+    order = cuda.randperm(m * n, generator=cuda.Generator(device="cuda").manual_seed(1), device="cuda")
+    mixed = z.view(-1)[order].view(m, n).contiguous()
+    for form in FORMS:
+        assert cuda.equal(_act(cuda, lib, mixed, act, odt, form).reshape(-1), y.view(-1)[order]), form
+        if slope is not None and form != "few":
+            assert cuda.equal(_slope(cuda, lib, mixed, act, odt, form).reshape(-1), slope.view(-1)[order]), form
+    assert lib.ko_poll_device_status() == 0
