@@ -16,7 +16,7 @@
 //   its slope   g(-a) = Phi(-a) - a phi(a) = e^(-a^2 / 2) r(a), g(a) = 1 - g(-a), r of degree 8 fitted the same way on [0, 5]
 //               with the weight e^(-a^2 / 2): 1.1e-6
 //   logistic    one ex2 and one reciprocal a value; arguments are held above -200 (silu) and -40 (gelu_tanh), where it is 0
-// Limits are put with max.NaN / min.NaN: a NaN stays one.  A value's result depends on nothing but the value: every form of the epilogue
+// Limits are put with max.NaN / min.NaN: a NaN stays one; an infinity gives the limit, inf or 0, and a slope of 1 or 0.  A value's result depends on nothing but the value: every form of the epilogue
 // gives the same bits for the same sums.
 // Half a step of FP16 is 2.4e-4 of a value.
 #pragma once
@@ -32,40 +32,6 @@ enum Activation : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh =
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kTwoRoot2OverPi = 2.0f * 0.79788456080286536f;
 
-// ---- exact forms ----
-// (__fmul_rn, __fadd_rn: no contraction with what the library functions begin or end with, so that they give the same bits
-// wherever they are expanded)
-__device__ __forceinline__ float logistic_exact(float v) { return 1.0f / __fadd_rn(1.0f, expf(-v)); }
-__device__ __forceinline__ float normal_cdf_exact(float z) { return 0.5f * erfcf(__fmul_rn(-z, 0.70710678118654752f)); }
-
-template <int kAct>
-__device__ __forceinline__ float activate_exact(float z) {
-    if constexpr (kAct == kActRelu) return z < 0.f ? 0.f : z;  // NaN stays NaN
-    if constexpr (kAct == kActGelu) return z * normal_cdf_exact(z);
-    if constexpr (kAct == kActGeluTanh) return z * logistic_exact(z * fmaf(kTwoRoot2OverPi * 0.044715f, z * z, kTwoRoot2OverPi));
-    if constexpr (kAct == kActSilu) return z * logistic_exact(z);
-    return z;
-}
-template <int kAct>
-__device__ __forceinline__ float slope_exact(float z) {
-    if constexpr (kAct == kActRelu) return z > 0.f ? 1.f : 0.f;
-    if constexpr (kAct == kActGelu) return fmaf(z * 0.39894228040143268f, expf(-0.5f * z * z), normal_cdf_exact(z));
-    if constexpr (kAct == kActGeluTanh) {
-        const float s = logistic_exact(z * fmaf(kTwoRoot2OverPi * 0.044715f, z * z, kTwoRoot2OverPi));
-        // s (1 - s) first: 0 for large |z|, where z^2 may be infinite
-        const float bend = s * (1.0f - s);
-        return bend == 0.f ? s : fmaf(z * bend, fmaf(3.0f * kTwoRoot2OverPi * 0.044715f, z * z, kTwoRoot2OverPi), s);
-    }
-    if constexpr (kAct == kActSilu) {
-        const float s = logistic_exact(z);
-        return s * fmaf(z, 1.0f - s, 1.0f);
-    }
-    return 1.f;
-}
-
-// ---- fast forms, two values ----
-__device__ __forceinline__ f32x2 both(float v) { return pair_of(v, v); }
-
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -76,6 +42,54 @@ __device__ __forceinline__ float min_nan(float a, float b) {
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
+
+// ---- exact forms ----
+// (__fmul_rn, __fadd_rn: no contraction with what the library functions begin or end with, so that they give the same bits
+// wherever they are expanded)
+__device__ __forceinline__ float logistic_exact(float v) { return 1.0f / __fadd_rn(1.0f, expf(-v)); }
+__device__ __forceinline__ float normal_cdf_exact(float z) { return 0.5f * erfcf(__fmul_rn(-z, 0.70710678118654752f)); }
+
+// At an infinity the limit: z is held (as far out as where the other factor is 0 or 1 in FP32) wherever it would meet a 0.
+template <int kAct>
+__device__ __forceinline__ float activate_exact(float z) {
+    if constexpr (kAct == kActRelu) return z < 0.f ? 0.f : z;  // NaN stays NaN
+    if constexpr (kAct == kActGelu) {
+        const float t = max_nan(z, -40.f);
+        return t * normal_cdf_exact(t);
+    }
+    if constexpr (kAct == kActGeluTanh) {
+        const float t = max_nan(z, -40.f);
+        return t * logistic_exact(t * fmaf(kTwoRoot2OverPi * 0.044715f, t * t, kTwoRoot2OverPi));
+    }
+    if constexpr (kAct == kActSilu) {
+        const float t = max_nan(z, -200.f);
+        return t * logistic_exact(t);
+    }
+    return z;
+}
+template <int kAct>
+__device__ __forceinline__ float slope_exact(float z) {
+    if constexpr (kAct == kActRelu) return z > 0.f ? 1.f : 0.f;
+    if constexpr (kAct == kActGelu) {
+        const float t = min_nan(max_nan(z, -40.f), 40.f);
+        return fmaf(t * 0.39894228040143268f, expf(-0.5f * t * t), normal_cdf_exact(t));
+    }
+    if constexpr (kAct == kActGeluTanh) {
+        const float s = logistic_exact(z * fmaf(kTwoRoot2OverPi * 0.044715f, z * z, kTwoRoot2OverPi));
+        // s (1 - s) first: 0 for large |z|, where z^2 may be infinite
+        const float bend = s * (1.0f - s);
+        return bend == 0.f ? s : fmaf(z * bend, fmaf(3.0f * kTwoRoot2OverPi * 0.044715f, z * z, kTwoRoot2OverPi), s);
+    }
+    if constexpr (kAct == kActSilu) {
+        const float t = min_nan(max_nan(z, -200.f), 200.f), s = logistic_exact(t);
+        return s * fmaf(t, 1.0f - s, 1.0f);
+    }
+    return 1.f;
+}
+
+// ---- fast forms, two values ----
+__device__ __forceinline__ f32x2 both(float v) { return pair_of(v, v); }
+
 __device__ __forceinline__ f32x2 at_least_pair(f32x2 z, float limit) {
     float a, b;
     pair_split(z, a, b);

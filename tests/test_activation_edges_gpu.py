@@ -88,6 +88,29 @@ def test_slopes_far_out_beside_ordinary_values(cuda, lib, kind, out, act, form):
     assert lib.ko_poll_device_status() == 0
 
 
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("kind,out", [("f16", "f16"), ("bf16", "bf16"), ("f16", "f32"), ("bf16", "f32")])
+def test_infinite_pre_activations(cuda, lib, kind, out, act, form):
+    """The limits, for every type of result: act is inf and 0, its slope 1 and 0.  (FP16 pre-activations become infinite by overflow.)"""
+    dtype, odt = _dtype(cuda, kind), _dtype(cuda, out)
+    m, n = 64, 64
+    inf = float("inf")
+    bias = cuda.zeros(n, device="cuda", dtype=dtype)
+    bias[5::9], bias[2::9] = inf, -inf
+    z = _ordinary(cuda, m, n, dtype, 3)
+    up, down = bias == inf, bias == -inf
+    y = _act(cuda, lib, z, act, odt, form, bias)
+    assert (y[:, up] == inf).all()
+    assert (y[:, down] == (-inf if act == "none" else 0)).all()
+    assert y[:, ~(up | down)].isfinite().all()
+    if form != "few" and act != "none":
+        z = z + bias
+        dx = _slope(cuda, lib, z, act, odt, form)
+        assert (dx[:, up] == 1).all() and (dx[:, down] == 0).all() and dx.isfinite().all()
+    assert lib.ko_poll_device_status() == 0
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("kind,out", [("f16", "f16"), ("bf16", "bf16"), ("f16", "f32"), ("bf16", "f32")])
 def test_every_form_gives_the_same_bits(cuda, lib, kind, out, act):
