@@ -13,8 +13,12 @@
 //   gelu        Phi(-a) = 2^p(a) for a = |z|, Phi(a) = 1 - Phi(-a).  p is log2 Phi(-a), almost a parabola, as a polynomial of
 //               degree 7 (least maximal error on [0, 5.5], found by linear programming on 4000 Chebyshev nodes): 5e-6 relative
 //               in Phi up to there, and it falls on below the FP32 range, so a gelu is off by at most 6e-7
-//   its slope   g(-a) = Phi(-a) - a phi(a) = e^(-a^2 / 2) r(a), g(a) = 1 - g(-a), r of degree 8 fitted the same way on [0, 5]
-//               with the weight e^(-a^2 / 2): 1.1e-6
+//   its slope   g(-a) = Phi(-a) - a phi(a) = e^(-a^2 / 2) r(a), g(a) = 1 - g(-a).  r is of degree 9, fitted on [0, 5.5] by linear
+//               programming (20000 Chebyshev nodes) to an error that is small both ways: 8e-7 of g absolutely and, from a = 2 on, 7.5e-4
+//               of g itself; beyond, g is below 5e-7 and off by less than 1e-9.  So gradients through z = -5 keep their size:
+//               degree 8 with an absolute bound of 1e-6 was off by 8 % at -4.9 and by several times the slope at -6.  Every further
+//               degree costs 1.5 % of a product, which binds on the FMA pipe here (16384 x 1024 x 4096: degree 8 126 us, 10 130; two powers
+//               of 2, good to 1.4e-4 as far as -13, 134)
 //   logistic    one ex2 and one reciprocal a value; arguments are held above -200 (silu) and -40 (gelu_tanh), where it is 0
 // Limits are put with max.NaN / min.NaN: a NaN stays one; an infinity gives the limit, inf or 0, and a slope of 1 or 0.  A value's result depends on nothing but the value: every form of the epilogue
 // gives the same bits for the same sums.
@@ -167,14 +171,15 @@ __device__ __forceinline__ f32x2 slope_pair(f32x2 z) {
         float e0, e1;
         const f32x2 a = magnitude_pair(z, 16.f);  // e^-128 = 0; the polynomial stays finite
         pair_split(pair_mul(pair_mul(a, a), both(-0.5f * kLog2e)), e0, e1);
-        f32x2 r = pair_fma(a, both(3.7967514795e-05f), both(-6.1627244577e-04f));
-        r = pair_fma(a, r, both(4.4045890681e-03f));
-        r = pair_fma(a, r, both(-1.8838131800e-02f));
-        r = pair_fma(a, r, both(5.6169025600e-02f));
-        r = pair_fma(a, r, both(-1.2998859584e-01f));
-        r = pair_fma(a, r, both(2.4928604066e-01f));
-        r = pair_fma(a, r, both(-7.9781925678e-01f));
-        r = pair_fma(a, r, both(4.9999898672e-01f));
+        f32x2 r = pair_fma(a, both(-3.9254905460e-06f), both(9.0380679467e-05f));
+        r = pair_fma(a, r, both(-9.0088939760e-04f));
+        r = pair_fma(a, r, both(5.2183372900e-03f));
+        r = pair_fma(a, r, both(-2.0162180066e-02f));
+        r = pair_fma(a, r, both(5.7404585183e-02f));
+        r = pair_fma(a, r, both(-1.3062055409e-01f));
+        r = pair_fma(a, r, both(2.4944375455e-01f));
+        r = pair_fma(a, r, both(-7.9783397913e-01f));
+        r = pair_fma(a, r, both(4.9999925494e-01f));
         return reflect_pair(z, pair_mul(r, pair_of(exp2_approx(e0), exp2_approx(e1))));
     } else if constexpr (kAct == kActGeluTanh) {
         // the slope is 1 beyond 16; held there, z^2 times nothing stays nothing

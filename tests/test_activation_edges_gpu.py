@@ -134,3 +134,32 @@ def test_every_form_gives_the_same_bits(cuda, lib, kind, out, act):
         if slope is not None and form != "few":
             assert cuda.equal(_slope(cuda, lib, mixed, act, odt, form).reshape(-1), slope.view(-1)[order]), form
     assert lib.ko_poll_device_status() == 0
+
+
+@pytest.mark.parametrize("form", FORMS[1:])
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_small_slopes_keep_their_size(cuda, lib, kind, act, form):
+    """Slopes of 16-bit gradients where they vanish: off by 8e-4 of themselves (GELU's fit 7.4e-4, its nine FP32 steps 2e-5, the rest of
+    the arithmetic 2^-20) and half a step of the type -- not by a fixed amount that is more than the slope."""
+    import math
+
+    dtype = _dtype(cuda, kind)
+    lowest = {"gelu": -5.5, "gelu_tanh": -6.0, "silu": -80.0}[act]
+    if kind == "f16":       # the slope is to stay a normal FP16 number
+        lowest = {"gelu": -4.5, "gelu_tanh": -4.0, "silu": -11.0}[act]
+    z = cuda.linspace(lowest, -3.0, 256 * 64, device="cuda").to(dtype).view(256, 64)
+    z = z.reshape(-1)[cuda.randperm(z.numel(), generator=cuda.Generator(device="cuda").manual_seed(2), device="cuda")].view(256, 64).contiguous()
+    t = z.double()
+    c = math.sqrt(2.0 / math.pi)
+    if act == "gelu":
+        want = 0.5 * cuda.special.erfc(-t * math.sqrt(0.5)) + t * cuda.exp(-t * t / 2) * (0.5 * c)
+    else:
+        u = 2 * c * (t + 0.044715 * t ** 3) if act == "gelu_tanh" else t
+        du = 2 * c * (1 + 3 * 0.044715 * t ** 2) if act == "gelu_tanh" else 1.0
+        s = cuda.sigmoid(u)
+        want = s + t * s * cuda.sigmoid(-u) * du
+    got = _slope(cuda, lib, z, act, dtype, form).double()
+    half = cuda.finfo(dtype).eps / 2
+    worst = ((got - want).abs() / want.abs()).max().item()
+    assert worst <= 8e-4 + half * (1 + 8e-4), worst
