@@ -20,8 +20,8 @@ int check_linear(const char *name, int in_fmt, int out_fmt, int activation, int6
 
 namespace {
 
-template <bool kBf16, bool kOut16, int kTiles, int kSlabs, int kWarps>
-int launch_few_tokens(const ko::FewTokensParams &q, const ko::DeviceInfo &info, cudaStream_t s) {
+template <bool kBf16, bool kOut16, bool kPromote, int kTiles, int kSlabs, int kWarps>
+int launch_few_tokens_as(const ko::FewTokensParams &q, const ko::DeviceInfo &info, cudaStream_t s) {
     constexpr int kChunks = 4;
     const long long groups = ((long long)q.p.N + 16 * kSlabs - 1) / (16 * kSlabs);
     // Blocks share a stretch of W rows, each with its part of K, while that leaves at most four blocks per SM and every warp
@@ -30,8 +30,15 @@ int launch_few_tokens(const ko::FewTokensParams &q, const ko::DeviceInfo &info, 
     unsigned cluster = 1;
     while (cluster < 8 && groups * cluster * 2 <= 4LL * info.sm_count && (long long)cluster * 2 * kWarps * 32 * kChunks <= q.p.K) cluster *= 2;
     KO_REQUIRE(groups * cluster <= 0x7fffffffLL, KO_ERR_SHAPE, "linear: %lld blocks exceed the grid limit", groups * cluster);
-    return ko::launch_clustered_overlapped(ko::linear_few_tokens_kernel<kBf16, kOut16, kTiles, kSlabs, kChunks, kWarps>,
+    return ko::launch_clustered_overlapped(ko::linear_few_tokens_kernel<kBf16, kOut16, kPromote, kTiles, kSlabs, kChunks, kWarps>,
                                            (unsigned)(groups * cluster), 32u * kWarps, cluster, 0, s, q);
+}
+// a warp's accumulators take as much of K of a 16-bit result as a tile's (less where blocks share it)
+template <bool kBf16, bool kOut16, int kTiles, int kSlabs, int kWarps>
+int launch_few_tokens(const ko::FewTokensParams &q, const ko::DeviceInfo &info, cudaStream_t s) {
+    if (!kOut16 || q.p.K > ko::blocks_in_one_accumulator(true) * 64 * kWarps)
+        return launch_few_tokens_as<kBf16, kOut16, true, kTiles, kSlabs, kWarps>(q, info, s);
+    return launch_few_tokens_as<kBf16, kOut16, !kOut16, kTiles, kSlabs, kWarps>(q, info, s);
 }
 // Up to 16 tokens, and whenever K is short, 16 rows of W a block and eight warps; beyond, 32 rows, so that a token's
 // fragments serve two slabs, and four warps (32 x 4096 x 4096: 11.8 against 14.8 us, 20 x 2000 x 8192 11.3 against 15.1;

@@ -213,16 +213,11 @@ int run_product(LinearParams p, const void *A, const void *B, void *workspace, s
         if (p.extra)
             if (int st = make_store_map(encode, &p.map_extra, Epi::kExtra16 ? p.fmt + 1 : 0, const_cast<void *>(p.extra), p.M, p.N, Epi::kChunk)) return st;
     }
-    // FP32 results of more than 1024 values of K a work unit: partial sums are promoted (see LinearEpilogue)
+    // long sums: those of parts are promoted (see LinearEpilogue)
     const long long unit_blocks = ((p.K + tc::kBK - 1) / tc::kBK + plan.split - 1) / plan.split;
-    const bool promote = !kOut16 && unit_blocks > 16;
-    int st = KO_OK;
-    if constexpr (!kOut16) {
-        if (promote) st = launch_product<LinearEpilogue<kMode, false, true>>(plan, tma, map_a, map_b, map_d, p, info.sm_count, s);
-        else st = launch_product<Epi>(plan, tma, map_a, map_b, map_d, p, info.sm_count, s);
-    } else {
-        st = launch_product<Epi>(plan, tma, map_a, map_b, map_d, p, info.sm_count, s);
-    }
+    const int st = unit_blocks > blocks_in_one_accumulator(kOut16)
+                       ? launch_product<LinearEpilogue<kMode, kOut16, true>>(plan, tma, map_a, map_b, map_d, p, info.sm_count, s)
+                       : launch_product<Epi>(plan, tma, map_a, map_b, map_d, p, info.sm_count, s);
     if (st != KO_OK) return st;
     if constexpr (kMode == LinearMode::kWeightGrad)
         if (fold && plan.split == 1) return launch_overlapped(linear_fold_sums_kernel<256>, (unsigned)((p.M + 255) / 256), 256u, (size_t)0, s, p);

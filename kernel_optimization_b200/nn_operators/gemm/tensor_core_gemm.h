@@ -49,7 +49,6 @@ constexpr int kBM = 128;          // rows of D per tile = TMEM lanes
 constexpr int kBK = 64;           // K elements per stage: 64 * 2 B = one 128-byte swizzle row
 constexpr int kUmmaK = 16;        // K per tcgen05.mma for 16-bit inputs
 constexpr int kThreads = 192;     // 6 warps: producer, MMA, 4 x epilogue
-constexpr int kPeriod = 14;       // K-blocks per accumulator where partial sums are promoted (896 values of K)
 
 // codes written to the status word (first failure wins)
 enum : unsigned { kStatusOk = 0, kTimeoutProducer = 1, kTimeoutMma = 2, kTimeoutEpilogue = 3, kTimeoutDrain = 4 };
@@ -276,7 +275,8 @@ struct PlainEpilogue {
     static constexpr int kWarps = 4;  // epilogue warps, a multiple of 4: each quadrant of TMEM lanes is shared by kWarps / 4
     static constexpr bool kTransA = false;
     static constexpr bool kFused = false;
-    static constexpr bool kPromote = false; // true: partial sums of kPeriod K-blocks are added outside the tensor cores (see there)
+    static constexpr bool kPromote = false;  // true: partial sums of kPeriod K-blocks are added outside the tensor cores (see there)
+    static constexpr int kPeriod = 0;
     static constexpr int kSumWarps = 0;  // warps that add up the columns of A as stored (kTransA), beside the product
 };
 
@@ -534,7 +534,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int tiles_m = (p.M + kTileM - 1) / kTileM, tiles_n = p.tiles_n ? p.tiles_n : (p.N + BN - 1) / BN;
     const int k_blocks = (p.K + kBK - 1) / kBK;
-    [[maybe_unused]] const int period = Epi::kPromote ? kPeriod : k_blocks;  // K-blocks that share an accumulator
+    [[maybe_unused]] const int period = Epi::kPromote ? Epi::kPeriod : k_blocks;  // K-blocks that share an accumulator
     // work units: (tile, K slice), the slices of a tile next to each other so that they run at the same time
     const int split = p.split_k > 1 ? p.split_k : 1;
     const long long num_units = (long long)tiles_m * tiles_n * split;
@@ -759,8 +759,8 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 if (!kTmaStore && split == 1) Epi::bring_rows(fused, p, tm * kTileM + quad * 32, col0 + share * Epi::kChunk, lane);
             }
             if constexpr (Epi::kPromote) {
-                const int periods = (kb1 - kb0 + kPeriod - 1) / kPeriod;
-                ok = Epi::template promote<BN, false>(tmem_base + ((uint32_t)(quad * 32) << 16), share, periods, local_tile, acc_ready_bar(0),
+                const int periods = (kb1 - kb0 + Epi::kPeriod - 1) / Epi::kPeriod;
+                ok = Epi::template promote<BN, false>(tmem_base + ((uint32_t)(quad * 32) << 16), share, Epi::kChunk == 64 && split == 1, periods, local_tile, acc_ready_bar(0),
                                                       acc_free_bar(0), abort_flag);
                 local_tile += (uint32_t)periods - 1;  // the accumulator that holds the sums
             }

@@ -154,7 +154,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
     };
     const int tiles_m = (p.M + kTileM - 1) / kTileM, tiles_n = p.tiles_n ? p.tiles_n : (p.N + BN - 1) / BN;
     const int k_blocks = (p.K + kBK - 1) / kBK;
-    [[maybe_unused]] const int period = Epi::kPromote ? kPeriod : k_blocks;  // K-blocks that share an accumulator
+    [[maybe_unused]] const int period = Epi::kPromote ? Epi::kPeriod : k_blocks;  // K-blocks that share an accumulator
     const long long pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     // work units as in the single-CTA kernel; only fused epilogues are given K slices
     const int split = Epi::kFused && p.split_k > 1 ? p.split_k : 1;
@@ -374,8 +374,8 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
             if constexpr (Epi::kFused)
                 if (split == 1) Epi::bring(fused, p, row_base, col0 + share * Epi::kChunk);  // while the tile is being computed
             if constexpr (Epi::kPromote) {
-                const int periods = (kb1 - kb0 + kPeriod - 1) / kPeriod;
-                ok = Epi::template promote<BN, true>(tmem_base + ((uint32_t)(quad * 32) << 16), share, periods, local_tile, acc_ready_bar(0),
+                const int periods = (kb1 - kb0 + Epi::kPeriod - 1) / Epi::kPeriod;
+                ok = Epi::template promote<BN, true>(tmem_base + ((uint32_t)(quad * 32) << 16), share, Epi::kChunk == 64 && split == 1, periods, local_tile, acc_ready_bar(0),
                                                      map_to_cluster_rank(acc_free_bar(0), 0), abort_flag);
                 local_tile += (uint32_t)periods - 1;  // the accumulator that holds the sums
             }

@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kBlock) linear_fold_sums_kernel(const LinearPa
     if (row < p.M) p.dbias[row] = fold_sum_parts(p, row);
 }
 
-// kPromote (FP32 results of more than 1024 values of K): the tensor cores cut their accumulator off at every addition instead of
+// kPromote (FP32 results of more than 1024 values of K, 16-bit ones of more than 16384, see blocks_in_one_accumulator): the tensor cores cut their accumulator off at every addition instead of
 // rounding it, so an error grows with K on the side of smaller magnitudes -- 4.5e-6 of the result (2-norm) at K = 4096, 1.9e-5 at
 // 16384, where a blocked FP32 sum is off by 6e-7 and 1.5e-6.  A tile is then taken in periods of 896 values of K, each into the
 // other of the two accumulators, and the epilogue warps add the periods' sums, rounded to nearest, in registers (128 a thread for a
@@ -167,13 +167,19 @@ __global__ void __launch_bounds__(kBlock) linear_fold_sums_kernel(const LinearPa
 // 1024 dW: 101 us either way).  With several the total holds one of the accumulators while it is being stored, and the next
 // tile gets no further than a period meanwhile: 4096^3 to FP32 101 -> 145 us.  (Storing from the registers instead spilled them: 206 with periods of 1024;
 // periods of 512, too short for the additions: 204.)
+// K-blocks of 64 that one accumulator may take.  16-bit results: what is cut off stays below a sixteenth of half a step of FP16, 2^-15, up to
+// 16384 values of K (terms of one sign: 2^-25 of the result for each of K / 16 instructions).  In one accumulator over 400000
+// positive terms FP16 results were off by more than a step; their periods are of 8192 (dW of 65536 tokens, 2048 x 2048, to BF16
+// 366 -> 383 us, most of it the operand stage that the further epilogue warps' boxes take; with periods of 896 422).
+constexpr int blocks_in_one_accumulator(bool out16) { return out16 ? 256 : 16; }
+
 template <LinearMode kMode, bool kOut16, bool kPromoteSums = false>
 struct LinearEpilogue {
     using Params = LinearParams;
     static constexpr bool kTransA = kMode == LinearMode::kWeightGrad;
     static constexpr bool kPromote = kPromoteSums;
+    static constexpr int kPeriod = kOut16 ? 128 : 14;  // K-blocks of an accumulator: 896 values of K, or 8192
     static constexpr int kWarps = kTransA && !kPromote ? 4 : 8;
-    static_assert(!kPromote || !kOut16, "what is rounded to 16 bits does not show it");
     static constexpr bool kFused = true;
     static constexpr int kSumWarps = kTransA ? 2 : 0;  // 64 columns of dY each, see ColumnSums
     using Sums = ColumnSums;
@@ -193,24 +199,26 @@ struct LinearEpilogue {
 
     // The promoted sums of a tile's `periods` accumulators, the first of them number `first` of the CTA's sequence: all but the
     // last are added up in registers -- this warp's 32 rows of the chunks share * 32, share * 32 + 64, ... -- and given
-    // back; the last receives the total, for the rest of the epilogue to find there.  t_rows: TMEM address of the warp's
+    // back; the last receives the total, for the rest of the epilogue to find there.  wide: the chunks are those of a 16-bit result, 64
+    // columns from share * 64, from there + 128 and so on.  t_rows: TMEM address of the warp's
     // rows in accumulator 0; ready, free: the accumulators' mbarriers (free as a shared::cluster address where the MMAs are
     // issued by another CTA).  False when a wait ran out.  A function of its own, so that its registers and those of the
     // code around it do not add up.
     template <int BN, bool kRemote>
-    __device__ __noinline__ static bool promote(uint32_t t_rows, int share, int periods, uint32_t first, uint32_t ready, uint32_t free,
+    __device__ __noinline__ static bool promote(uint32_t t_rows, int share, bool wide, int periods, uint32_t first, uint32_t ready, uint32_t free,
                                                 volatile int *abort_flag) {
         constexpr int kChunks = BN / 64;
         f32x2 sums[kChunks][16];
         for (uint32_t n = first; n < first + (uint32_t)periods; ++n) {
-            const uint32_t acc = n & 1u, t_row = t_rows + acc * BN + share * 32;
+            const uint32_t acc = n & 1u, t_row = t_rows + acc * BN + share * (wide ? 64 : 32);
             if (!warp_all(mbar_wait(ready + 8u * acc, (n >> 1) & 1u, abort_flag))) return false;
             tc::tc_fence_after();
             const bool last = n + 1 == first + (uint32_t)periods;
 #pragma unroll
             for (int j = 0; j < kChunks; ++j) {
                 float f[32];
-                tc::tmem_ld_32x32(t_row + j * 64, f);
+                const uint32_t at = t_row + (wide ? (j >> 1) * 128 + (j & 1) * 32 : j * 64);
+                tc::tmem_ld_32x32(at, f);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const f32x2 part = pair_of(f[2 * i], f[2 * i + 1]);
@@ -219,7 +227,7 @@ struct LinearEpilogue {
                 if (last) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) pair_split(sums[j][i], f[2 * i], f[2 * i + 1]);
-                    tc::tmem_st_32x32(t_row + j * 64, f);
+                    tc::tmem_st_32x32(at, f);
                 }
             }
             if (last) {

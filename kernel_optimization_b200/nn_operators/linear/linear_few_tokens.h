@@ -44,8 +44,8 @@ struct FewTokensParams {
     const void *X, *W;
 };
 
-// kTiles: token tiles of 8; kChunks: 32-wide pieces of K a warp loads together
-template <bool kBf16, bool kOut16, int kTiles, int kSlabs, int kChunks, int kWarps>
+// kTiles: token tiles of 8; kChunks: 32-wide pieces of K a warp loads together; kPromote: for FP32 results, and 16-bit ones of long sums
+template <bool kBf16, bool kOut16, bool kPromote, int kTiles, int kSlabs, int kChunks, int kWarps>
 __global__ void __launch_bounds__(32 * kWarps) linear_few_tokens_kernel(const __grid_constant__ FewTokensParams q) {
     const LinearParams &p = q.p;
     constexpr int kRows = 16 * kSlabs, kCols = 8 * kTiles;
@@ -88,9 +88,9 @@ __global__ void __launch_bounds__(32 * kWarps) linear_few_tokens_kernel(const __
                     if (first + c * 32 < p.K) asm volatile("prefetch.global.L2 [%0];" ::"l"(w_row[s][h] + first + c * 32));
     grid_dependency_wait();
     const int stride = ranks * kWarps * 32 * kChunks;
-    // An FP32 result is not to show how the matrix instructions cut their accumulators off (see LinearEpilogue): every 1024 values of
+    // A result is not to show how the matrix instructions cut their accumulators off (see LinearEpilogue): every 1024 values of
     // K a warp adds them to sums of its own.
-    float sum[kOut16 ? 1 : kSlabs][kOut16 ? 1 : kTiles][4] = {};
+    float sum[kPromote ? kSlabs : 1][kPromote ? kTiles : 1][4] = {};
     int pieces = 0;
     for (int k0 = first; k0 < p.K; k0 += stride) {
         uint4 w[kChunks][kSlabs][2], x[kChunks][kTiles];
@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(32 * kWarps) linear_few_tokens_kernel(const __
                     mma_16x8x16<kBf16>(acc[s][i], w[c][s][0].x, w[c][s][1].x, w[c][s][0].y, w[c][s][1].y, x[c][i].x, x[c][i].y);
                     mma_16x8x16<kBf16>(acc[s][i], w[c][s][0].z, w[c][s][1].z, w[c][s][0].w, w[c][s][1].w, x[c][i].z, x[c][i].w);
                 }
-        if constexpr (!kOut16) {
+        if constexpr (kPromote) {
             if (++pieces == 1024 / (32 * kChunks)) {
                 pieces = 0;
 #pragma unroll
@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(32 * kWarps) linear_few_tokens_kernel(const __
         for (int i = 0; i < kTiles; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                part[warp][s * 16 + (e >> 1) * 8 + g][i * 8 + 2 * t + (e & 1)] = kOut16 ? acc[s][i][e] : sum[s * !kOut16][i * !kOut16][e] + acc[s][i][e];
+                part[warp][s * 16 + (e >> 1) * 8 + g][i * 8 + 2 * t + (e & 1)] = kPromote ? sum[s * kPromote][i * kPromote][e] + acc[s][i][e] : acc[s][i][e];
     __syncthreads();
     // element i of the block: token i / kRows, W row i % kRows (stores of a token's outputs are then contiguous)
     for (int i = threadIdx.x; i < kRows * kCols; i += 32 * kWarps) {
