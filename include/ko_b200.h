@@ -171,7 +171,8 @@ int ko_layernorm_f16(const uint16_t *in, uint16_t *out, int64_t rows, int32_t co
  * nothing.  `residual` is the gradient that reaches x past the norm (the skip connection of a pre-norm
  * block).  FP32 arithmetic; dx is rounded once to the element type; dgamma and dbeta are FP32 [cols],
  * overwritten, and may each be NULL.  Column sums are added in a fixed order: the same call gives the same
- * bits.  dx may be the same buffer as dy, x or residual; other overlaps are not allowed.
+ * bits.  dx may be the same buffer as dy, x or residual; other overlaps are not allowed.  Addresses are
+ * multiples of the element's size; rows on the 16-byte grid are fastest.
  * `workspace`: device memory of ko_layernorm_backward_workspace(...) bytes for this shape (16-byte aligned,
  * contents irrelevant before and after), used by this call only: calls that may overlap on the GPU, and
  * captured graphs that may be replayed at the same time, need one each.  Nothing is allocated or kept, so
@@ -312,8 +313,8 @@ int ko_gemm_tc(int in_fmt, int out_fmt, int b_row_major, int64_t M, int64_t N, i
  * even once.  FP32 results use the CUDA library's erfcf / expf; for 16-bit results the activations are accurate to
  * about 1e-6 absolutely before that rounding.  An infinite pre-activation (FP16's beyond 65504) gives the limit: inf or 0, a slope of
  * 1 or 0; a NaN stays one.
- * Row pitches must be multiples of 16 bytes: K % 8 == 0, and N % 8 == 0 in the backward calls (the forward call takes
- * any N); X, W and dY 16-byte aligned.  Any M: up to 32 tokens the forward call runs a kernel that streams W, beyond
+ * Row pitches must be multiples of 16 bytes: K % 8 == 0 (K >= 8 in the forward call), and N % 8 == 0 in the backward calls
+ * (N >= 8 for dX; the forward call takes any N); X, W and dY 16-byte aligned.  Any M: up to 32 tokens the forward call runs a kernel that streams W, beyond
  * that tiles on tcgen05.  Y may be the residual, dX (16-bit) may be Z, dW may be C; other overlaps are not allowed.
  * An activation in ko_linear_backward_input needs Z; without one (KO_ACT_NONE) Z is ignored.
  * `workspace`: as for ko_layernorm_backward_*; ko_linear_*_workspace gives the bytes for a shape (often 0, then it may

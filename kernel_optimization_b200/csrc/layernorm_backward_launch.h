@@ -10,7 +10,6 @@
 namespace ko {
 namespace ln_backward {
 
-
 // How a call is cut up.
 struct Plan {
     int row_chunks;      // blocks along the rows = partial rows
@@ -139,6 +138,9 @@ int dispatch(int dtype, const T *dy, const T *x, T *dx, int64_t rows, int32_t co
         return KO_OK;
     }
     KO_REQUIRE(dy != nullptr && x != nullptr && dx != nullptr, KO_ERR_INVALID_ARG, "layernorm backward: NULL pointer");
+    for (const T *p : {dy, x, (const T *)dx, gamma, residual})
+        KO_REQUIRE(ko::aligned_to(p, sizeof(T)), KO_ERR_ALIGN, "layernorm backward: an operand is not aligned to its element");
+    KO_REQUIRE(ko::aligned_to(dgamma, 4) && ko::aligned_to(dbeta, 4), KO_ERR_ALIGN, "layernorm backward: dgamma and dbeta must be aligned to 4 bytes");
     KO_REQUIRE(dgamma == nullptr || dgamma != dbeta, KO_ERR_INVALID_ARG, "layernorm backward: dgamma and dbeta must not be the same buffer");
     ko::DeviceInfo info;
     if (int st = ko::current_device_info(&info)) return st;

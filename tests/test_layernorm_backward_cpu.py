@@ -32,3 +32,18 @@ def test_wrapper_refuses_host_tensors_and_wrong_ranks(ko):
         ko.layernorm_backward(x[0], x[0], 1e-5)
     with pytest.raises(ValueError):
         ko.layernorm_backward(x.double(), x.double(), 1e-5)
+
+
+@pytest.mark.parametrize("entry,size", [("f32", 4), ("f16", 2), ("bf16", 2)])
+def test_addresses_between_elements(lib, entry, size):
+    """Refused before any CUDA call: the kernels would load and store across element boundaries, which the hardware does not do."""
+    p = 1 << 20   # made-up addresses, never dereferenced
+
+    def call(dy=p, x=2 * p, dx=3 * p, gamma=None, residual=None, dgamma=None, dbeta=None):
+        return getattr(lib, f"ko_layernorm_backward_{entry}")(dy, x, dx, 4, 16, 1e-5, gamma, residual, dgamma, dbeta, 0, 4 * p, 1 << 20, None)
+
+    for name, at in (("dy", p), ("x", 2 * p), ("dx", 3 * p), ("gamma", 5 * p), ("residual", 6 * p)):
+        for off in range(1, size):
+            assert call(**{name: at + off}) == 2 and b"aligned" in lib.ko_last_error_string(), (name, off)
+    for off in (1, 2, 3):
+        assert call(dgamma=7 * p + off) == 2 and call(dbeta=7 * p + off) == 2
