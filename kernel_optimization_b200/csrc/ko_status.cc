@@ -1,23 +1,24 @@
 // Status strings, thread-local last-error text and the per-device property cache.
 #include "ko_internal.h"
 
+#include <cstring>
 #include <mutex>
-#include <string>
 
 namespace ko {
 namespace {
-thread_local std::string g_last_error;
+constexpr size_t kErrorBytes = 512;
+thread_local char g_last_error[kErrorBytes];
 std::mutex g_info_mutex;
 DeviceInfo g_info[64];
 }  // namespace
 
 int fail(int status, const char *fmt, ...) {
-    char buf[512];
+    char buf[kErrorBytes];  // an argument may be the text of the last error
     va_list ap;
     va_start(ap, fmt);
     std::vsnprintf(buf, sizeof buf, fmt, ap);
     va_end(ap);
-    g_last_error = buf;
+    std::memcpy(g_last_error, buf, sizeof buf);
     return status;
 }
 
@@ -49,6 +50,7 @@ int current_device_info(DeviceInfo *out) {
 }
 }  // namespace ko
 
+#include <exception>
 #include <map>
 #include <utility>
 
@@ -60,11 +62,15 @@ int ensure_dynamic_smem(const void *kernel, size_t bytes) {
     static std::map<std::pair<const void *, int>, size_t> configured;
     int dev = 0;
     KO_CUDA(cudaGetDevice(&dev));
-    std::lock_guard<std::mutex> lock(mu);
-    size_t &have = configured[{kernel, dev}];
-    if (bytes > have) {
-        KO_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-        have = bytes;
+    try {
+        std::lock_guard<std::mutex> lock(mu);
+        size_t &have = configured[{kernel, dev}];
+        if (bytes > have) {
+            KO_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+            have = bytes;
+        }
+    } catch (const std::exception &e) {  // the callers are C entry points
+        return fail(KO_ERR_CUDA, "recording a kernel's shared memory: %s", e.what());
     }
     return KO_OK;
 }
@@ -85,7 +91,7 @@ const char *ko_status_string(int status) {
     }
 }
 
-const char *ko_last_error_string(void) { return ko::g_last_error.c_str(); }
+const char *ko_last_error_string(void) { return ko::g_last_error; }
 
 int ko_version(void) { return 100; /* 0.1.0 */ }
 

@@ -6,9 +6,7 @@
 #include "tensor_maps.h"
 
 #include <algorithm>
-#include <map>
-#include <mutex>
-#include <utility>
+#include <atomic>
 
 #include "../nn_operators/gemm/tensor_core_gemm_pair.h"
 #include "../nn_operators/linear/linear_epilogue.h"
@@ -114,18 +112,13 @@ inline size_t product_workspace(int64_t M, int64_t N, int64_t K, int sms, bool s
     return most;
 }
 
-// clusters of two CTAs of a pair kernel that the current device holds at once (cached per kernel and device)
-inline int resident_pairs_of(const void *kernel, unsigned threads, size_t smem, int *out) {
-    static std::mutex mu;
-    static std::map<std::pair<const void *, int>, int> cached;
-    int dev = 0;
-    KO_CUDA(cudaGetDevice(&dev));
-    std::lock_guard<std::mutex> lock(mu);
-    int &n = cached[{kernel, dev}];
+// clusters of two CTAs of a pair kernel that the current device holds at once; `cached`: per device, 0 = not asked yet (whoever asks at the
+// same time gets the same answer)
+inline int resident_pairs_of(const void *kernel, unsigned threads, size_t smem, int device, std::atomic<int> *cached, int *out) {
+    int n = cached[device].load(std::memory_order_relaxed);
     if (n == 0) {
-        int fresh = 0;
-        if (int st = max_resident_clusters(kernel, threads, 2, smem, &fresh)) return st;
-        n = fresh;
+        if (int st = max_resident_clusters(kernel, threads, 2, smem, &n)) return st;
+        cached[device].store(n, std::memory_order_relaxed);
     }
     *out = n;
     return KO_OK;
@@ -142,14 +135,15 @@ int launch_product_tile(const CUtensorMap &ma, const CUtensorMap &mb, const CUte
 }
 
 template <class Epi>
-int launch_product_pair(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &md, const LinearParams &p, cudaStream_t s) {
+int launch_product_pair(const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &md, const LinearParams &p, const DeviceInfo &info, cudaStream_t s) {
     using Cfg = typename tc::PairConfigFor<Epi>::type;
     auto kernel = tc::gemm_tcgen05_pair_kernel<true, Epi>;
     const void *id = reinterpret_cast<const void *>(kernel);
     constexpr unsigned threads = 64u + 32u * (Epi::kWarps + Epi::kSumWarps);
     if (int st = ensure_dynamic_smem(id, Cfg::kSmemBytes)) return st;
+    static std::atomic<int> cached[64];  // device ordinals, see current_device_info
     int resident = 0;
-    if (int st = resident_pairs_of(id, threads, Cfg::kSmemBytes, &resident)) return st;
+    if (int st = resident_pairs_of(id, threads, Cfg::kSmemBytes, info.device, cached, &resident)) return st;
     const long long units = (long long)((p.M + 255) / 256) * ((p.N + 255) / 256) * p.split_k;
     return launch_clustered_overlapped(kernel, 2u * (unsigned)std::min<long long>(units, resident), threads, 2u, (size_t)Cfg::kSmemBytes, s, ma,
                                        mb, mb, md, p);
@@ -160,8 +154,9 @@ int launch_product_pair(const CUtensorMap &ma, const CUtensorMap &mb, const CUte
 // Everything has been checked but the workspace.
 template <class Epi>
 int launch_product(const ProductPlan &plan, bool tma, const CUtensorMap &ma, const CUtensorMap &mb, const CUtensorMap &md, const LinearParams &p,
-                   int sms, cudaStream_t s) {
-    if (plan.pair) return launch_product_pair<Epi>(ma, mb, md, p, s);
+                   const DeviceInfo &info, cudaStream_t s) {
+    const int sms = info.sm_count;
+    if (plan.pair) return launch_product_pair<Epi>(ma, mb, md, p, info, s);
     if (!tma) return launch_product_tile<Epi, 128, false>(ma, mb, md, p, sms, s);
     if (plan.bn == 128) return launch_product_tile<Epi, 128, true>(ma, mb, md, p, sms, s);
     return launch_product_tile<Epi, 256, true>(ma, mb, md, p, sms, s);
@@ -216,8 +211,8 @@ int run_product(LinearParams p, const void *A, const void *B, void *workspace, s
     // long sums: those of parts are promoted (see LinearEpilogue)
     const long long unit_blocks = ((p.K + tc::kBK - 1) / tc::kBK + plan.split - 1) / plan.split;
     const int st = unit_blocks > blocks_in_one_accumulator(kOut16)
-                       ? launch_product<LinearEpilogue<kMode, kOut16, true>>(plan, tma, map_a, map_b, map_d, p, info.sm_count, s)
-                       : launch_product<Epi>(plan, tma, map_a, map_b, map_d, p, info.sm_count, s);
+                       ? launch_product<LinearEpilogue<kMode, kOut16, true>>(plan, tma, map_a, map_b, map_d, p, info, s)
+                       : launch_product<Epi>(plan, tma, map_a, map_b, map_d, p, info, s);
     if (st != KO_OK) return st;
     if constexpr (kMode == LinearMode::kWeightGrad)
         if (fold && plan.split == 1) return launch_overlapped(linear_fold_sums_kernel<256>, (unsigned)((p.M + 255) / 256), 256u, (size_t)0, s, p);
