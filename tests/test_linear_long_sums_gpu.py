@@ -72,7 +72,7 @@ def test_few_tokens_of_many_features(cuda, lib, ko, kind, m):
 
 
 @pytest.mark.parametrize("m", [1, 8, 13, 20, 32])
-@pytest.mark.parametrize("k", [4096, 16384])
+@pytest.mark.parametrize("k", [4096, 16384, 131072])
 def test_fp32_results_for_few_tokens(cuda, ko, m, k):
     """A warp takes an eighth or a quarter of K, in pieces of 128, and puts its accumulators aside every 1024 values (64 instructions):
     terms of one sign, so each is off by 2^-25 of the accumulator on average, 32 * 2^-24 of the result.  Of K / 4 values in one
@@ -82,3 +82,27 @@ def test_fp32_results_for_few_tokens(cuda, ko, m, k):
     got = ko.linear(x, w, out_dtype=cuda.float32)
     off = ((got.double() - want) / want).abs().mean().item()
     assert off <= (32 + 8) * 2.0 ** -24, off * 2 ** 24
+
+
+@pytest.mark.parametrize("n,k", [(256, 512), (1032, 264), (2048, 2048), (250, 1001)])
+def test_fp32_results_take_short_periods(cuda, lib, ko, n, k):
+    """Terms of either sign.  A cut takes 0.36 * 2^-23 of the accumulator on average (half a unit of the last place, over mantissas), the
+    accumulator is two thirds of a period's sum in size (it grows with the root of the terms), and the cuts go against its sign: at most
+    0.24 * 2^-23 of the sum for each instruction of a period, which does not average out over periods.  With 56 instructions, 896 terms,
+    1.6e-6 of the result's 2-norm; the periods' additions are rounded, and 2^-24 of each averages out.  Periods of 2048 terms would be
+    off by more than twice as much."""
+    m = 16384
+    bound = 0.24 * 56 * 2.0 ** -23 + (m / 896) ** 0.5 * 2.0 ** -24
+
+    def off(got, want):
+        return ((got.double() - want).norm() / want.norm()).item()
+
+    gen = cuda.Generator(device="cuda").manual_seed(n + k)
+    a = cuda.randn(n, m, generator=gen, device="cuda").bfloat16()
+    w = cuda.randn(k, m, generator=gen, device="cuda").bfloat16()
+    want = a.double() @ w.double().t()
+    assert off(ko.linear(a, w, out_dtype=cuda.float32), want) <= bound
+    if n % 8 == 0:
+        assert off(ko.linear_backward_weight(a.t().contiguous(), w.t().contiguous(), return_bias=False), want) <= bound
+        assert off(ko.linear_backward_input(a, w.t().contiguous(), out_dtype=cuda.float32), want) <= bound
+    assert lib.ko_poll_device_status() == 0
