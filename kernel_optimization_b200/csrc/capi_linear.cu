@@ -100,6 +100,8 @@ int ko_linear(int in_fmt, int out_fmt, int activation, int64_t M, int64_t N, int
 
 int ko_linear_tuned(int in_fmt, int out_fmt, int activation, int64_t M, int64_t N, int64_t K, const void *X, const void *W, const void *bias,
                     const void *residual, void *Y, void *Z, void *workspace, size_t workspace_bytes, int tile, int slices, void *stream) {
+    KO_REQUIRE(tile == 0 || tile == 128 || tile == 256 || tile == 2048, KO_ERR_INVALID_ARG, "linear: tile code %d not in {128,256,2048}", tile);
+    KO_REQUIRE(slices == 0 || tile != 0, KO_ERR_INVALID_ARG, "linear: slices need a tile code");
     return linear_dispatch(in_fmt, out_fmt, activation, M, N, K, X, W, bias, residual, Y, Z, workspace, workspace_bytes, stream, {tile, slices});
 }
 

@@ -56,3 +56,14 @@ def test_wrappers_refuse_host_tensors(ko):
                  lambda: ko.linear(x[0], w), lambda: ko.linear(x, w, activation="swish"), lambda: ko.linear(x.double(), w.double())):
         with pytest.raises(ValueError):
             call()
+
+
+def test_pinned_plans(lib):
+    """Slices without a tile are refused for any number of tokens, few ones included, which no plan would have used them for."""
+    def call(m, tile, slices):
+        return lib.ko_linear_tuned(1, 2, 0, m, 64, 256, P, 2 * P, None, None, 3 * P, None, None, 0, tile, slices, None)
+
+    for m in (4, 64):
+        assert call(m, 0, 2) == 1 and b"slices" in lib.ko_last_error_string()
+        assert call(m, 64, 0) == 1 and b"tile code" in lib.ko_last_error_string()
+    assert lib.ko_linear_backward_weight_tuned(1, 0, 64, 64, 64, P, 2 * P, None, 3 * P, None, None, 0, 0, 2, None) == 1
