@@ -87,7 +87,8 @@ inline int pin_product(const PinnedPlan &pin, int64_t M, int64_t N, int64_t K, b
 // Tiles of a row of tiles that share the column sums of dY (see ColumnSums): one, whose sums are dbias, or four, whose parts
 // have to be added.  One that takes all K-blocks falls behind the others (a K-block's sums take longer than its MMAs in the 128 x 128
 // tile), adding parts is a launch, 1.2 us of the device, where K is not cut anyway.  One / four, without the sums (us): 777 tokens of
-// 1000 x 520 9.6 / 10.9, 9.5; 1024 tokens of 1024 x 1024 10.4 / 10.2, 8.7; 2048 tokens 16.7 / 14.2, 12.4; 16384 of 4096 x 1024 121 / 107, 105.
+// 1000 x 520 9.6 / 10.9, 9.5; 1024 tokens of 1024 x 1024 10.4 / 10.2, 8.7; 2048 tokens 16.7 / 14.2, 12.4; in
+// pairs, 16384 of 4096 x 1024, 104 with the two shares that four columns of tiles give, 103.
 // Of a pair of CTAs only the leader adds, the upper rows of its tile in even columns of tiles and the lower ones in odd columns: two
 // columns of tiles for every share.
 inline int sum_shares(const ProductPlan &plan, int64_t N, int64_t K) {

@@ -91,7 +91,7 @@ __device__ __forceinline__ void block_allreduce_sums(float (&v)[N], float *scrat
 // reductions' shuffles over many elements.
 //
 // Measured (B200, with the kernel that adds the partial rows; copy bandwidth 6447 GB/s): BF16 [32768, 4096] with residual
-// 185 us = 5.80 TB/s (173 us = 4.66 TB/s without: there the instruction slots bind, 70 % of them taken), FP32 [16384, 768]
+// 190 us = 5.64 TB/s (177 us = 4.55 TB/s without: there the instruction slots bind, 70 % of them taken), FP32 [16384, 768]
 // 30 us = 5.0 TB/s of which the second kernel is 3, FP32 [8192, 5120] with residual 103 us = 6.5 TB/s, FP16 [30000, 1001]
 // 54 us = 3.3 TB/s (two-byte loads).
 constexpr int kBackwardWarpsPerSm = 16;  // at 128 registers a thread

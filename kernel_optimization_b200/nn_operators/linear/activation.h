@@ -17,8 +17,8 @@
 //               programming (20000 Chebyshev nodes) to an error that is small both ways: 8e-7 of g absolutely and, from a = 2 on, 7.5e-4
 //               of g itself; beyond, g is below 5e-7 and off by less than 1e-9.  So gradients through z = -5 keep their size:
 //               degree 8 with an absolute bound of 1e-6 was off by 8 % at -4.9 and by several times the slope at -6.  Every further
-//               degree costs 1.5 % of a product, which binds on the FMA pipe here (16384 x 1024 x 4096: degree 8 126 us, 10 130; two powers
-//               of 2, good to 1.4e-4 as far as -13, 134)
+//               degree costs 1.5 % of a product (16384 x 1024 x 4096: degree 8 125 us, 9 127, 10 130; Phi and phi apart, two powers of 2,
+//               good to 1.4e-4 as far as -13, 134)
 //   logistic    one ex2 and one reciprocal a value; arguments are held above -200 (silu) and -40 (gelu_tanh), where it is 0
 // Limits are put with max.NaN / min.NaN: a NaN stays one; an infinity gives the limit, inf or 0, and a slope of 1 or 0.  A value's result depends on nothing but the value: every form of the epilogue
 // gives the same bits for the same sums.

@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(kBlock) linear_fold_sums_kernel(const LinearPa
 // other of the two accumulators, and the epilogue warps add the periods' sums, rounded to nearest, in registers (128 a thread for a
 // tile 256 columns wide) while the next period is being multiplied: 9e-7 at any K.  Hidden where a CTA has one tile (16384 x 4096 x
 // 1024 dW: 101 us either way).  With several the total holds one of the accumulators while it is being stored, and the next
-// tile gets no further than a period meanwhile: 4096^3 to FP32 101 -> 145 us.  (Storing from the registers instead spilled them: 206 with periods of 1024;
+// tile gets no further than a period meanwhile: 4096^3 to FP32 101 -> 135 .. 145 us.  (Storing from the registers instead spilled them: 206 with periods of 1024;
 // periods of 512, too short for the additions: 204.)
 // K-blocks of 64 that one accumulator may take.  16-bit results: what is cut off stays below a sixteenth of half a step of FP16, 2^-15, up to
 // 16384 values of K (terms of one sign: 2^-25 of the result for each of K / 16 instructions).  In one accumulator over 400000
