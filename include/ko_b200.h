@@ -311,11 +311,11 @@ int ko_gemm_tc(int in_fmt, int out_fmt, int b_row_major, int64_t M, int64_t N, i
  * C[N,K] and dbias may be NULL.  bias and Z have the inputs' type; dbias is FP32; residual and Y, dX, C and dW
  * are FP32 (out_fmt 0) or the inputs' type (out_fmt 1 for FP16, 2 for BF16): the FP32 result is rounded to nearest
  * even once.  FP32 results use the CUDA library's erfcf / expf; for 16-bit results the activations are accurate to
- * about 1e-6 absolutely before that rounding.  An infinite pre-activation (FP16's beyond 65504) gives the limit: inf or 0, a slope of
- * 1 or 0; a NaN stays one.
+ * about 1e-6 absolutely before that rounding.  An infinite pre-activation (FP16's beyond 65504) gives the limit: inf or
+ * 0, a slope of 1 or 0; a NaN stays one.
  * Row pitches must be multiples of 16 bytes: K % 8 == 0 (K >= 8 in the forward call), and N % 8 == 0 in the backward calls
- * (N >= 8 for dX; the forward call takes any N); X, W and dY 16-byte aligned.  Any M: up to 32 tokens the forward call runs a kernel that streams W, beyond
- * that tiles on tcgen05.  Y may be the residual, dX (16-bit) may be Z, dW may be C; other overlaps are not allowed.
+ * (N >= 8 for dX; the forward call takes any N); X, W and dY 16-byte aligned.  Any M: up to 32 tokens the forward call
+ * runs a kernel that streams W, beyond that tiles on tcgen05.  Y may be the residual, dX (16-bit) may be Z, dW may be C; other overlaps are not allowed.
  * An activation in ko_linear_backward_input needs Z; without one (KO_ACT_NONE) Z is ignored.
  * `workspace`: as for ko_layernorm_backward_*; ko_linear_*_workspace gives the bytes for a shape (often 0, then it may
  * be NULL).  Nothing is allocated or kept, every call can be captured.  All sums have a fixed order: the same call

@@ -760,8 +760,8 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             }
             if constexpr (Epi::kPromote) {
                 const int periods = (kb1 - kb0 + Epi::kPeriod - 1) / Epi::kPeriod;
-                ok = Epi::template promote<BN, false>(tmem_base + ((uint32_t)(quad * 32) << 16), share, Epi::kChunk == 64 && split == 1, periods, local_tile, acc_ready_bar(0),
-                                                      acc_free_bar(0), abort_flag);
+                ok = Epi::template promote<BN, false>(tmem_base + ((uint32_t)(quad * 32) << 16), share, Epi::kChunk == 64 && split == 1, periods,
+                                                      local_tile, acc_ready_bar(0), acc_free_bar(0), abort_flag);
                 local_tile += (uint32_t)periods - 1;  // the accumulator that holds the sums
             }
             const uint32_t acc = MT == 1 ? (local_tile & 1u) : 0u, acc_phase = (MT == 1 ? (local_tile >> 1) : local_tile) & 1u;

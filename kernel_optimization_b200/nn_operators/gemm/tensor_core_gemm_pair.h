@@ -375,8 +375,8 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid
                 if (split == 1) Epi::bring(fused, p, row_base, col0 + share * Epi::kChunk);  // while the tile is being computed
             if constexpr (Epi::kPromote) {
                 const int periods = (kb1 - kb0 + Epi::kPeriod - 1) / Epi::kPeriod;
-                ok = Epi::template promote<BN, true>(tmem_base + ((uint32_t)(quad * 32) << 16), share, Epi::kChunk == 64 && split == 1, periods, local_tile, acc_ready_bar(0),
-                                                     map_to_cluster_rank(acc_free_bar(0), 0), abort_flag);
+                ok = Epi::template promote<BN, true>(tmem_base + ((uint32_t)(quad * 32) << 16), share, Epi::kChunk == 64 && split == 1, periods,
+                                                     local_tile, acc_ready_bar(0), map_to_cluster_rank(acc_free_bar(0), 0), abort_flag);
                 local_tile += (uint32_t)periods - 1;  // the accumulator that holds the sums
             }
             const uint32_t acc = local_tile & 1u, acc_phase = (local_tile >> 1) & 1u;

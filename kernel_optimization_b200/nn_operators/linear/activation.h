@@ -15,13 +15,13 @@
 //               in Phi up to there, and it falls on below the FP32 range, so a gelu is off by at most 6e-7
 //   its slope   g(-a) = Phi(-a) - a phi(a) = e^(-a^2 / 2) r(a), g(a) = 1 - g(-a).  r is of degree 9, fitted on [0, 5.5] by linear
 //               programming (20000 Chebyshev nodes) to an error that is small both ways: 8e-7 of g absolutely and, from a = 2 on, 7.5e-4
-//               of g itself; beyond, g is below 5e-7 and off by less than 1e-9.  So gradients through z = -5 keep their size:
+//               of g itself; beyond, g is below 6e-7 and off by at most 1.1e-9.  So gradients through z = -5 keep their size:
 //               degree 8 with an absolute bound of 1e-6 was off by 8 % at -4.9 and by several times the slope at -6.  Every further
 //               degree costs 1.5 % of a product (16384 x 1024 x 4096: degree 8 125 us, 9 127, 10 130; Phi and phi apart, two powers of 2,
 //               good to 1.4e-4 as far as -13, 134)
 //   logistic    one ex2 and one reciprocal a value; arguments are held above -200 (silu) and -40 (gelu_tanh), where it is 0
-// Limits are put with max.NaN / min.NaN: a NaN stays one; an infinity gives the limit, inf or 0, and a slope of 1 or 0.  A value's result depends on nothing but the value: every form of the epilogue
-// gives the same bits for the same sums.
+// Limits are put with max.NaN / min.NaN: a NaN stays one; an infinity gives the limit, inf or 0, and a slope of 1 or 0.  A value's
+// result depends on nothing but the value: every form of the epilogue gives the same bits for the same sums.
 // Half a step of FP16 is 2.4e-4 of a value.
 #pragma once
 

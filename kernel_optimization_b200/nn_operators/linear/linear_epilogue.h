@@ -159,18 +159,18 @@ __global__ void __launch_bounds__(kBlock) linear_fold_sums_kernel(const LinearPa
     if (row < p.M) p.dbias[row] = fold_sum_parts(p, row);
 }
 
-// kPromote (FP32 results of more than 1024 values of K, 16-bit ones of more than 16384, see blocks_in_one_accumulator): the tensor cores cut their accumulator off at every addition instead of
-// rounding it, so an error grows with K on the side of smaller magnitudes -- 4.5e-6 of the result (2-norm) at K = 4096, 1.9e-5 at
-// 16384, where a blocked FP32 sum is off by 6e-7 and 1.5e-6.  A tile is then taken in periods of 896 values of K, each into the
-// other of the two accumulators, and the epilogue warps add the periods' sums, rounded to nearest, in registers (128 a thread for a
-// tile 256 columns wide) while the next period is being multiplied: 9e-7 at any K.  Hidden where a CTA has one tile (16384 x 4096 x
-// 1024 dW: 101 us either way).  With several the total holds one of the accumulators while it is being stored, and the next
-// tile gets no further than a period meanwhile: 4096^3 to FP32 101 -> 135 .. 145 us.  (Storing from the registers instead spilled them: 206 with periods of 1024;
-// periods of 512, too short for the additions: 204.)
-// K-blocks of 64 that one accumulator may take.  16-bit results: what is cut off stays below a sixteenth of half a step of FP16, 2^-15, up to
-// 16384 values of K (terms of one sign: 2^-25 of the result for each of K / 16 instructions).  In one accumulator over 400000
-// positive terms FP16 results were off by more than a step; their periods are of 8192 (dW of 65536 tokens, 2048 x 2048, to BF16
-// 366 -> 383 us, most of it the operand stage that the further epilogue warps' boxes take; with periods of 896 422).
+// kPromote (FP32 results of more than 1024 values of K, 16-bit ones of more than 16384): the tensor cores cut their accumulator off
+// at every addition instead of rounding it, so an error grows with K on the side of smaller magnitudes -- 4.5e-6 of the result
+// (2-norm) at K = 4096, 1.9e-5 at 16384, where a blocked FP32 sum is off by 6e-7 and 1.5e-6.  A tile is then taken in periods of 896
+// values of K, each into the other of the two accumulators, and the epilogue warps add the periods' sums, rounded to nearest, in
+// registers (128 a thread for a tile 256 columns wide) while the next period is being multiplied: 9e-7 at any K.  Hidden where a CTA
+// has one tile (16384 x 4096 x 1024 dW: 101 us either way).  With several the total holds one of the accumulators while it is being
+// stored, and the next tile gets no further than a period meanwhile: 4096^3 to FP32 101 -> 135 .. 145 us.  (Storing from the registers
+// instead spilled them: 206 with periods of 1024; periods of 512, too short for the additions: 204.)
+// K-blocks of 64 that one accumulator may take.  16-bit results: what is cut off stays below a sixteenth of half a step of FP16,
+// 2^-15, up to 16384 values of K (terms of one sign: 2^-25 of the result for each of K / 16 instructions).  In one accumulator over
+// 400000 positive terms FP16 results were off by more than a step.  Their periods are of 8192 (dW of 65536 tokens, 2048 x 2048, to
+// BF16 366 -> 383 us; with periods of 896 422).
 constexpr int blocks_in_one_accumulator(bool out16) { return out16 ? 256 : 16; }
 
 template <LinearMode kMode, bool kOut16, bool kPromoteSums = false>
